@@ -61,6 +61,7 @@ extern "C" {
 #define ASRFE_DT_F32 0
 #define ASRFE_DT_BF16 1
 #define ASRFE_DT_F16 2
+#define ASRFE_DT_E4M3 3 /* storage of a key / value cache only: OCP e4m3 bytes under power-of-two scales (asrfe_kv_cache) */
 
 /* Threading.  A context is immutable once its tables and weights are loaded: asrfe_fbank, asrfe_lfr_cmvn,
  * asrfe_frontend and asrfe_encoder_forward only enqueue kernels on the caller's stream and may be called from
@@ -285,6 +286,87 @@ int32_t asrfe_vad_forward(asrfe_ctx* ctx, const float* feats, const int32_t* len
  * 10 log10(sum over the frame's 400 samples of x^2 + 1e-6) with x in [-1, 1]; 0 for rows past a clip's frames. */
 int32_t asrfe_frame_decibel(asrfe_ctx* ctx, const void* pcm, int32_t pcm_dtype, int64_t pcm_stride, const int32_t* pcm_lens,
                             int32_t batch, int32_t t_max, float* decibel, void* stream);
+
+/* ---- a paged cache of keys and values, the attention of new positions over it, and the choice of a token ------------
+ * No counterpart in the reference's own code: it configures a streaming recogniser with look-back (chunk [0, 4, 5],
+ * encoder look-back 4, decoder look-back 1: voice-service/app/services/voice_interface.py:651-653) and leaves the call
+ * commented out (:1753-1809).  These are the operators a streaming or autoregressive model needs next to the batch
+ * encoder: sessions share one pool of pages, a step appends its new positions, attends over the session's pages and
+ * chooses a token.  None of them needs loaded weights; the context carries the device and the error text.
+ *
+ * A batch of n_tokens packed rows holds the new positions of `batch` sequences: rows cu_q[b] .. cu_q[b + 1] - 1 are
+ * sequence b's (cu_q [batch + 1] int32, cu_q[0] = 0, not decreasing; rows at and past cu_q[batch] belong to nobody and
+ * are neither read nor written).  kv_lens[b] (int32) counts the positions of sequence b including its new ones, which
+ * are the last: row t of sequence b is position kv_lens[b] - cu_q[b + 1] + t (a negative position, from more new rows
+ * than positions, is not stored and sees nothing).  Position p lives in row p % page_size of page
+ * block_table[b * table_stride + p / page_size]; positions past table_stride pages do not exist.  A page number outside
+ * 0 .. n_pages - 1 (-1 for a page that was given back) is a page of which nothing is stored, read or seen. */
+typedef struct asrfe_kv_cache {
+    void* k;                 /* [n_pages][n_heads][page_size][head_dim], 16-byte aligned; dtype F16, BF16 or E4M3 */
+    void* v;                 /* the same for the values */
+    uint8_t* k_exp;          /* E4M3: [n_pages][n_heads][page_size], a stored value is code * 2^(exp - 127); else NULL */
+    uint8_t* v_exp;
+    int32_t n_pages;
+    int32_t page_size;       /* 16, 32, 64, 128 or 256 positions */
+    int32_t n_heads;         /* key / value heads, 1 .. 256 */
+    int32_t head_dim;        /* 64 or 128 */
+    int32_t dtype;           /* ASRFE_DT_F16, ASRFE_DT_BF16 or ASRFE_DT_E4M3 */
+} asrfe_kv_cache;
+
+/* Writes the new rows' keys and values into their pages.  k, v: rows of head_dim elements of `dtype` (F16 or BF16: the
+ * cache's own type, any of the two for an E4M3 cache), element (t, h, d) at t * token_stride + h * head_stride + d
+ * (strides in elements, multiples of 8; bases 16-byte aligned), so slices of one fused projection can be passed as they
+ * are.  16-bit caches get the elements as they are.  E4M3 caches get, per row and head, the exponent e = the least
+ * integer >= -126 with max |x| <= 448 * 2^e over the finite elements (0 where all are zero), stored as e + 127, and the
+ * codes round-to-nearest-even(x * 2^-e); an infinity is stored as +-448, a NaN as NaN.  Two rows for one place (a page
+ * shared by two sequences that both append to it) leave either. */
+int32_t asrfe_kv_append(asrfe_ctx* ctx, const asrfe_kv_cache* cache, const void* k, const void* v, int32_t dtype,
+                        int64_t k_token_stride, int64_t k_head_stride, int64_t v_token_stride, int64_t v_head_stride,
+                        int32_t n_tokens, const int32_t* cu_q, const int32_t* kv_lens, const int32_t* block_table,
+                        int32_t table_stride, int32_t batch, void* stream);
+
+/* Reads positions 0 .. t_max - 1 of every sequence back: k, v [batch][t_max][n_heads][head_dim] dense, of `dtype` (as in
+ * asrfe_kv_append; 16-byte aligned).  Positions at and past kv_lens[b], and those of pages that do not exist, are zero.
+ * Every e4m3 code under its scale is exact in bf16 and, inside its range, in fp16 (beyond it: +-65504). */
+int32_t asrfe_kv_read(asrfe_ctx* ctx, const asrfe_kv_cache* cache, const int32_t* kv_lens, const int32_t* block_table,
+                      int32_t table_stride, int32_t batch, int32_t t_max, void* k, void* v, int32_t dtype, void* stream);
+
+/* Attention of the new rows over the cache: out[t][h] = sum_j p_j v_j, p = softmax_j(scale * q[t][h] . k_j) over the
+ * positions j the row sees, h's keys being those of cache head h / (n_q_heads / n_heads).  A row at position i sees j <
+ * kv_lens[b] with j <= i (causal != 0), and, where window > 0, j > i - window or j < sinks.  A row that sees nothing is
+ * zero.  What a row does not see has no influence on it, infinities and NaN in hidden keys or values included (a visible
+ * value that is infinite counts as long as its weight does not vanish in 16 bits).  The caller's new positions have to be in the cache
+ * already (asrfe_kv_append on the same stream).  q, out: elements (t, h, d) at t * token_stride + h * head_stride + d,
+ * strides multiples of 8, bases 16-byte aligned, of `dtype` (F16 or BF16; the cache's own for a 16-bit cache).
+ * n_q_heads: a multiple of n_heads.  max_kv: an upper bound of kv_lens (it shapes the launch; positions past it are not
+ * seen).  Scores, softmax statistics and sums are fp32; the weights p enter their product in `dtype`.
+ * workspace: >= asrfe_paged_attention_workspace_bytes(...) of the same numbers, 256-byte aligned, of this call alone
+ * until it has run (a captured graph keeps using the one it was captured with). */
+int64_t asrfe_paged_attention_workspace_bytes(const asrfe_ctx* ctx, const asrfe_kv_cache* cache, int32_t n_tokens,
+                                              int32_t n_q_heads, int32_t batch, int32_t max_kv);
+int32_t asrfe_paged_attention(asrfe_ctx* ctx, const asrfe_kv_cache* cache, const void* q, int32_t dtype,
+                              int64_t q_token_stride, int64_t q_head_stride, int32_t n_tokens, int32_t n_q_heads,
+                              const int32_t* cu_q, const int32_t* kv_lens, const int32_t* block_table,
+                              int32_t table_stride, int32_t batch, int32_t max_kv, int32_t window, int32_t sinks,
+                              int32_t causal, float scale, void* out, int64_t out_token_stride, int64_t out_head_stride,
+                              void* workspace, int64_t workspace_bytes, void* stream);
+
+/* One token per row of logits [rows][vocab] (row stride ld elements, dtype F32, F16 or BF16), in the place of the arg-max
+ * of asrfe_decoder_forward.  With w_i = exp((l_i - max l) / temperature): order the vocabulary by falling logit, equal
+ * ones by rising index; keep the first top_k (top_k <= 0 or >= vocab: all); of those the shortest prefix whose weights
+ * sum to at least top_p of theirs (top_p >= 1: all); of those the ones with w_i >= min_p; always the first.  ids[r] is
+ * the lowest index at which the running sum of the kept weights, in the order of the vocabulary, exceeds u[r] times
+ * their sum (u in [0, 1)), logprobs[r] (optional) the logarithm of its share of that sum.  temperature, top_k, top_p,
+ * min_p, u: one per row; each of the first four may be NULL (1, all, all, all).  A temperature that is not above zero
+ * takes the first of the order (the arg-max).  NaN logits count as -inf, and a -inf logit is never chosen; where a row
+ * holds +inf logits, they share all the weight.  A row with nothing above -inf gives 0 and logprob -inf.  token_num
+ * [rows / rows_per] (optional): rows r with r % rows_per >= token_num[r / rows_per] get -1 and logprob 0 (rows behind an
+ * utterance's tokens, as asrfe_decoder_forward marks them).  Weights are formed and summed with errors below 1e-9 and
+ * the sums do not depend on the order of execution: the same call gives the same bits. */
+int32_t asrfe_sample_tokens(asrfe_ctx* ctx, const void* logits, int32_t dtype, int64_t ld, int32_t rows, int32_t vocab,
+                            const float* u, const float* temperature, const int32_t* top_k, const float* top_p,
+                            const float* min_p, const int32_t* token_num, int32_t rows_per, int32_t* ids,
+                            float* logprobs, void* stream);
 
 /* asrfe_encoder_forward for callers that cannot allocate device memory (code under HIP graph capture, tight serving
  * loops, harnesses that forbid hipMalloc): no workspace argument.  No counterpart in the reference.  The scratch is a

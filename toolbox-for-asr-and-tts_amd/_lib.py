@@ -13,7 +13,7 @@ _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(_HERE, "libasrfe.so")
 
 PCM_I16, PCM_F32, PCM_F32_WIRE = 0, 1, 2
-DT_F32, DT_BF16, DT_F16 = 0, 1, 2
+DT_F32, DT_BF16, DT_F16, DT_E4M3 = 0, 1, 2, 3
 
 ERROR_NAMES = {
     0: "OK",
@@ -101,6 +101,20 @@ class VadConfig(C.Structure):
     ]
 
 
+class KvCache(C.Structure):
+    _fields_ = [
+        ("k", C.c_void_p),
+        ("v", C.c_void_p),
+        ("k_exp", C.c_void_p),
+        ("v_exp", C.c_void_p),
+        ("n_pages", C.c_int32),
+        ("page_size", C.c_int32),
+        ("n_heads", C.c_int32),
+        ("head_dim", C.c_int32),
+        ("dtype", C.c_int32),
+    ]
+
+
 PROF_KINDS = ["fbank", "frontend", "lfr_cmvn", "pe_table", "layernorm", "gemm_qkv", "fsmn", "attention", "gemm_out",
               "gemm_ffn1", "gemm_ffn2", "post_attn"]
 
@@ -161,6 +175,20 @@ SIGNATURES = {
                                       C.c_void_p, C.c_int64, C.c_void_p]),
     "asrfe_frame_decibel": (C.c_int32, [C.c_void_p, C.c_void_p, C.c_int32, C.c_int64, C.c_void_p, C.c_int32, C.c_int32,
                                         C.c_void_p, C.c_void_p]),
+    "asrfe_kv_append": (C.c_int32, [C.c_void_p, C.POINTER(KvCache), C.c_void_p, C.c_void_p, C.c_int32, C.c_int64, C.c_int64,
+                                    C.c_int64, C.c_int64, C.c_int32, C.c_void_p, C.c_void_p, C.c_void_p, C.c_int32, C.c_int32,
+                                    C.c_void_p]),
+    "asrfe_kv_read": (C.c_int32, [C.c_void_p, C.POINTER(KvCache), C.c_void_p, C.c_void_p, C.c_int32, C.c_int32, C.c_int32,
+                                  C.c_void_p, C.c_void_p, C.c_int32, C.c_void_p]),
+    "asrfe_paged_attention_workspace_bytes": (C.c_int64, [C.c_void_p, C.POINTER(KvCache), C.c_int32, C.c_int32, C.c_int32,
+                                                          C.c_int32]),
+    "asrfe_paged_attention": (C.c_int32, [C.c_void_p, C.POINTER(KvCache), C.c_void_p, C.c_int32, C.c_int64, C.c_int64, C.c_int32,
+                                          C.c_int32, C.c_void_p, C.c_void_p, C.c_void_p, C.c_int32, C.c_int32, C.c_int32,
+                                          C.c_int32, C.c_int32, C.c_int32, C.c_float, C.c_void_p, C.c_int64, C.c_int64,
+                                          C.c_void_p, C.c_int64, C.c_void_p]),
+    "asrfe_sample_tokens": (C.c_int32, [C.c_void_p, C.c_void_p, C.c_int32, C.c_int64, C.c_int32, C.c_int32, C.c_void_p, C.c_void_p,
+                                        C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p, C.c_int32, C.c_void_p, C.c_void_p,
+                                        C.c_void_p]),
     "asrfe_host_mel_banks": (C.c_int32, [C.POINTER(Config), C.POINTER(C.c_double)]),
     "asrfe_host_window": (C.c_int32, [C.POINTER(Config), C.POINTER(C.c_double)]),
     "asrfe_profile_begin": (C.c_int32, [C.c_void_p, C.c_int32]),

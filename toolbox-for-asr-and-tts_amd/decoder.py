@@ -16,6 +16,7 @@ import numpy as np
 import torch
 
 from . import _lib
+from .sampling import sample_tokens
 
 SOS, EOS, BLANK = 1, 2, 0
 FRAME_MS = 60  # one encoder frame: lfr_n (6) frames of 10 ms
@@ -79,18 +80,25 @@ class ParaformerHead:
         return ptr, self._ws.numel() - (ptr - self._ws.data_ptr())
 
     def forward(self, encoder_out: torch.Tensor, encoder_out_lens, n_max: int | None = None, return_logits: bool = False,
-                return_alphas: bool = False, return_fire_frames: bool = False):
+                return_alphas: bool = False, return_fire_frames: bool = False, sampling: dict | None = None):
         """encoder_out [B, T', 512] float32 on the device, lens [B] -> dict with ``token_ids`` [B, n_max] int32 (-1 behind
         an utterance's tokens), ``token_num`` [B] int32, ``embeds`` [B, n_max, 512], and on request ``logits``
         [B, n_max, vocab], ``alphas`` [B, T' + 1] and ``fire_frames`` [B, n_max] int32 (the encoder frame at which token n
         fires, -1 behind the fires: token n spans (fire[n - 1], fire[n]] frames of 60 ms).  ``n_max`` defaults to T' + 1,
-        which always suffices (every frame fires at most once)."""
+        which always suffices (every frame fires at most once).  ``sampling``: draw the ids from the logits instead of taking
+        the arg-max: ``{"u": [B, n_max] float32 random numbers in [0, 1), "temperature", "top_k", "top_p", "min_p"}``, the last
+        four as ``sample_tokens`` takes them (one number, or a tensor with one per row [B * n_max]); adds ``logprobs``
+        [B, n_max]."""
         if not encoder_out.is_cuda or encoder_out.dtype != torch.float32 or encoder_out.dim() != 3 or encoder_out.shape[2] != 512:
             raise ValueError("ParaformerHead: encoder_out must be a float32 CUDA tensor [B, T', 512]")
         x = encoder_out.contiguous()
         b, tp, _ = x.shape
         dev = x.device
         n_max = tp + 1 if n_max is None else int(n_max)
+        if sampling is not None:
+            u = sampling.get("u")
+            if set(sampling) - {"u", "temperature", "top_k", "top_p", "min_p"} or not isinstance(u, torch.Tensor) or u.shape != (b, n_max):
+                raise ValueError("ParaformerHead: sampling takes u [B, n_max], temperature, top_k, top_p and min_p")
         lens = torch.as_tensor(encoder_out_lens).to(device=dev, dtype=torch.int32).contiguous()
         if lens.numel() != b:
             raise ValueError("ParaformerHead: one length per utterance")
@@ -99,7 +107,7 @@ class ParaformerHead:
         ids = torch.full((b, n_max), -1, dtype=torch.int32, device=dev)
         alphas = torch.empty((b, tp + 1), dtype=torch.float32, device=dev) if (return_alphas or return_fire_frames) else None
         fires = torch.full((b, n_max), -1, dtype=torch.int32, device=dev) if return_fire_frames else None
-        logits = torch.empty((b * n_max, self.logits_stride), dtype=torch.float32, device=dev) if return_logits else None
+        logits = torch.empty((b * n_max, self.logits_stride), dtype=torch.float32, device=dev) if return_logits or sampling is not None else None
         out = {"token_ids": ids, "token_num": token_num, "embeds": embeds}
         if b and tp:
             ptr, avail = self._workspace(self.workspace_bytes(b, tp, n_max), dev)
@@ -114,7 +122,15 @@ class ParaformerHead:
                 self.ctx.check(self.ctx.lib.asrfe_decoder_forward(
                     self.ctx.handle, x.data_ptr(), lens.data_ptr(), b, tp, embeds.data_ptr(), token_num.data_ptr(), n_max,
                     ids.data_ptr(), logits.data_ptr() if logits is not None else None, ptr, avail, st))
-        if logits is not None:
+        if sampling is not None:
+            logprobs = torch.zeros((b, n_max), dtype=torch.float32, device=dev)
+            if b and tp and n_max:
+                settings = {k: v for k, v in sampling.items() if k != "u"}
+                _, lp = sample_tokens(self.ctx, logits[:, : self.vocab_size], sampling["u"].reshape(-1), token_num=token_num,
+                                      ids=ids.view(-1), **settings)
+                logprobs = lp.view(b, n_max)
+            out["logprobs"] = logprobs
+        if return_logits:
             out["logits"] = logits.view(b, n_max, self.logits_stride)[:, :, : self.vocab_size]
         if alphas is not None and return_alphas:
             out["alphas"] = alphas
