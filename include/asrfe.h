@@ -299,12 +299,12 @@ int32_t asrfe_frame_decibel(asrfe_ctx* ctx, const void* pcm, int32_t pcm_dtype, 
  * are neither read nor written).  kv_lens[b] (int32) counts the positions of sequence b including its new ones, which
  * are the last: row t of sequence b is position kv_lens[b] - cu_q[b + 1] + t (a negative position, from more new rows
  * than positions, is not stored and sees nothing).  Position p lives in row p % page_size of page
- * block_table[b * table_stride + p / page_size]; positions past table_stride pages do not exist.  A page number outside
+ * block_table[b * table_stride + p / page_size]; positions past table_stride pages do not exist (at most 2^30 positions a row).  A page number outside
  * 0 .. n_pages - 1 (-1 for a page that was given back) is a page of which nothing is stored, read or seen. */
 typedef struct asrfe_kv_cache {
     void* k;                 /* [n_pages][n_heads][page_size][head_dim], 16-byte aligned; dtype F16, BF16 or E4M3 */
     void* v;                 /* the same for the values */
-    uint8_t* k_exp;          /* E4M3: [n_pages][n_heads][page_size], a stored value is code * 2^(exp - 127); else NULL */
+    uint8_t* k_exp;          /* E4M3: [n_pages][n_heads][page_size], 16-byte aligned, a stored value is code * 2^(exp - 127); else NULL */
     uint8_t* v_exp;
     int32_t n_pages;
     int32_t page_size;       /* 16, 32, 64, 128 or 256 positions */

@@ -29,11 +29,12 @@ int32_t view_of(asrfe_ctx* ctx, const char* who, const asrfe_kv_cache* c, int32_
     if ((1 << shift) != c->page_size) return bad(ctx, ASRFE_ERR_SHAPE, who, "page_size must be 16, 32, 64, 128 or 256");
     if (c->n_heads < 1 || c->n_heads > 256) return bad(ctx, ASRFE_ERR_SHAPE, who, "1 to 256 key / value heads");
     if (c->n_pages < 1) return bad(ctx, ASRFE_ERR_SHAPE, who, "the cache has no pages");
-    if (batch < 0 || batch > 65535 || table_stride < 0 || table_stride > (INT32_MAX >> shift))
-        return bad(ctx, ASRFE_ERR_SHAPE, who, "batch in 0..65535, table_stride >= 0 with fewer than 2^31 positions in a row of the table");
+    if (batch < 0 || batch > 65535 || table_stride < 0 || table_stride > ((1 << 30) >> shift))
+        return bad(ctx, ASRFE_ERR_SHAPE, who, "batch in 0..65535, table_stride >= 0 with at most 2^30 positions in a row of the table");
     if (!c->k || !c->v || !aligned16(c->k) || !aligned16(c->v)) return bad(ctx, ASRFE_ERR_BAD_ARG, who, "the cache's k and v must be 16-byte aligned");
     if ((c->dtype == ASRFE_DT_E4M3) != (c->k_exp != nullptr) || (c->dtype == ASRFE_DT_E4M3) != (c->v_exp != nullptr))
         return bad(ctx, ASRFE_ERR_BAD_ARG, who, "k_exp and v_exp belong to an E4M3 cache and to no other");
+    if (!aligned16(c->k_exp) || !aligned16(c->v_exp)) return bad(ctx, ASRFE_ERR_BAD_ARG, who, "k_exp and v_exp must be 16-byte aligned");
     int dev = -1;
     if (hipGetDevice(&dev) != hipSuccess || dev != ctx->device)
         return bad(ctx, ASRFE_ERR_BAD_ARG, who, "the context belongs to another device than the current one");
@@ -128,13 +129,12 @@ extern "C" int32_t asrfe_paged_attention(asrfe_ctx* ctx, const asrfe_kv_cache* c
     p.n_tokens = n_tokens;
     p.n_q_heads = n_q_heads;
     p.group = n_q_heads / cache->n_heads;
-    const int64_t exist = static_cast<int64_t>(table_stride) << p.c.page_shift;  // (below 2^31: checked above)
-    p.max_kv = static_cast<int>(std::min<int64_t>(max_kv, exist));
-    p.window = window;
-    p.sinks = sinks;
+    p.max_kv = std::min(max_kv, table_stride << p.c.page_shift);  // (at most 2^30: checked above)
+    p.window = std::min(window, 1 << 30);
+    p.sinks = std::min(sinks, 1 << 30);
     p.causal = causal != 0;
     p.scale_log2 = scale * 1.4426950408889634f;
-    return launch_paged_attention(ctx, p, cache->head_dim, dtype, cache->dtype == ASRFE_DT_E4M3, workspace, static_cast<hipStream_t>(stream));
+    return launch_paged_attention(ctx, p, cache->head_dim, dtype, cache->dtype == ASRFE_DT_E4M3, workspace, max_kv, static_cast<hipStream_t>(stream));
 }
 
 extern "C" int32_t asrfe_sample_tokens(asrfe_ctx* ctx, const void* logits, int32_t dtype, int64_t ld, int32_t rows, int32_t vocab,

@@ -6,6 +6,8 @@
 
 namespace asrfe {
 
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+
 // Largest b with cu_q[b] <= t, for a wave-uniform t: every step a wave compares 64 entries and keeps the interval behind
 // the last one that is not above t, so 65535 sequences take three dependent loads.  -1 if the row belongs to nobody.
 __device__ __forceinline__ int find_sequence(const int32_t* __restrict__ cu_q, int batch, int t) {
@@ -39,19 +41,21 @@ __device__ __forceinline__ int64_t cache_row(const PagedView& c, int page, int h
 }
 
 // Eight e4m3 codes (two dwords) times 2^(exp - 127), rounded to the 16-bit type: exact wherever the type has the value.
-template <bool F16>
-__device__ __forceinline__ uint4 dequantise8(uint2 codes, uint32_t exp) {
+// LARGE: the scale may lead out of fp16's range; what does becomes its largest value.
+template <bool F16, bool LARGE>
+__device__ __forceinline__ u32x4 dequantise8(uint32_t c0, uint32_t c1, uint32_t exp) {
     const float scale = exp ? __uint_as_float(exp << 23) : 0x1p-127f;
-    uint32_t r[4];
-#pragma unroll
-    for (int i = 0; i < 2; ++i) {
-        const uint32_t w = i ? codes.y : codes.x;
-        const auto lo = __builtin_amdgcn_cvt_pk_f32_fp8(w, false);
-        const auto hi = __builtin_amdgcn_cvt_pk_f32_fp8(w, true);
-        r[2 * i] = pack_elem2<F16>(lo[0] * scale, lo[1] * scale);
-        r[2 * i + 1] = pack_elem2<F16>(hi[0] * scale, hi[1] * scale);
-    }
-    return make_uint4(r[0], r[1], r[2], r[3]);
+    auto two = [&](uint32_t w, auto high) -> uint32_t {
+        constexpr bool H = decltype(high)::value;
+        if constexpr (F16 && LARGE) {
+            const auto f = __builtin_amdgcn_cvt_pk_f32_fp8(w, H);
+            auto in = [&](float v) { return v != v ? v : __builtin_amdgcn_fmed3f(v * scale, -65504.0f, 65504.0f); };
+            return pack_elem2<F16>(in(f[0]), in(f[1]));
+        }
+        if constexpr (F16) return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w, scale, H));
+        else return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, scale, H));
+    };
+    return u32x4{two(c0, std::false_type{}), two(c0, std::true_type{}), two(c1, std::false_type{}), two(c1, std::true_type{})};
 }
 
 inline int32_t launched(asrfe_ctx* ctx, const char* who) {

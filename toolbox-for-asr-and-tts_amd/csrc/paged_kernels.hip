@@ -86,7 +86,6 @@ template <int D, bool F16, bool E4M3>
 __global__ __launch_bounds__(kPagedThreads) void kv_read_kernel(const KvReadParams p) {
     constexpr int kLanes = D / 8;
     constexpr int kRows = 64 / kLanes;
-    saturate_fp16_conversions<F16>();
     const int64_t w = static_cast<int64_t>(blockIdx.x) * (kPagedThreads / 64) + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     if (w >= static_cast<int64_t>(p.c.batch) * p.t_max) return;
     const int lane = threadIdx.x & 63, sub = lane / kLanes, col = lane % kLanes;
@@ -99,15 +98,17 @@ __global__ __launch_bounds__(kPagedThreads) void kv_read_kernel(const KvReadPara
         const int64_t to = (w * p.c.n_heads + h) * D + 8 * col;
 #pragma unroll
         for (int kv = 0; kv < 2; ++kv) {
-            uint4 x = make_uint4(0, 0, 0, 0);
+            u32x4 x = {0, 0, 0, 0};
             if (page >= 0) {
                 const char* src = kv ? p.c.v : p.c.k;
-                if constexpr (E4M3)
-                    x = dequantise8<F16>(*reinterpret_cast<const uint2*>(src + row * D + 8 * col), (kv ? p.c.v_exp : p.c.k_exp)[row]);
-                else
-                    x = *reinterpret_cast<const uint4*>(src + row * (2 * D) + 16 * col);
+                if constexpr (E4M3) {
+                    const uint2 codes = *reinterpret_cast<const uint2*>(src + row * D + 8 * col);
+                    x = dequantise8<F16, true>(codes.x, codes.y, (kv ? p.c.v_exp : p.c.k_exp)[row]);
+                } else {
+                    x = *reinterpret_cast<const u32x4*>(src + row * (2 * D) + 16 * col);
+                }
             }
-            *reinterpret_cast<uint4*>((kv ? p.v : p.k) + to) = x;
+            *reinterpret_cast<u32x4*>((kv ? p.v : p.k) + to) = x;
         }
     }
 }

@@ -45,6 +45,8 @@ class PagedKvCache:
             raise ValueError("PagedKvCache: k_exp and v_exp must be uint8 [n_pages, n_heads, page_size]")
         if any(not t.is_cuda or not t.is_contiguous() or t.device != k.device for t in bufs):
             raise ValueError("PagedKvCache: buffers must be contiguous CUDA tensors on one device")
+        if any(t.data_ptr() % 16 for t in bufs):
+            raise ValueError("PagedKvCache: buffers must be 16-byte aligned")
         self.ctx, self.k, self.v, self.k_exp, self.v_exp = ctx, k, v, k_exp, v_exp
         self.n_pages, self.n_heads, self.page_size, self.head_dim = k.shape
         self.dtype, self.device = k.dtype, k.device
