@@ -48,13 +48,51 @@ __device__ __forceinline__ __attribute__((address_space(3))) T* lds(uint32_t add
     return (__attribute__((address_space(3))) T*)addr;
 }
 
+// 1 / a sum of weights; 0 where there were none, NaN where a score was
+__device__ __forceinline__ float inverse(float sum) { return sum > 0.0f ? 1.0f / sum : (sum == 0.0f ? 0.0f : sum); }
+
+// Workgroups are dealt round-robin over the 8 XCDs: a contiguous range for each, so that those that share keys share an L2.
+__device__ __forceinline__ int xcd_contiguous(int bid, int n) {
+    const int xcd = bid & 7, q = n >> 3, r = n & 7;
+    return (xcd < r ? xcd * (q + 1) : r * (q + 1) + (xcd - r) * q) + (bid >> 3);
+}
+
+// bytes of 135 or more, a scale of 2^8 or more, which can lead out of fp16's range: bit 7, and 7 in the rest
+__device__ __forceinline__ uint32_t large_scales(uint32_t x) { return x & 0x80808080u & ((x & 0x7f7f7f7fu) + 0x79797979u); }
+
+// Infinities and NaN among pairs of 16-bit elements.  An element whose exponent field is all ones carries into its sign bit
+// when one is added below the field.
+//
+// A product meets them where a weight of zero (a hidden key) would make NaN of them: there the finite part is multiplied as
+// usual, and for each kind of the others a product of indicators tells which (channel, row) pairs meet one under a weight
+// that is not zero.
+template <bool F16>
+struct OddValues {
+    static constexpr uint32_t kExp = (F16 ? 0x7c00u : 0x7f80u) * 0x10001u, kUnit = (F16 ? 0x0400u : 0x0080u) * 0x10001u;
+    static constexpr uint32_t kMant = kUnit - 0x10001u, kSign = 0x80008000u, kRest = 0x7fff7fffu, kOne = F16 ? 0x3c00u : 0x3f80u;
+    __device__ static uint32_t any(const u32x4 w) {  // its sign bits
+        const u32x4 t = (w & kExp) + kUnit;
+        return t[0] | t[1] | t[2] | t[3];
+    }
+    __device__ static u32x4 odd(const u32x4 w) { return ((w & kExp) + kUnit) & kSign; }
+    __device__ static u32x4 finite(const u32x4 w) { return w & ~((odd(w) >> 15) * 0xffffu); }
+    __device__ static u32x4 kind(const u32x4 w, int t) {  // ones in the place of +inf, -inf, NaN
+        const u32x4 o = odd(w), nan = ((w & kMant) + kRest) & o;
+        return ((t == 0 ? (o & ~nan & ~w) : t == 1 ? (o & ~nan & w) : nan) >> 15) * kOne;
+    }
+    __device__ static u32x4 nonzero(const u32x4 w) { return ((((w & kRest) + kRest) & kSign) >> 15) * kOne; }
+    __device__ static float value(int t) { return t == 0 ? INFINITY : t == 1 ? -INFINITY : __builtin_nanf(""); }
+};
+
 // How a call is cut into workgroups.
 struct AttnPlan {
-    int row_tile;    // 32 or 128 rows
+    int row_tile;    // 16, 32 or 128 rows
     int n_tiles;     // upper bound of the row tiles of all sequences
     int n_split;     // parts a tile's keys may be cut into
     int chunk;       // key tiles of a part
     int key_tile;    // 32 or 64 positions
+    int most_split;  // parts the workspace has room for: a window only lessens them
+    bool one_wave;   // so few key tiles that a single wave takes a row tile
 };
 
 struct AttnJob {
@@ -64,35 +102,37 @@ struct AttnJob {
     float* part_ml;  // [item][part][row][2]: running maximum (scaled, base 2) and sum
 };
 
+// How a row tile's n_vt key tiles are cut: never into more parts than the launch has places for, whatever the host took for
+// the number of tiles.
+struct Parts {
+    int chunk, n;
+    __device__ Parts(const AttnJob& job, int n_vt) {
+        const int least = (n_vt + job.n_split - 1) / job.n_split;
+        chunk = job.chunk > least ? job.chunk : least;
+        n = n_vt <= chunk ? 1 : (n_vt + chunk - 1) / chunk;
+    }
+};
+
 // What a row tile covers.
 struct TileSpan {
     int b, row0, n_rows, tok0, pos0, len;
     int sink_tiles, first, n_vt;  // key tiles: 0 .. sink_tiles - 1, then first ..; n_vt of them
 };
 
-// Row tile `tile` -> its sequence.  Sequence b's tiles start at cu_q[b] * group / row_tile + b: never fewer places than it
-// needs, and the search for them is one comparison of 64 sequences per step.
+// Sequence b's row tiles begin at cu_q[b] * group / row_tile + b: never fewer places than it needs.
+template <int RT>
+__device__ __forceinline__ int first_tile(const PagedAttnParams& p, int b, int cu) {
+    return static_cast<int>(static_cast<int64_t>(cu) * p.group / RT) + b;
+}
+
+// What row tile `tile` covers of sequence b; false if none of its rows.
 template <int RT, int TK>
-__device__ __forceinline__ bool tile_span(const PagedAttnParams& p, int tile, TileSpan& s) {
-    const int lane = threadIdx.x & 63;
-    int lo = 0, span = p.c.batch, step = 1;
-    while (step * 64 < span) step *= 64;
-    auto start = [&](int i) { return static_cast<int>(static_cast<int64_t>(p.c.cu_q[i]) * p.group / RT) + i; };
-    for (;; step >>= 6) {
-        const int i = lo + lane * step;
-        const bool below = i < lo + span && start(i) <= tile;
-        const int c = __builtin_popcountll(__ballot(below));
-        if (c == 0) return false;
-        lo += (c - 1) * step;
-        const int left = span - (c - 1) * step;
-        span = left < step ? left : step;
-        if (step == 1) break;
-    }
-    s.b = __builtin_amdgcn_readfirstlane(lo);
+__device__ __forceinline__ bool span_of(const PagedAttnParams& p, int b, int tile, TileSpan& s) {
+    s.b = b;
     const int cu0 = __builtin_amdgcn_readfirstlane(p.c.cu_q[s.b]), cu1 = __builtin_amdgcn_readfirstlane(p.c.cu_q[s.b + 1]);
     const int kv = __builtin_amdgcn_readfirstlane(p.c.kv_lens[s.b]);
     const int64_t n_rows = static_cast<int64_t>((cu1 < p.n_tokens ? cu1 : p.n_tokens) - cu0) * p.group;
-    const int64_t row0 = (static_cast<int64_t>(tile) - (static_cast<int64_t>(cu0) * p.group / RT + s.b)) * RT;
+    const int64_t row0 = (static_cast<int64_t>(tile) - first_tile<RT>(p, s.b, cu0)) * RT;
     if (cu0 < 0 || row0 < 0 || row0 >= n_rows) return false;
     s.n_rows = static_cast<int>(n_rows);
     s.row0 = static_cast<int>(row0);
@@ -114,6 +154,25 @@ __device__ __forceinline__ bool tile_span(const PagedAttnParams& p, int tile, Ti
     return true;
 }
 
+// Row tile `tile` -> its sequence: a search of 64 sequences per step.
+template <int RT, int TK>
+__device__ __forceinline__ bool tile_span(const PagedAttnParams& p, int tile, TileSpan& s) {
+    const int lane = threadIdx.x & 63;
+    int lo = 0, span = p.c.batch, step = 1;
+    while (step * 64 < span) step *= 64;
+    for (;; step >>= 6) {
+        const int i = lo + lane * step;
+        const bool below = i < lo + span && first_tile<RT>(p, i, p.c.cu_q[i]) <= tile;
+        const int c = __builtin_popcountll(__ballot(below));
+        if (c == 0) return false;
+        lo += (c - 1) * step;
+        const int left = span - (c - 1) * step;
+        span = left < step ? left : step;
+        if (step == 1) break;
+    }
+    return span_of<RT, TK>(p, __builtin_amdgcn_readfirstlane(lo), tile, s);
+}
+
 template <int D>
 __device__ __forceinline__ int swz_k(int r) {
     return D == 128 ? (r & 15) : ((r >> 1) & 7);
@@ -123,49 +182,39 @@ __device__ __forceinline__ int swz_v(int r) {
     return D == 128 ? (((r & 3) << 2) | ((r >> 2) & 3)) : ((((r >> 1) & 1) << 2) | ((r >> 2) & 3));
 }
 
-template <int D, bool E4M3, int RW, int KW>
-struct AttnShape {
-    static constexpr int kWaves = RW * KW;
-    static constexpr int kRowTile = 32 * RW;
-    static constexpr int kKeys = RW == 1 ? 32 : 64;                // positions of a key tile
-    static constexpr int kRowBytes = 2 * D;                        // of a position in the LDS
-    static constexpr int kTile = kKeys * kRowBytes;                // one of K, V
-    static constexpr int kBufs = E4M3 && RW == 1 ? 1 : 2;          // (e4m3, own tiles: the next one waits in registers)
-    static constexpr int kGroupLds = kBufs * 2 * kTile;            // of the waves that share tiles
-    static constexpr int kJoin = KW > 1 ? KW * (D / 2) * 256 + KW * 256 : 0;
-    static constexpr int kLds = KW * kGroupLds > kJoin ? KW * kGroupLds : kJoin;
-    static constexpr int kRpi = 1024 / kRowBytes;                  // rows one wave brings in with one load
-    static constexpr int kLoads = kKeys / (RW * kRpi);             // loads per wave for one of K, V
-    static constexpr int kVar = RW == 1 ? 16 / kRpi : 1;           // different places of a load inside its 16 rows
+// ---- many rows: prompts ------------------------------------------------------------------------------------------------
+// Four waves with 32 rows each share key tiles of 64 positions in the LDS: tile t + 1 arrives while tile t is used.
+template <int D, bool E4M3>
+struct ManyShape {
+    static constexpr int kKeys = 64, kRowTile = 128;
+    static constexpr int kRowBytes = 2 * D;               // of a position in the LDS
+    static constexpr int kTile = kKeys * kRowBytes;       // one of K, V
+    static constexpr int kRpi = 1024 / kRowBytes;         // rows one wave brings in with one load
+    static constexpr int kLoads = kKeys / (4 * kRpi);     // loads per wave for one of K, V
     static constexpr int kPieces = kKeys / 16;
-    static constexpr int kPerCu = 160 * 1024 / kLds >= 2 ? 2 : 1;  // workgroups of a compute unit
-    static constexpr int kWavesPerSimd = kPerCu * kWaves >= 8 ? 2 : 1;
 };
 
-template <int D, bool F16, bool E4M3, int RW, int KW>
-__global__ __launch_bounds__(64 * RW * KW, (AttnShape<D, E4M3, RW, KW>::kWavesPerSimd)) void paged_attn_kernel(const AttnJob job) {
-    using S = AttnShape<D, E4M3, RW, KW>;
-    constexpr int kKeys = S::kKeys, kRowBytes = S::kRowBytes, kTile = S::kTile, kChunks = kRowBytes / 16, kMt = D / 32, kKk = kKeys / 32;
-    __shared__ __attribute__((aligned(1024))) char smem[S::kLds];
+template <int D, bool F16, bool E4M3>
+__global__ __launch_bounds__(256, 2) void paged_attn_many_kernel(const AttnJob job) {
+    using S = ManyShape<D, E4M3>;
+    constexpr int kKeys = S::kKeys, kRowBytes = S::kRowBytes, kTile = S::kTile, kChunks = kRowBytes / 16, kMt = D / 32;
+    __shared__ __attribute__((aligned(1024))) char smem[4 * kTile];
     // (no saturate_fp16_conversions here: in that mode the matrix instructions lose infinities and NaN in their accumulators)
     const PagedAttnParams& p = job.p;
     const int tid = threadIdx.x, lane = tid & 63, l31 = lane & 31, h = lane >> 5;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-    const int rw = RW == 1 ? 0 : wave, kw = RW == 1 ? wave : 0;
-    // workgroups are dealt round-robin over the 8 XCDs: give each a contiguous range, row tiles of one head together
-    const int nwg = gridDim.x, bid = blockIdx.x;
-    const int xcd = bid & 7, xq = nwg >> 3, xr = nwg & 7;
-    const int logical = (xcd < xr ? xcd * (xq + 1) : xr * (xq + 1) + (xcd - xr) * xq) + (bid >> 3);
+    const int logical = xcd_contiguous(blockIdx.x, gridDim.x);
     const int part = logical % job.n_split, item = logical / job.n_split;
     const int tile = item % job.n_tiles, kvh = item / job.n_tiles;
     TileSpan ts;
-    if (!tile_span<32 * RW, kKeys>(p, tile, ts)) return;
-    const int n_parts = ts.n_vt <= job.chunk ? 1 : (ts.n_vt + job.chunk - 1) / job.chunk;
+    if (!tile_span<S::kRowTile, kKeys>(p, tile, ts)) return;
+    const Parts parts(job, ts.n_vt);
+    const int n_parts = parts.n;
     if (part >= n_parts) return;
-    const int vt0 = part * job.chunk, vt1 = vt0 + job.chunk < ts.n_vt ? vt0 + job.chunk : ts.n_vt;
+    const int vt0 = part * parts.chunk, vt1 = vt0 + parts.chunk < ts.n_vt ? vt0 + parts.chunk : ts.n_vt;
 
     // ---- this wave's rows, this lane's row
-    const int rbase = ts.row0 + rw * 32;
+    const int rbase = ts.row0 + wave * 32;
     const bool has_rows = rbase < ts.n_rows;
     const int row = rbase + l31 < ts.n_rows ? rbase + l31 : ts.n_rows - 1;
     const int tok = row / p.group, hq = kvh * p.group + row % p.group;
@@ -203,62 +252,55 @@ __global__ __launch_bounds__(64 * RW * KW, (AttnShape<D, E4M3, RW, KW>::kWavesPe
     // LDS addresses.  A row's 16-byte pieces are swizzled by functions of the row that are linear over its bits, so every
     // address below is one base per lane, an exclusive or with a constant and a constant offset.  The bases are hidden from
     // the compiler where they are used: it would keep each sum in a register of its own through the loop, and spill.
-    const uint32_t own_base = __builtin_amdgcn_readfirstlane(lds_addr_of(smem + kw * S::kGroupLds));
-    // 16-bit caches, straight into the LDS: load i of this wave covers rows (i * RW + rw) * kRpi .. + kRpi - 1 of the tile,
-    // a lane 16 bytes; the place in the LDS follows the lane, so the swizzle is applied to the source (K and V differ)
-    const int lrow = lane / kChunks, lchunk = lane % kChunks;
-    uint32_t voff_k[S::kVar], voff_v[S::kVar];
-#pragma unroll
-    for (int i = 0; i < S::kVar; ++i) {
-        const int r = ((RW == 1 ? i : rw) * S::kRpi & 15) + lrow;
-        voff_k[i] = r * kRowBytes + (lchunk ^ swz_k<D>(r)) * 16;
-        voff_v[i] = r * kRowBytes + (lchunk ^ swz_v<D>(r)) * 16;
-    }
-    auto issue16 = [&](const Pieces& pc, int buf) {
-        const uint32_t dst = __builtin_amdgcn_readfirstlane(own_base + buf * 2 * kTile + rw * 1024);
+    const uint32_t lds0 = __builtin_amdgcn_readfirstlane(lds_addr_of(smem));
+    // 16-bit caches, straight into the LDS: load i of this wave covers rows (4 i + wave) * kRpi .. + kRpi - 1 of the tile, a
+    // lane 16 bytes; the place in the LDS follows the lane, so the swizzle is applied to the source (K and V differ)
+    const int lrow = (wave * S::kRpi & 15) + lane / kChunks, lchunk = lane % kChunks;
+    const uint32_t voff_k = lrow * kRowBytes + (lchunk ^ swz_k<D>(lrow)) * 16, voff_v = lrow * kRowBytes + (lchunk ^ swz_v<D>(lrow)) * 16;
+    auto issue16 = [&](const Pieces& pc, int buf) __attribute__((always_inline)) {
+        const uint32_t dst = __builtin_amdgcn_readfirstlane(lds0 + buf * 2 * kTile + wave * 1024);
         static_for<S::kLoads>([&](auto ic) {
             constexpr int I = decltype(ic)::value;
             int64_t at;
-            if constexpr (RW * S::kRpi == 32) {
+            if constexpr (S::kRpi == 8) {
                 const int64_t even = pc.row[2 * I], odd = pc.row[2 * I + 1];
-                at = rw & 2 ? odd : even;
+                at = wave & 2 ? odd : even;
             } else {
-                at = pc.row[I * RW * S::kRpi / 16];
+                at = pc.row[I];
             }
-            lds_dma16(uniform(p.c.k + at * kRowBytes), voff_k[I % S::kVar], dst + I * RW * 1024);
-            lds_dma16(uniform(p.c.v + at * kRowBytes), voff_v[I % S::kVar], dst + kTile + I * RW * 1024);
+            lds_dma16(uniform(p.c.k + at * kRowBytes), voff_k, dst + I * 4096);
+            lds_dma16(uniform(p.c.v + at * kRowBytes), voff_v, dst + kTile + I * 4096);
         });
     };
-    // e4m3, through registers: a lane takes 16 codes of each of kLoads8 consecutive rows, so their exponents lie side by side
-    constexpr int kLpr = D / 16, kLoads8 = kKeys / RW * kLpr / 64;
+    // e4m3, through registers: a wave takes a piece, a lane 16 codes of each of kLoads8 consecutive rows, so that their
+    // exponents lie side by side
+    constexpr int kLpr = D / 16, kLoads8 = 16 * kLpr / 64;
     const int r8 = (lane / kLpr) * kLoads8, c8 = lane % kLpr;  // first row (of the wave's), pair of 16-byte pieces
     u32x4 k8[E4M3 ? kLoads8 : 1], v8[E4M3 ? kLoads8 : 1];
     uint32_t ke8 = 0, ve8 = 0;
-    auto issue8 = [&](const Pieces& pc) {
+    auto issue8 = [&](const Pieces& pc) __attribute__((always_inline)) {
         if constexpr (E4M3) {
             int64_t at = pc.row[0];
-            const int piece = RW == 1 ? r8 >> 4 : rw;
 #pragma unroll
             for (int g = 1; g < S::kPieces; ++g) {
                 const int64_t x = pc.row[g];
-                at = piece == g ? x : at;
+                at = wave == g ? x : at;
             }
-            at += r8 & 15;
-            const char* kp = p.c.k + at * D + 16 * c8;
-            const char* vp = p.c.v + at * D + 16 * c8;
+            const char* kp = p.c.k + (at + r8) * D + 16 * c8;
+            const char* vp = p.c.v + (at + r8) * D + 16 * c8;
 #pragma unroll
             for (int i = 0; i < kLoads8; ++i) {
                 k8[i] = *reinterpret_cast<const u32x4*>(kp + i * D);
                 v8[i] = *reinterpret_cast<const u32x4*>(vp + i * D);
             }
-            using E = std::conditional_t<kLoads8 == 4, uint32_t, std::conditional_t<kLoads8 == 2, uint16_t, uint8_t>>;
-            ke8 = *reinterpret_cast<const E*>(p.c.k_exp + at);
-            ve8 = *reinterpret_cast<const E*>(p.c.v_exp + at);
+            using E = std::conditional_t<kLoads8 == 2, uint16_t, uint8_t>;
+            ke8 = *reinterpret_cast<const E*>(p.c.k_exp + at + r8);
+            ve8 = *reinterpret_cast<const E*>(p.c.v_exp + at + r8);
         }
     };
-    const int r8w = (RW == 1 ? 0 : rw * 16) + r8;
+    const int r8w = wave * 16 + r8;
     const uint32_t put_k = r8w * kRowBytes + ((2 * c8) ^ swz_k<D>(r8w)) * 16, put_v = r8w * kRowBytes + ((2 * c8) ^ swz_v<D>(r8w)) * 16;
-    auto put8 = [&](uint32_t tile_base) {
+    auto put8 = [&](uint32_t tile_base) __attribute__((always_inline)) {
         if constexpr (E4M3) {
             uint32_t kb = tile_base + put_k, vb = tile_base + kTile + put_v;
             asm volatile("" : "+v"(kb), "+v"(vb));
@@ -273,19 +315,15 @@ __global__ __launch_bounds__(64 * RW * KW, (AttnShape<D, E4M3, RW, KW>::kWavesPe
                     *lds<u32x4>((vb ^ ((swz_v<D>(i) ^ 1) * 16)) + i * kRowBytes) = dequantise8<F16, kLarge>(v8[i][2], v8[i][3], ve);
                 }
             };
-            // a scale of 2^8 or more can lead out of fp16's range (bytes of 135 or more: bit 7, and 7 in the rest)
-            auto big = [](uint32_t x) { return x & 0x80808080u & ((x & 0x7f7f7f7fu) + 0x79797979u); };
-            if (F16 && __any((big(ke8) | big(ve8)) != 0)) put(std::true_type{});
+            if (F16 && __any((large_scales(ke8) | large_scales(ve8)) != 0)) put(std::true_type{});
             else put(std::false_type{});
         }
     };
 
     // ---- first tile, queries
-    constexpr int kStep = KW;
-    int vt = vt0 + kw;
     uint32_t valid = 0;  // of the tile that is about to be used: which of its pieces exist
-    if (vt < vt1) {
-        const Pieces pc = pieces_of(vt);
+    if (vt0 < vt1) {
+        const Pieces pc = pieces_of(vt0);
         valid = pc.valid;
         if constexpr (E4M3) issue8(pc);
         else issue16(pc, 0);
@@ -315,11 +353,11 @@ __global__ __launch_bounds__(64 * RW * KW, (AttnShape<D, E4M3, RW, KW>::kWavesPe
         for (int e = 0; e < 16; ++e) oacc[mt][e] = 0.0f;
     float mc = -INFINITY, l_run = 0.0f;  // running maximum (scaled, base 2) and sum of this lane's half of the keys
 
-    auto compute = [&](uint32_t tile_base, int key0, uint32_t valid, auto edge_c) __attribute__((always_inline)) {
+    auto compute = [&](uint32_t tile_base, int key0, uint32_t exist, auto edge_c) __attribute__((always_inline)) {
         constexpr bool edge = decltype(edge_c)::value;
-        f32x16 sacc[kKk];
+        f32x16 sacc[2];
 #pragma unroll
-        for (int kk = 0; kk < kKk; ++kk)
+        for (int kk = 0; kk < 2; ++kk)
 #pragma unroll
             for (int e = 0; e < 16; ++e) sacc[kk][e] = 0.0f;
         uint32_t kb = tile_base + get_k;
@@ -327,23 +365,23 @@ __global__ __launch_bounds__(64 * RW * KW, (AttnShape<D, E4M3, RW, KW>::kWavesPe
 #pragma unroll
         for (int s = 0; s < D / 16; ++s)
 #pragma unroll
-            for (int kk = 0; kk < kKk; ++kk) {
+            for (int kk = 0; kk < 2; ++kk) {
                 const u16x8 kf = *lds<const u16x8>((kb ^ (s << 5)) + kk * 32 * kRowBytes);
                 sacc[kk] = mfma32<F16>(kf, qf[s], sacc[kk]);
             }
         if constexpr (edge) {
 #pragma unroll
-            for (int kk = 0; kk < kKk; ++kk)
+            for (int kk = 0; kk < 2; ++kk)
 #pragma unroll
                 for (int e = 0; e < 16; ++e) {
                     const int j = key0 + kk * 32 + (e & 3) + 8 * (e >> 2) + 4 * h;
-                    const bool see = (j < hi) & ((j >= lo) | (j < p.sinks)) & (((valid >> (kk * 2 + (e >> 3))) & 1) != 0);
+                    const bool see = (j < hi) & ((j >= lo) | (j < p.sinks)) & (((exist >> (kk * 2 + (e >> 3))) & 1) != 0);
                     sacc[kk][e] = see ? sacc[kk][e] : -INFINITY;
                 }
         }
         float rmax = sacc[0][0];
 #pragma unroll
-        for (int kk = 0; kk < kKk; ++kk)
+        for (int kk = 0; kk < 2; ++kk)
 #pragma unroll
             for (int e = 0; e < 16; ++e) rmax = fmaxf(rmax, sacc[kk][e]);
         {   // the row's other keys sit in lane ^ 32
@@ -363,9 +401,9 @@ __global__ __launch_bounds__(64 * RW * KW, (AttnShape<D, E4M3, RW, KW>::kWavesPe
                 for (int e = 0; e < 16; ++e) oacc[mt][e] *= alpha;
         }
         float psum = 0.0f;
-        u32x4 pf[kKk][2];
+        u32x4 pf[2][2];
 #pragma unroll
-        for (int kk = 0; kk < kKk; ++kk)
+        for (int kk = 0; kk < 2; ++kk)
 #pragma unroll
             for (int s2 = 0; s2 < 2; ++s2)
 #pragma unroll
@@ -377,7 +415,7 @@ __global__ __launch_bounds__(64 * RW * KW, (AttnShape<D, E4M3, RW, KW>::kWavesPe
                 }
         l_run = l_run * alpha + psum;
 #pragma unroll
-        for (int kk = 0; kk < kKk; ++kk)
+        for (int kk = 0; kk < 2; ++kk)
 #pragma unroll
             for (int s2 = 0; s2 < 2; ++s2) asm volatile("" : "+v"(pf[kk][s2]));  // (packed here: not in 32 bits up to their use)
         uint32_t vb = tile_base + kTile + get_v;
@@ -386,210 +424,559 @@ __global__ __launch_bounds__(64 * RW * KW, (AttnShape<D, E4M3, RW, KW>::kWavesPe
             const uint32_t at = vb ^ (mt * 64);
             const v4s a = __builtin_amdgcn_ds_read_tr16_b64_v4i16(lds<v4s>(at + (kk * 32 + s2 * 16) * kRowBytes));
             const v4s b = __builtin_amdgcn_ds_read_tr16_b64_v4i16(lds<v4s>((at ^ 32) + (kk * 32 + s2 * 16 + 8) * kRowBytes));
-            return __builtin_bit_cast(u16x8, __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7));
+            return __builtin_bit_cast(u32x4, __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7));
         };
-        // A 16-bit element whose exponent field is all ones carries into its sign bit when one is added below the field.
-        constexpr uint32_t kExp = (F16 ? 0x7c00u : 0x7f80u) * 0x10001u, kUnit = (F16 ? 0x0400u : 0x0080u) * 0x10001u;
-        constexpr uint32_t kMant = kUnit - 0x10001u, kSign = 0x80008000u, kRest = 0x7fff7fffu, kOne = F16 ? 0x3c00u : 0x3f80u;
+        auto times = [&](const u32x4 v, const u32x4 w, const f32x16 acc) { return mfma32<F16>(__builtin_bit_cast(u16x8, v), __builtin_bit_cast(u16x8, w), acc); };
+        using O = OddValues<F16>;
         bool special = false;
         if constexpr (edge) {
             uint32_t any = 0;
 #pragma unroll
-            for (int kk = 0; kk < kKk; ++kk)
+            for (int kk = 0; kk < 2; ++kk)
 #pragma unroll
                 for (int s2 = 0; s2 < 2; ++s2) {
 #pragma unroll
-                    for (int mt = 0; mt < kMt; ++mt) {
-                        const u32x4 w = __builtin_bit_cast(u32x4, v_frag(kk, s2, mt));
-                        const u32x4 t = (w & kExp) + kUnit;
-                        any |= t[0] | t[1] | t[2] | t[3];
-                    }
+                    for (int mt = 0; mt < kMt; ++mt) any |= O::any(v_frag(kk, s2, mt));
                     __builtin_amdgcn_sched_barrier(0);
                 }
-            special = __any((any & kSign) != 0);
+            special = __any((any & O::kSign) != 0);
         }
         if (!special) {
 #pragma unroll
-            for (int kk = 0; kk < kKk; ++kk)
+            for (int kk = 0; kk < 2; ++kk)
 #pragma unroll
                 for (int s2 = 0; s2 < 2; ++s2)
 #pragma unroll
-                    for (int mt = 0; mt < kMt; ++mt) oacc[mt] = mfma32<F16>(v_frag(kk, s2, mt), __builtin_bit_cast(u16x8, pf[kk][s2]), oacc[mt]);
+                    for (int mt = 0; mt < kMt; ++mt) oacc[mt] = times(v_frag(kk, s2, mt), pf[kk][s2], oacc[mt]);
         } else {
-            // Infinities and NaN in V: the finite part as usual, then, for each kind of the others, a product of
-            // indicators tells which (channel, row) pairs meet one under a weight that is not zero.
 #pragma unroll
-            for (int kk = 0; kk < kKk; ++kk)
+            for (int kk = 0; kk < 2; ++kk)
 #pragma unroll
-                for (int s2 = 0; s2 < 2; ++s2) {
-                    const u32x4 on = ((((pf[kk][s2] & kRest) + kRest) & kSign) >> 15) * kOne;
+                for (int s2 = 0; s2 < 2; ++s2)
 #pragma unroll
                     for (int mt = 0; mt < kMt; ++mt) {
-                        const u32x4 v = __builtin_bit_cast(u32x4, v_frag(kk, s2, mt));
-                        const u32x4 odd = ((v & kExp) + kUnit) & kSign, nan = ((v & kMant) + kRest) & odd;
-                        oacc[mt] = mfma32<F16>(__builtin_bit_cast(u16x8, v & ~((odd >> 15) * 0xffffu)), __builtin_bit_cast(u16x8, pf[kk][s2]), oacc[mt]);
+                        const u32x4 v = v_frag(kk, s2, mt);
+                        oacc[mt] = times(O::finite(v), pf[kk][s2], oacc[mt]);
 #pragma unroll
                         for (int t = 0; t < 3; ++t) {
-                            const u32x4 is = t == 0 ? (odd & ~nan & ~v) : t == 1 ? (odd & ~nan & v) : nan;
-                            f32x16 n;
+                            f32x16 hit;
 #pragma unroll
-                            for (int e = 0; e < 16; ++e) n[e] = 0.0f;
-                            n = mfma32<F16>(__builtin_bit_cast(u16x8, (is >> 15) * kOne), __builtin_bit_cast(u16x8, on), n);
-                            const float add = t == 0 ? INFINITY : t == 1 ? -INFINITY : __builtin_nanf("");
+                            for (int e = 0; e < 16; ++e) hit[e] = 0.0f;
+                            hit = times(O::kind(v, t), O::nonzero(pf[kk][s2]), hit);
 #pragma unroll
-                            for (int e = 0; e < 16; ++e) oacc[mt][e] += n[e] > 0.0f ? add : 0.0f;
+                            for (int e = 0; e < 16; ++e) oacc[mt][e] += hit[e] > 0.0f ? O::value(t) : 0.0f;
                             __builtin_amdgcn_sched_barrier(0);
                         }
                     }
-                }
         }
     };
 
     int buf = 0;
-    while (vt < vt1) {
-        const int next = vt + kStep;
-        const bool more = next < vt1;
-        if constexpr (E4M3) {
-            put8(own_base + buf * 2 * kTile);
-            if (RW > 1) __syncthreads();
-            else asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-        } else {
-            // this wave's loads of the tile are in, and its reads of the tile before are done with the other buffer
-            asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
-            if (RW > 1) __syncthreads();
-        }
+    for (int vt = vt0; vt < vt1; ++vt) {
+        if constexpr (E4M3) put8(lds0 + buf * 2 * kTile);
+        else asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // this wave's loads of the tile are in
+        __syncthreads();  // and all others'; and no wave reads the other buffer any more
         const uint32_t now = valid;
-        if (more) {
-            const Pieces pc = pieces_of(next);
+        if (vt + 1 < vt1) {
+            const Pieces pc = pieces_of(vt + 1);
             valid = pc.valid;
             if constexpr (E4M3) issue8(pc);
             else issue16(pc, buf ^ 1);
         }
         const int key0 = key0_of(vt);
-        // (hidden from every row of the wave: the end of a prompt's shorter rows)
+        // (a tile may be hidden from every row of a wave: the keys behind a prompt's first rows, the window of its last ones)
         if (has_rows && key0 < w_hi_max && (key0 + kKeys > w_lo_min || key0 < p.sinks)) {
             const bool inside = key0 + kKeys <= w_hi_min && (key0 >= w_lo_max || key0 + kKeys <= p.sinks) && now == (1u << S::kPieces) - 1;
-            if (inside) compute(own_base + buf * 2 * kTile, key0, now, std::false_type{});
-            else compute(own_base + buf * 2 * kTile, key0, now, std::true_type{});
+            if (inside) compute(lds0 + buf * 2 * kTile, key0, now, std::false_type{});
+            else compute(lds0 + buf * 2 * kTile, key0, now, std::true_type{});
         }
-        if (S::kBufs == 2) buf ^= 1;
-        vt = next;
+        buf ^= 1;
     }
 
     // ---- results: lane (l31, h) holds of its row the channels 32 mt + 8 (e >> 2) + 4 h + (e & 3)
-    float l_tot = l_run + __shfl_xor(l_run, 32);
-    float* po = job.part_o + ((static_cast<int64_t>(item) * job.n_split + part) * S::kRowTile + rw * 32 + l31) * D;
-    float* pml = job.part_ml + ((static_cast<int64_t>(item) * job.n_split + part) * S::kRowTile + rw * 32 + l31) * 2;
-    uint16_t* out = p.out + (ts.tok0 + tok) * p.o_ts + hq * p.o_hs;
-    const bool mine = has_rows && rbase + l31 < ts.n_rows;
-    auto store = [&](int f, float a, float b, float cc, float d, float inv) {  // channels of flat accumulator index f .. f + 3
-        const int ch = 32 * (f >> 4) + 8 * ((f & 15) >> 2) + 4 * h;
-        if (n_parts == 1) {
-            const uint2 w = make_uint2(pack_result<F16>(a * inv, b * inv), pack_result<F16>(cc * inv, d * inv));
-            if (mine) *reinterpret_cast<uint2*>(out + ch) = w;
-        } else if (mine) {
-            *reinterpret_cast<float4*>(po + ch) = make_float4(a, b, cc, d);
+    if (!has_rows || rbase + l31 >= ts.n_rows) return;
+    const float l_tot = l_run + __shfl_xor(l_run, 32);
+    const float inv = inverse(l_tot);
+    const int64_t part_row = (static_cast<int64_t>(item) * job.n_split + part) * S::kRowTile + wave * 32 + l31;
+    uint16_t* out = p.out + (ts.tok0 + tok) * p.o_ts + hq * p.o_hs + 4 * h;
+    float* po = job.part_o + part_row * D + 4 * h;
+#pragma unroll
+    for (int mt = 0; mt < kMt; ++mt)
+#pragma unroll
+        for (int e = 0; e < 16; e += 4) {
+            const float4 o = make_float4(oacc[mt][e], oacc[mt][e + 1], oacc[mt][e + 2], oacc[mt][e + 3]);
+            const int ch = 32 * mt + 2 * e;
+            if (n_parts == 1) *reinterpret_cast<uint2*>(out + ch) = make_uint2(pack_result<F16>(o.x * inv, o.y * inv), pack_result<F16>(o.z * inv, o.w * inv));
+            else *reinterpret_cast<float4*>(po + ch) = o;
+        }
+    if (n_parts > 1 && h == 0) *reinterpret_cast<float2*>(job.part_ml + part_row * 2) = make_float2(mc, l_tot);
+}
+
+// ---- few rows: single tokens, short chunks ---------------------------------------------------------------------------
+// A wave has the 16 * NQ rows of the tile and key tiles of 32 positions of its own.  With v_mfma_f32_16x16x32 the first
+// operand is 16 keys by 32 channels, 8 consecutive channels per lane: K goes from memory straight to registers, one tile
+// ahead; V goes to the LDS and is read transposed.  The scores of a lane are those of keys 4 g .. 4 g + 3 (g = lane / 16) of
+// either half of the tile, for row lane % 16: taken in this order they are the second operand of O^T = V^T P^T as they are.
+template <int D, bool E4M3, int NQ, int KW>
+struct FewShape {
+    static constexpr int kRowBytes = 2 * D;
+    static constexpr int kTile = 32 * kRowBytes;                   // V of a key tile
+    static constexpr int kBufs = E4M3 ? 1 : 2;                     // (e4m3: the next one waits in registers)
+    static constexpr int kAcc = NQ * (D / 16) * 4;                 // accumulators of a lane
+    static constexpr int kJoin = KW > 1 ? KW * kAcc * 256 + KW * NQ * 128 : 0;
+    static constexpr int kLds = KW * kBufs * kTile > kJoin ? KW * kBufs * kTile : kJoin;
+    static constexpr int kRpi = 1024 / kRowBytes, kLoads = 32 / kRpi, kVar = 16 / kRpi;
+    static constexpr int kKs = E4M3 ? D / 64 : D / 32;             // 16-byte loads of K per lane and 16 keys
+};
+
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+
+template <bool F16>
+__device__ __forceinline__ f32x4 mfma16(const u32x4 a, const u32x4 b, const f32x4 c) {
+    if constexpr (F16) return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
+    else return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+}
+
+// maximum and sum over the four lanes that hold one row
+__device__ __forceinline__ float max_of_row(float v) {
+    const auto a = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    v = fmaxf(__uint_as_float(a[0]), __uint_as_float(a[1]));
+    const auto b = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    return fmaxf(__uint_as_float(b[0]), __uint_as_float(b[1]));
+}
+__device__ __forceinline__ float sum_of_row(float v) {
+    v += __shfl_xor(v, 32);
+    return v + __shfl_xor(v, 16);
+}
+
+template <int D, bool F16, bool E4M3, int NQ, int KW>
+__global__ __launch_bounds__(64 * KW, (NQ == 1 ? 2 : 1)) void paged_attn_few_kernel(const AttnJob job) {
+    using S = FewShape<D, E4M3, NQ, KW>;
+    constexpr int kRowBytes = S::kRowBytes, kTile = S::kTile, kChunks = kRowBytes / 16, kMb = D / 16, kRt = 16 * NQ, kKeys = 32, kKs = S::kKs;
+    __shared__ __attribute__((aligned(1024))) char smem[S::kLds];
+    const PagedAttnParams& p = job.p;
+    const int lane = threadIdx.x & 63, col = lane & 15, g = lane >> 4;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int logical = xcd_contiguous(blockIdx.x, gridDim.x);
+    const int part = logical % job.n_split, item = logical / job.n_split;
+    const int tile = item % job.n_tiles, kvh = item / job.n_tiles;
+    TileSpan ts;
+    if (!tile_span<kRt, kKeys>(p, tile, ts)) return;
+    const Parts parts(job, ts.n_vt);
+    const int n_parts = parts.n;
+    if (part >= n_parts) return;
+    const int vt0 = part * parts.chunk, vt1 = vt0 + parts.chunk < ts.n_vt ? vt0 + parts.chunk : ts.n_vt;
+
+    // ---- rows
+    const int last = ts.row0 + kRt - 1 < ts.n_rows ? ts.row0 + kRt - 1 : ts.n_rows - 1;
+    const int pmin = __builtin_amdgcn_readfirstlane(ts.pos0 + ts.row0 / p.group), pmax = __builtin_amdgcn_readfirstlane(ts.pos0 + last / p.group);
+    auto hi_of = [&](int i) { return i < 0 ? 0 : (p.causal && i + 1 < ts.len ? i + 1 : ts.len); };
+    auto lo_of = [&](int i) { return p.window > 0 && i - p.window + 1 > 0 ? i - p.window + 1 : 0; };
+    const int w_hi_min = hi_of(pmin), w_lo_max = lo_of(pmax);
+    int hi[NQ], lo[NQ];
+    int64_t out_at[NQ];
+    u32x4 qf[NQ][D / 32];
+    const uint32_t flip = p.scale_log2 < 0.0f ? 0x80008000u : 0u;
+    const float c = fmaxf(__builtin_fabsf(p.scale_log2), 1e-37f);  // (a scale of zero weighs all positions the same)
+#pragma unroll
+    for (int n = 0; n < NQ; ++n) {
+        const int r = ts.row0 + 16 * n + col, row = r < ts.n_rows ? r : ts.n_rows - 1;
+        const int tok = row / p.group, hq = kvh * p.group + row % p.group;
+        hi[n] = hi_of(ts.pos0 + tok);
+        lo[n] = lo_of(ts.pos0 + tok);
+        out_at[n] = (ts.tok0 + tok) * p.o_ts + hq * p.o_hs;
+        const uint16_t* qp = p.q + (ts.tok0 + tok) * p.q_ts + hq * p.q_hs;
+        // the channels of step s, in the order in which this lane has those of its keys
+#pragma unroll
+        for (int s = 0; s < D / 32; ++s) {
+            const int d = E4M3 ? 64 * (s >> 1) + 16 * g + 8 * (s & 1) : 32 * s + 8 * g;
+            qf[n][s] = *reinterpret_cast<const u32x4*>(qp + d) ^ flip;
+        }
+    }
+
+    // ---- key tiles
+    const const_i32 table = (const_i32)(p.c.block_table + static_cast<int64_t>(ts.b) * p.c.table_stride);
+    const int page_mask = (1 << p.c.page_shift) - 1;
+    auto key0_of = [&](int vt) { return (vt < ts.sink_tiles ? vt : ts.first + vt - ts.sink_tiles) * kKeys; };
+    struct Pieces {
+        int64_t row[2];
+        uint32_t valid;
+    };
+    auto pieces_of = [&](int vt) {
+        Pieces r;
+        r.valid = 0;
+        const int key0 = key0_of(vt);
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+            const int key = key0 + 16 * u, i = key >> p.c.page_shift;
+            const int page = table[i < p.c.table_stride ? i : p.c.table_stride - 1];
+            const bool ok = i < p.c.table_stride && page >= 0 && page < p.c.n_pages;
+            r.valid |= ok ? 1u << u : 0u;
+            r.row[u] = ((static_cast<int64_t>(ok ? page : 0) * p.c.n_heads + kvh) << p.c.page_shift) + (key & page_mask);
+        }
+        return r;
+    };
+    const uint32_t own_base = __builtin_amdgcn_readfirstlane(lds_addr_of(smem + wave * S::kBufs * kTile));
+    const int lrow = lane / kChunks, lchunk = lane % kChunks;
+    uint32_t voff_v[E4M3 ? 1 : S::kVar];
+    if constexpr (!E4M3) {
+#pragma unroll
+        for (int i = 0; i < S::kVar; ++i) {
+            const int r = i * S::kRpi + lrow;
+            voff_v[i] = r * kRowBytes + (lchunk ^ swz_v<D>(r)) * 16;
+        }
+    }
+    constexpr int kStored = E4M3 ? D : 2 * D;
+    const uint32_t voff_k = col * kStored + 16 * g;
+    constexpr int kLpr = D / 16, kLoads8 = 32 * kLpr / 64;
+    const int r8 = (lane / kLpr) * kLoads8, c8 = lane % kLpr;
+    u32x4 v8[E4M3 ? kLoads8 : 1];
+    uint32_t ve8 = 0;
+    struct Keys {
+        u32x4 w[2][kKs];
+        uint32_t exp[2];
+    };
+    auto issue = [&](const Pieces& pc, Keys& k, int buf) __attribute__((always_inline)) {
+        if constexpr (E4M3) {
+            const int64_t even = pc.row[0], odd = pc.row[1];
+            const int64_t at = (r8 & 16 ? odd : even) + (r8 & 15);
+            const char* vp = p.c.v + at * D + 16 * c8;
+#pragma unroll
+            for (int i = 0; i < kLoads8; ++i) v8[i] = *reinterpret_cast<const u32x4*>(vp + i * D);
+            using E = std::conditional_t<kLoads8 == 4, uint32_t, uint16_t>;
+            ve8 = *reinterpret_cast<const E*>(p.c.v_exp + at);
+        } else {
+            const uint32_t dst = __builtin_amdgcn_readfirstlane(own_base + buf * kTile);
+            static_for<S::kLoads>([&](auto ic) {
+                constexpr int I = decltype(ic)::value;
+                lds_dma16(uniform(p.c.v + pc.row[I * S::kRpi / 16] * kRowBytes), voff_v[I % S::kVar], dst + I * 1024);
+            });
+        }
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+            const char* kp = uniform(p.c.k + pc.row[u] * kStored);
+#pragma unroll
+            for (int s = 0; s < kKs; ++s) k.w[u][s] = *reinterpret_cast<const u32x4*>(kp + voff_k + 64 * s);
+            if constexpr (E4M3) k.exp[u] = reinterpret_cast<const uint8_t*>(uniform(reinterpret_cast<const char*>(p.c.k_exp) + pc.row[u]))[static_cast<uint32_t>(col)];
         }
     };
-    if constexpr (KW == 1) {
-        const float inv = l_tot > 0.0f ? 1.0f / l_tot : (l_tot == 0.0f ? 0.0f : l_tot);
+    const uint32_t put_v = r8 * kRowBytes + ((2 * c8) ^ swz_v<D>(r8)) * 16;
+    uint32_t get_v;  // V read transposed: lane 4 q + pp of 16 fetches key row 4 g + q, channels 4 pp ..; it receives 4 keys of a channel
+    {
+        const int q = col >> 2, pp = col & 3, r = 4 * g + q;
+        get_v = r * kRowBytes + ((pp >> 1) ^ swz_v<D>(r)) * 16 + 8 * (pp & 1);
+    }
+
+    f32x4 oacc[NQ][kMb];
+    float mc[NQ], l_run[NQ];
 #pragma unroll
-        for (int f = 0; f < 16 * kMt; f += 4) store(f, oacc[f >> 4][f & 15], oacc[f >> 4][(f & 15) + 1], oacc[f >> 4][(f & 15) + 2], oacc[f >> 4][(f & 15) + 3], inv);
-        if (n_parts > 1 && mine && h == 0) *reinterpret_cast<float2*>(pml) = make_float2(mc, l_tot);
+    for (int n = 0; n < NQ; ++n) {
+        mc[n] = -INFINITY;
+        l_run[n] = 0.0f;
+#pragma unroll
+        for (int m = 0; m < kMb; ++m) oacc[n][m] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+    }
+
+    auto compute = [&](const Keys& k, uint32_t tile_base, int key0, uint32_t valid, auto edge_c) __attribute__((always_inline)) {
+        constexpr bool edge = decltype(edge_c)::value;
+        f32x4 sacc[NQ][2];
+#pragma unroll
+        for (int n = 0; n < NQ; ++n)
+#pragma unroll
+            for (int u = 0; u < 2; ++u) sacc[n][u] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+        const bool large = F16 && E4M3 && __any((k.exp[0] >= 135) | (k.exp[1] >= 135));
+#pragma unroll
+        for (int s = 0; s < D / 32; ++s)
+#pragma unroll
+            for (int u = 0; u < 2; ++u) {
+                u32x4 kf;
+                if constexpr (E4M3) {
+                    const uint32_t a = k.w[u][s >> 1][2 * (s & 1)], b = k.w[u][s >> 1][2 * (s & 1) + 1];
+                    kf = large ? dequantise8<F16, true>(a, b, k.exp[u]) : dequantise8<F16, false>(a, b, k.exp[u]);
+                } else {
+                    kf = k.w[u][s];
+                }
+#pragma unroll
+                for (int n = 0; n < NQ; ++n) sacc[n][u] = mfma16<F16>(kf, qf[n][s], sacc[n][u]);
+            }
+        u32x4 pf[NQ];
+#pragma unroll
+        for (int n = 0; n < NQ; ++n) {
+            if constexpr (edge) {
+#pragma unroll
+                for (int u = 0; u < 2; ++u)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        const int j = key0 + 16 * u + 4 * g + i;
+                        const bool see = (j < hi[n]) & ((j >= lo[n]) | (j < p.sinks)) & (((valid >> u) & 1) != 0);
+                        sacc[n][u][i] = see ? sacc[n][u][i] : -INFINITY;
+                    }
+            }
+            float rmax = sacc[n][0][0];
+#pragma unroll
+            for (int u = 0; u < 2; ++u)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) rmax = fmaxf(rmax, sacc[n][u][i]);
+            rmax = max_of_row(rmax);
+            // the maximum only has to keep exp2 in range: it is raised when a tile exceeds it by more than 2^8
+            const bool grew = rmax * c > mc[n] + 8.0f;
+            const float m_new = grew ? rmax * c : mc[n];
+            const float alpha = grew ? __builtin_amdgcn_exp2f(mc[n] - m_new) : 1.0f;
+            mc[n] = m_new;
+            const float sub = m_new == -INFINITY ? 0.0f : m_new;  // (nothing seen yet: every weight below is exp2(-inf))
+            if (__any(grew)) {
+#pragma unroll
+                for (int m = 0; m < kMb; ++m) oacc[n][m] *= alpha;
+            }
+            float psum = 0.0f;
+#pragma unroll
+            for (int u = 0; u < 2; ++u)
+#pragma unroll
+                for (int i = 0; i < 4; i += 2) {
+                    const float a = __builtin_amdgcn_exp2f(fmaf(sacc[n][u][i], c, -sub));
+                    const float b = __builtin_amdgcn_exp2f(fmaf(sacc[n][u][i + 1], c, -sub));
+                    psum += a + b;
+                    pf[n][2 * u + i / 2] = pack_elem2<F16>(a, b);
+                }
+            l_run[n] = l_run[n] * alpha + psum;
+        }
+        uint32_t vb = tile_base + get_v;
+        asm volatile("" : "+v"(vb));
+        auto v_frag = [&](int m) {
+            const uint32_t at = vb ^ (m * 32);
+            const v4s a = __builtin_amdgcn_ds_read_tr16_b64_v4i16(lds<v4s>(at));
+            const v4s b = __builtin_amdgcn_ds_read_tr16_b64_v4i16(lds<v4s>(at + 16 * kRowBytes));
+            return __builtin_bit_cast(u32x4, __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7));
+        };
+        using O = OddValues<F16>;
+        bool special = false;
+        if constexpr (edge) {
+            uint32_t any = 0;
+#pragma unroll
+            for (int m = 0; m < kMb; ++m) any |= O::any(v_frag(m));
+            special = __any((any & O::kSign) != 0);
+        }
+        if (!special) {
+#pragma unroll
+            for (int m = 0; m < kMb; ++m) {
+                const u32x4 v = v_frag(m);
+#pragma unroll
+                for (int n = 0; n < NQ; ++n) oacc[n][m] = mfma16<F16>(v, pf[n], oacc[n][m]);
+            }
+        } else {
+#pragma unroll
+            for (int m = 0; m < kMb; ++m) {
+                const u32x4 v = v_frag(m);
+#pragma unroll
+                for (int n = 0; n < NQ; ++n) {
+                    oacc[n][m] = mfma16<F16>(O::finite(v), pf[n], oacc[n][m]);
+#pragma unroll
+                    for (int t = 0; t < 3; ++t) {
+                        const f32x4 hit = mfma16<F16>(O::kind(v, t), O::nonzero(pf[n]), f32x4{0.0f, 0.0f, 0.0f, 0.0f});
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) oacc[n][m][i] += hit[i] > 0.0f ? O::value(t) : 0.0f;
+                        __builtin_amdgcn_sched_barrier(0);
+                    }
+                }
+            }
+        }
+    };
+
+    int vt = vt0 + wave;
+    uint32_t valid = 0;  // of the tile that is about to be used: which of its pieces exist
+    Keys ka, kb;
+    if (vt < vt1) {
+        const Pieces pc = pieces_of(vt);
+        valid = pc.valid;
+        issue(pc, ka, 0);
+    }
+    auto turn = [&](Keys& now_k, Keys& next_k, int buf) __attribute__((always_inline)) {
+        // everything of this tile is in, and the reads of the tile before are done with the other buffer
+        __builtin_amdgcn_s_waitcnt(0x0070);  // vmcnt(0) lgkmcnt(0)
+        asm volatile("" ::: "memory");
+        if constexpr (E4M3) {
+            uint32_t vb = own_base + put_v;
+            asm volatile("" : "+v"(vb));
+            auto put = [&](auto big) __attribute__((always_inline)) {
+#pragma unroll
+                for (int i = 0; i < kLoads8; ++i) {
+                    const uint32_t e = (ve8 >> (8 * i)) & 255u;
+                    *lds<u32x4>((vb ^ (swz_v<D>(i) * 16)) + i * kRowBytes) = dequantise8<F16, decltype(big)::value>(v8[i][0], v8[i][1], e);
+                    *lds<u32x4>((vb ^ ((swz_v<D>(i) ^ 1) * 16)) + i * kRowBytes) = dequantise8<F16, decltype(big)::value>(v8[i][2], v8[i][3], e);
+                }
+            };
+            if (F16 && __any(large_scales(ve8) != 0)) put(std::true_type{});
+            else put(std::false_type{});
+            asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+        }
+        const uint32_t now = valid;
+        const int next = vt + KW, key0 = key0_of(vt);
+        if (next < vt1) {
+            const Pieces pc = pieces_of(next);
+            valid = pc.valid;
+            issue(pc, next_k, E4M3 ? 0 : buf ^ 1);
+        }
+        const uint32_t base = own_base + (E4M3 ? 0 : buf * kTile);
+        if (key0 + kKeys <= w_hi_min && (key0 >= w_lo_max || key0 + kKeys <= p.sinks) && now == 3) compute(now_k, base, key0, now, std::false_type{});
+        else compute(now_k, base, key0, now, std::true_type{});
+        vt = next;
+    };
+    while (vt < vt1) {
+        turn(ka, kb, 0);
+        if (vt >= vt1) break;
+        turn(kb, ka, 1);
+    }
+
+    // ---- results: lane (col, g) holds of row col the channels 16 m + 4 g .. + 3
+    const int64_t part_row = (static_cast<int64_t>(item) * job.n_split + part) * kRt;
+    auto store = [&](int n, int m, float4 o, float inv) {
+        if (ts.row0 + 16 * n + col >= ts.n_rows) return;
+        const int ch = 16 * m + 4 * g;
+        if (n_parts == 1) *reinterpret_cast<uint2*>(p.out + out_at[n] + ch) = make_uint2(pack_result<F16>(o.x * inv, o.y * inv), pack_result<F16>(o.z * inv, o.w * inv));
+        else *reinterpret_cast<float4*>(job.part_o + (part_row + 16 * n + col) * D + ch) = o;
+    };
+    auto store_ml = [&](int n, float m, float l) {
+        if (n_parts > 1 && g == 0 && ts.row0 + 16 * n + col < ts.n_rows) *reinterpret_cast<float2*>(job.part_ml + (part_row + 16 * n + col) * 2) = make_float2(m, l);
+    };
+#pragma unroll
+    for (int n = 0; n < NQ; ++n) l_run[n] = sum_of_row(l_run[n]);
+    if constexpr (KW == 1) {
+#pragma unroll
+        for (int n = 0; n < NQ; ++n) {
+#pragma unroll
+            for (int m = 0; m < kMb; ++m) store(n, m, make_float4(oacc[n][m][0], oacc[n][m][1], oacc[n][m][2], oacc[n][m][3]), inverse(l_run[n]));
+            store_ml(n, mc[n], l_run[n]);
+        }
     } else {
         // the waves' sums are brought to one maximum and added through the LDS
-        constexpr int kN = 16 * kMt, kOwn = kN / KW;
-        float* ml = reinterpret_cast<float*>(smem);
-        float* os = ml + KW * 64;
+        float* ml = reinterpret_cast<float*>(smem);  // [wave][n][maximum of 16 rows, sum of 16 rows]
+        float* os = ml + KW * NQ * 32;
         __syncthreads();  // all waves are done with their tiles
-        if (h == 0) {
-            ml[wave * 64 + l31] = mc;
-            ml[wave * 64 + 32 + l31] = l_tot;
-        }
-        __syncthreads();
-        float top = mc, sum = 0.0f;
 #pragma unroll
-        for (int i = 0; i < KW; ++i) top = fmaxf(top, ml[i * 64 + l31]);
-        const float sub = top == -INFINITY ? 0.0f : top;
-#pragma unroll
-        for (int i = 0; i < KW; ++i) sum += ml[i * 64 + 32 + l31] * __builtin_amdgcn_exp2f(ml[i * 64 + l31] - sub);
-        const float f0 = __builtin_amdgcn_exp2f(mc - sub);
-#pragma unroll
-        for (int f = 0; f < kN; f += 4)
-            *reinterpret_cast<float4*>(os + ((wave * (kN / 4) + f / 4) * 64 + lane) * 4) =
-                make_float4(oacc[f >> 4][f & 15] * f0, oacc[f >> 4][(f & 15) + 1] * f0, oacc[f >> 4][(f & 15) + 2] * f0, oacc[f >> 4][(f & 15) + 3] * f0);
-        __syncthreads();
-        const float inv = sum > 0.0f ? 1.0f / sum : (sum == 0.0f ? 0.0f : sum);
-#pragma unroll
-        for (int x = 0; x < kOwn; x += 4) {
-            const int f = wave * kOwn + x;
-            float4 a = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-#pragma unroll
-            for (int i = 0; i < KW; ++i) {
-                const float4 t = *reinterpret_cast<const float4*>(os + ((i * (kN / 4) + f / 4) * 64 + lane) * 4);
-                a.x += t.x; a.y += t.y; a.z += t.z; a.w += t.w;
+        for (int n = 0; n < NQ; ++n)
+            if (g == 0) {
+                ml[(wave * NQ + n) * 32 + col] = mc[n];
+                ml[(wave * NQ + n) * 32 + 16 + col] = l_run[n];
             }
-            store(f, a.x, a.y, a.z, a.w, inv);
+        __syncthreads();
+        float inv[NQ];
+#pragma unroll
+        for (int n = 0; n < NQ; ++n) {
+            float top = mc[n], sum = 0.0f;
+#pragma unroll
+            for (int i = 0; i < KW; ++i) top = fmaxf(top, ml[(i * NQ + n) * 32 + col]);
+            const float sub = top == -INFINITY ? 0.0f : top;
+#pragma unroll
+            for (int i = 0; i < KW; ++i) sum += ml[(i * NQ + n) * 32 + 16 + col] * __builtin_amdgcn_exp2f(ml[(i * NQ + n) * 32 + col] - sub);
+            const float f = __builtin_amdgcn_exp2f(mc[n] - sub);
+#pragma unroll
+            for (int m = 0; m < kMb; ++m)
+                *reinterpret_cast<float4*>(os + (((wave * NQ + n) * kMb + m) * 64 + lane) * 4) = make_float4(oacc[n][m][0] * f, oacc[n][m][1] * f, oacc[n][m][2] * f, oacc[n][m][3] * f);
+            inv[n] = inverse(sum);
+            if (wave == 0) store_ml(n, top, sum);
         }
-        if (n_parts > 1 && mine && h == 0 && wave == 0) *reinterpret_cast<float2*>(pml) = make_float2(top, sum);
+        __syncthreads();
+#pragma unroll
+        for (int n = 0; n < NQ; ++n)
+            for (int m = wave; m < kMb; m += KW) {
+                float4 a = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll
+                for (int i = 0; i < KW; ++i) {
+                    const float4 t = *reinterpret_cast<const float4*>(os + (((i * NQ + n) * kMb + m) * 64 + lane) * 4);
+                    a.x += t.x; a.y += t.y; a.z += t.z; a.w += t.w;
+                }
+                store(n, m, a, inv[n]);
+            }
     }
 }
 
-// Joins the parts of a row tile: a thread has 4 channels of a row.
+// Joins the parts of one row (at most kMostParts): a thread adds four channels over every eighth part or so, the sums meet in
+// the LDS.
+constexpr int kMostParts = 256;
+
 template <int D, bool F16, int RT, int TK>
 __global__ __launch_bounds__(256) void paged_join_kernel(const AttnJob job) {
+    constexpr int kT = D / 4, kSlices = 256 / kT;
+    __shared__ float weight[kMostParts];
+    __shared__ float4 sums[kSlices][kT];
+    __shared__ float red[8];
     const PagedAttnParams& p = job.p;
-    const int item = blockIdx.x, tile = item % job.n_tiles, kvh = item / job.n_tiles;
+    const int t = blockIdx.x / p.n_q_heads, hq = blockIdx.x % p.n_q_heads, kvh = hq / p.group, tid = threadIdx.x;
+    const int b = __builtin_amdgcn_readfirstlane(find_sequence(p.c.cu_q, p.c.batch, t));
+    if (b < 0) return;
+    const int cu0 = p.c.cu_q[b], row = (t - cu0) * p.group + hq % p.group, r = row % RT;
+    const int tile = first_tile<RT>(p, b, cu0) + row / RT;
     TileSpan ts;
-    if (!tile_span<RT, TK>(p, tile, ts)) return;
-    const int n_parts = (ts.n_vt + job.chunk - 1) / job.chunk;
-    if (ts.n_vt <= job.chunk) return;
-    constexpr int kT = D / 4;
-    const int d = 4 * (threadIdx.x % kT);
-    for (int r = threadIdx.x / kT; r < RT && ts.row0 + r < ts.n_rows; r += 256 / kT) {
-        const int64_t base = static_cast<int64_t>(item) * job.n_split * RT + r;
-        float top = -INFINITY;
-        for (int i = 0; i < n_parts; ++i) top = fmaxf(top, job.part_ml[(base + static_cast<int64_t>(i) * RT) * 2]);
-        const float sub = top == -INFINITY ? 0.0f : top;
-        float sum = 0.0f;
-        float4 a = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    if (tile >= job.n_tiles || !span_of<RT, TK>(p, b, tile, ts)) return;
+    const int n_parts = Parts(job, ts.n_vt).n;
+    if (n_parts == 1) return;
+    const int64_t base = (static_cast<int64_t>(kvh) * job.n_tiles + tile) * job.n_split * RT + r;
+    float2 ml = make_float2(-INFINITY, 0.0f);
+    if (tid < n_parts) ml = *reinterpret_cast<const float2*>(job.part_ml + (base + static_cast<int64_t>(tid) * RT) * 2);
+    float top = ml.x;
+#pragma unroll
+    for (int o = 32; o >= 1; o >>= 1) top = fmaxf(top, __shfl_xor(top, o));
+    if ((tid & 63) == 0) red[tid >> 6] = top;
+    __syncthreads();
+    top = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
+    const float f = __builtin_amdgcn_exp2f(ml.x - (top == -INFINITY ? 0.0f : top));
+    weight[tid] = f;
+    float sum = ml.y * f;
+#pragma unroll
+    for (int o = 32; o >= 1; o >>= 1) sum += __shfl_xor(sum, o);
+    if ((tid & 63) == 0) red[4 + (tid >> 6)] = sum;
+    __syncthreads();
+    const int d = tid % kT, slice = tid / kT;
+    float4 a = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
 #pragma unroll 4
-        for (int i = 0; i < n_parts; ++i) {
-            const int64_t at = base + static_cast<int64_t>(i) * RT;
-            const float2 ml = *reinterpret_cast<const float2*>(job.part_ml + at * 2);
-            const float4 o = *reinterpret_cast<const float4*>(job.part_o + at * D + d);
-            const float f = __builtin_amdgcn_exp2f(ml.x - sub);
-            sum = fmaf(ml.y, f, sum);
-            a.x = fmaf(o.x, f, a.x);
-            a.y = fmaf(o.y, f, a.y);
-            a.z = fmaf(o.z, f, a.z);
-            a.w = fmaf(o.w, f, a.w);
-        }
-        const float inv = sum > 0.0f ? 1.0f / sum : (sum == 0.0f ? 0.0f : sum);
-        const int row = ts.row0 + r, tok = row / p.group, hq = kvh * p.group + row % p.group;
-        uint16_t* out = p.out + (ts.tok0 + tok) * p.o_ts + hq * p.o_hs + d;
-        *reinterpret_cast<uint2*>(out) = make_uint2(pack_result<F16>(a.x * inv, a.y * inv), pack_result<F16>(a.z * inv, a.w * inv));
+    for (int i = slice; i < n_parts; i += kSlices) {
+        const float4 o = *reinterpret_cast<const float4*>(job.part_o + (base + static_cast<int64_t>(i) * RT) * D + 4 * d);
+        const float w = weight[i];
+        a.x = fmaf(o.x, w, a.x);
+        a.y = fmaf(o.y, w, a.y);
+        a.z = fmaf(o.z, w, a.z);
+        a.w = fmaf(o.w, w, a.w);
     }
+    sums[slice][d] = a;
+    __syncthreads();
+    if (slice != 0) return;
+#pragma unroll
+    for (int i = 1; i < kSlices; ++i) {
+        const float4 o = sums[i][d];
+        a.x += o.x; a.y += o.y; a.z += o.z; a.w += o.w;
+    }
+    const float inv = inverse((red[4] + red[5]) + (red[6] + red[7]));
+    uint16_t* out = p.out + t * p.o_ts + hq * p.o_hs + 4 * d;
+    *reinterpret_cast<uint2*>(out) = make_uint2(pack_result<F16>(a.x * inv, a.y * inv), pack_result<F16>(a.z * inv, a.w * inv));
 }
 
 namespace {
-// Key tiles a part has at least: below this a part costs more than the time its neighbours save.
-constexpr int kMinChunk = 8;
+// Key tiles a part has at least: below this a part costs more than the time its neighbours save (one stream of 500 positions:
+// 9.3 us whole, 10.3 us as two parts and their join).
+constexpr int kMinChunk = 16;
+// Key tiles up to which one wave takes a row tile by itself (256 chunks of 10 frames under a window of 50: 13.5 us, with
+// four waves 19.9 us).
+constexpr int kOneWave = 4;
 
-AttnPlan plan_of(const asrfe_ctx* ctx, int n_heads, int n_tokens, int n_q_heads, int batch, int max_kv) {
+AttnPlan plan_of(const asrfe_ctx* ctx, int n_heads, int n_tokens, int n_q_heads, int batch, int max_kv, int window, int sinks) {
     AttnPlan a;
-    const int64_t rows = static_cast<int64_t>(n_tokens) * (n_q_heads / n_heads);
-    // up to 32 rows per sequence and head: the waves of a workgroup share the rows instead of the keys
-    a.row_tile = batch > 0 && rows <= static_cast<int64_t>(batch) * 32 ? 32 : 128;
-    a.key_tile = a.row_tile == 32 ? 32 : 64;
+    const int64_t rows = static_cast<int64_t>(n_tokens) * (n_q_heads / n_heads), seqs = std::max(batch, 1);
+    // up to 32 rows per sequence and head: every wave has all of them, and keys of its own
+    a.row_tile = rows <= seqs * 16 ? 16 : rows <= seqs * 32 ? 32 : 128;
+    a.key_tile = a.row_tile == 128 ? 64 : 32;
     a.n_tiles = static_cast<int>(rows / a.row_tile) + batch;
     const int64_t items = static_cast<int64_t>(a.n_tiles) * n_heads;
-    const int64_t tiles = std::max<int64_t>(1, (static_cast<int64_t>(max_kv) + a.key_tile - 1) / a.key_tile);
+    const int64_t all = std::max<int64_t>(1, (static_cast<int64_t>(max_kv) + a.key_tile - 1) / a.key_tile);
+    // what a row tile can see of a window: its keys, the tokens of the tile, and an end of a tile on either side
+    const int64_t seen = static_cast<int64_t>(window) + sinks + n_tokens / seqs;
+    const int64_t tiles = window > 0 ? std::min(all, seen / a.key_tile + 3) : all;
     // enough parts for every compute unit to have several, so that sequences of different lengths even out
-    const int64_t want = a.row_tile == 32 ? 16 * ctx->num_cus : 2 * ctx->num_cus;
-    const int64_t most = std::max<int64_t>(1, std::min<int64_t>({want / std::max<int64_t>(1, items), (tiles + kMinChunk - 1) / kMinChunk, 256}));
-    a.chunk = static_cast<int>((tiles + most - 1) / most);
+    const int64_t want = (a.row_tile == 128 ? 2 : 8) * ctx->num_cus;
+    auto most_of = [&](int64_t n) { return std::max<int64_t>(1, std::min<int64_t>({want / std::max<int64_t>(1, items), (n + kMinChunk - 1) / kMinChunk, kMostParts})); };
+    a.most_split = static_cast<int>(most_of(all));
+    a.chunk = static_cast<int>((tiles + most_of(tiles) - 1) / most_of(tiles));
     a.n_split = static_cast<int>((tiles + a.chunk - 1) / a.chunk);
+    a.one_wave = a.row_tile != 128 && a.chunk <= kOneWave;
     return a;
 }
 
@@ -597,9 +984,9 @@ int64_t align256(int64_t n) { return (n + 255) / 256 * 256; }
 }  // namespace
 
 int64_t paged_attention_workspace(const asrfe_ctx* ctx, int head_dim, int n_heads, int n_tokens, int n_q_heads, int batch, int max_kv) {
-    const AttnPlan a = plan_of(ctx, n_heads, n_tokens, n_q_heads, batch, max_kv);
-    if (a.n_split == 1) return 0;
-    const int64_t rows = static_cast<int64_t>(a.n_tiles) * n_heads * a.n_split * a.row_tile;
+    const AttnPlan a = plan_of(ctx, n_heads, n_tokens, n_q_heads, batch, max_kv, 0, 0);
+    if (a.most_split == 1) return 0;
+    const int64_t rows = static_cast<int64_t>(a.n_tiles) * n_heads * a.most_split * a.row_tile;
     return align256(rows * head_dim * 4) + align256(rows * 8);
 }
 
@@ -608,19 +995,23 @@ static int32_t launch_attn(asrfe_ctx* ctx, const AttnJob& job, const AttnPlan& a
     const int64_t items = static_cast<int64_t>(a.n_tiles) * job.p.c.n_heads, wgs = items * a.n_split;
     if (wgs > INT32_MAX) return set_err(ctx, ASRFE_ERR_SHAPE, "paged_attention: too many rows and heads for one launch");
     const dim3 grid(static_cast<uint32_t>(wgs));
-    if (a.row_tile == 32) hipLaunchKernelGGL((paged_attn_kernel<D, F16, E4M3, 1, 4>), grid, dim3(256), 0, s, job);
-    else hipLaunchKernelGGL((paged_attn_kernel<D, F16, E4M3, 4, 1>), grid, dim3(256), 0, s, job);
+    if (a.row_tile == 16 && a.one_wave) hipLaunchKernelGGL((paged_attn_few_kernel<D, F16, E4M3, 1, 1>), grid, dim3(64), 0, s, job);
+    else if (a.row_tile == 16) hipLaunchKernelGGL((paged_attn_few_kernel<D, F16, E4M3, 1, 4>), grid, dim3(256), 0, s, job);
+    else if (a.row_tile == 32 && a.one_wave) hipLaunchKernelGGL((paged_attn_few_kernel<D, F16, E4M3, 2, 1>), grid, dim3(64), 0, s, job);
+    else if (a.row_tile == 32) hipLaunchKernelGGL((paged_attn_few_kernel<D, F16, E4M3, 2, 4>), grid, dim3(256), 0, s, job);
+    else hipLaunchKernelGGL((paged_attn_many_kernel<D, F16, E4M3>), grid, dim3(256), 0, s, job);
     if (int32_t rc = launched(ctx, "paged_attention")) return rc;
     if (a.n_split == 1) return ASRFE_OK;
-    const dim3 jg(static_cast<uint32_t>(items));
-    if (a.row_tile == 32) hipLaunchKernelGGL((paged_join_kernel<D, F16, 32, 32>), jg, dim3(256), 0, s, job);
+    const dim3 jg(static_cast<uint32_t>(job.p.n_tokens) * job.p.n_q_heads);  // (at most 2^30: checked at the entry)
+    if (a.row_tile == 16) hipLaunchKernelGGL((paged_join_kernel<D, F16, 16, 32>), jg, dim3(256), 0, s, job);
+    else if (a.row_tile == 32) hipLaunchKernelGGL((paged_join_kernel<D, F16, 32, 32>), jg, dim3(256), 0, s, job);
     else hipLaunchKernelGGL((paged_join_kernel<D, F16, 128, 64>), jg, dim3(256), 0, s, job);
     return launched(ctx, "paged_attention join");
 }
 
 int32_t launch_paged_attention(asrfe_ctx* ctx, const PagedAttnParams& p, int head_dim, int dtype, bool e4m3, void* ws, int max_kv,
                                hipStream_t s) {
-    const AttnPlan a = plan_of(ctx, p.c.n_heads, p.n_tokens, p.n_q_heads, p.c.batch, max_kv);
+    const AttnPlan a = plan_of(ctx, p.c.n_heads, p.n_tokens, p.n_q_heads, p.c.batch, max_kv, p.window, p.sinks);
     AttnJob job{};
     job.p = p;
     job.n_tiles = a.n_tiles;
