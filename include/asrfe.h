@@ -308,7 +308,7 @@ typedef struct asrfe_kv_cache {
     uint8_t* v_exp;
     int32_t n_pages;
     int32_t page_size;       /* 16, 32, 64, 128 or 256 positions */
-    int32_t n_heads;         /* key / value heads, 1 .. 256 */
+    int32_t n_heads;         /* key / value heads, 1 .. 256 (n_pages * n_heads * page_size below 2^32) */
     int32_t head_dim;        /* 64 or 128 */
     int32_t dtype;           /* ASRFE_DT_F16, ASRFE_DT_BF16 or ASRFE_DT_E4M3 */
 } asrfe_kv_cache;

@@ -29,6 +29,7 @@ int32_t view_of(asrfe_ctx* ctx, const char* who, const asrfe_kv_cache* c, int32_
     if ((1 << shift) != c->page_size) return bad(ctx, ASRFE_ERR_SHAPE, who, "page_size must be 16, 32, 64, 128 or 256");
     if (c->n_heads < 1 || c->n_heads > 256) return bad(ctx, ASRFE_ERR_SHAPE, who, "1 to 256 key / value heads");
     if (c->n_pages < 1) return bad(ctx, ASRFE_ERR_SHAPE, who, "the cache has no pages");
+    if ((static_cast<int64_t>(c->n_pages) * c->n_heads << shift) > UINT32_MAX) return bad(ctx, ASRFE_ERR_SHAPE, who, "the cache has 2^32 rows or more");
     if (batch < 0 || batch > 65535 || table_stride < 0 || table_stride > ((1 << 30) >> shift))
         return bad(ctx, ASRFE_ERR_SHAPE, who, "batch in 0..65535, table_stride >= 0 with at most 2^30 positions in a row of the table");
     if (!c->k || !c->v || !aligned16(c->k) || !aligned16(c->v)) return bad(ctx, ASRFE_ERR_BAD_ARG, who, "the cache's k and v must be 16-byte aligned");

@@ -182,6 +182,48 @@ __device__ __forceinline__ int swz_v(int r) {
     return D == 128 ? (((r & 3) << 2) | ((r >> 2) & 3)) : ((((r >> 1) & 1) << 2) | ((r >> 2) & 3));
 }
 
+// Where the 16-position pieces of a key tile lie: rows of the cache, and which of them exist.  (Row numbers fit 32 bits: checked
+// at the entry.)  Pages that hold whole tiles take one look-up, smaller ones one per piece.
+template <int N>
+struct Pieces {
+    uint32_t row[N];
+    uint32_t valid;
+};
+
+struct PageWalk {
+    const_i32 table;
+    int stride, n_pages, shift;
+    uint32_t page_rows, head;  // rows of a page (all heads), first row of this head in it
+    __device__ PageWalk(const PagedView& c, int b, int kvh)
+        : table((const_i32)(c.block_table + static_cast<int64_t>(b) * c.table_stride)), stride(c.table_stride), n_pages(c.n_pages),
+          shift(c.page_shift), page_rows(static_cast<uint32_t>(c.n_heads) << c.page_shift), head(static_cast<uint32_t>(kvh) << c.page_shift) {}
+    __device__ __forceinline__ uint32_t find(int key, bool& ok) const {
+        const int i = key >> shift;
+        const int page = table[i < stride ? i : stride - 1];
+        ok = (i < stride) & (static_cast<uint32_t>(page) < static_cast<uint32_t>(n_pages));
+        return (ok ? page : 0) * page_rows + head + (key & ((1 << shift) - 1));
+    }
+    template <int N>
+    __device__ __forceinline__ Pieces<N> tile(int key0) const {
+        Pieces<N> r;
+        bool ok;
+        if (16 * N <= (1 << shift)) {
+            const uint32_t row = find(key0, ok);
+#pragma unroll
+            for (int g = 0; g < N; ++g) r.row[g] = row + 16 * g;
+            r.valid = ok ? (1u << N) - 1 : 0;
+        } else {
+            r.valid = 0;
+#pragma unroll
+            for (int g = 0; g < N; ++g) {
+                r.row[g] = find(key0 + 16 * g, ok);
+                r.valid |= ok ? 1u << g : 0u;
+            }
+        }
+        return r;
+    }
+};
+
 // ---- many rows: prompts ------------------------------------------------------------------------------------------------
 // Four waves with 32 rows each share key tiles of 64 positions in the LDS: tile t + 1 arrives while tile t is used.
 template <int D, bool E4M3>
@@ -224,30 +266,11 @@ __global__ __launch_bounds__(256, 2) void paged_attn_many_kernel(const AttnJob j
     auto hi_of = [&](int i) { return i < 0 ? 0 : (p.causal && i + 1 < ts.len ? i + 1 : ts.len); };
     auto lo_of = [&](int i) { return p.window > 0 && i - p.window + 1 > 0 ? i - p.window + 1 : 0; };
     const int hi = hi_of(pos), lo = lo_of(pos);
-    const int w_hi_min = hi_of(pmin), w_hi_max = hi_of(pmax), w_lo_min = lo_of(pmin), w_lo_max = lo_of(pmax);
+    const int w_hi_max = hi_of(pmax), w_lo_min = lo_of(pmin);
 
     // ---- key tiles: where their pieces lie
-    const const_i32 table = (const_i32)(p.c.block_table + static_cast<int64_t>(ts.b) * p.c.table_stride);
-    const int page_mask = (1 << p.c.page_shift) - 1;
-    struct Pieces {
-        int64_t row[S::kPieces];
-        uint32_t valid;
-    };
+    const PageWalk pages(p.c, ts.b, kvh);
     auto key0_of = [&](int vt) { return (vt < ts.sink_tiles ? vt : ts.first + vt - ts.sink_tiles) * kKeys; };
-    auto pieces_of = [&](int vt) {
-        Pieces r;
-        r.valid = 0;
-        const int key0 = key0_of(vt);
-#pragma unroll
-        for (int g = 0; g < S::kPieces; ++g) {
-            const int key = key0 + 16 * g, i = key >> p.c.page_shift;
-            const int page = table[i < p.c.table_stride ? i : p.c.table_stride - 1];
-            const bool ok = i < p.c.table_stride && page >= 0 && page < p.c.n_pages;
-            r.valid |= ok ? 1u << g : 0u;
-            r.row[g] = ((static_cast<int64_t>(ok ? page : 0) * p.c.n_heads + kvh) << p.c.page_shift) + (key & page_mask);
-        }
-        return r;
-    };
 
     // LDS addresses.  A row's 16-byte pieces are swizzled by functions of the row that are linear over its bits, so every
     // address below is one base per lane, an exclusive or with a constant and a constant offset.  The bases are hidden from
@@ -257,13 +280,13 @@ __global__ __launch_bounds__(256, 2) void paged_attn_many_kernel(const AttnJob j
     // lane 16 bytes; the place in the LDS follows the lane, so the swizzle is applied to the source (K and V differ)
     const int lrow = (wave * S::kRpi & 15) + lane / kChunks, lchunk = lane % kChunks;
     const uint32_t voff_k = lrow * kRowBytes + (lchunk ^ swz_k<D>(lrow)) * 16, voff_v = lrow * kRowBytes + (lchunk ^ swz_v<D>(lrow)) * 16;
-    auto issue16 = [&](const Pieces& pc, int buf) __attribute__((always_inline)) {
+    auto issue16 = [&](const Pieces<S::kPieces>& pc, int buf) __attribute__((always_inline)) {
         const uint32_t dst = __builtin_amdgcn_readfirstlane(lds0 + buf * 2 * kTile + wave * 1024);
         static_for<S::kLoads>([&](auto ic) {
             constexpr int I = decltype(ic)::value;
             int64_t at;
             if constexpr (S::kRpi == 8) {
-                const int64_t even = pc.row[2 * I], odd = pc.row[2 * I + 1];
+                const uint32_t even = pc.row[2 * I], odd = pc.row[2 * I + 1];
                 at = wave & 2 ? odd : even;
             } else {
                 at = pc.row[I];
@@ -278,12 +301,12 @@ __global__ __launch_bounds__(256, 2) void paged_attn_many_kernel(const AttnJob j
     const int r8 = (lane / kLpr) * kLoads8, c8 = lane % kLpr;  // first row (of the wave's), pair of 16-byte pieces
     u32x4 k8[E4M3 ? kLoads8 : 1], v8[E4M3 ? kLoads8 : 1];
     uint32_t ke8 = 0, ve8 = 0;
-    auto issue8 = [&](const Pieces& pc) __attribute__((always_inline)) {
+    auto issue8 = [&](const Pieces<S::kPieces>& pc) __attribute__((always_inline)) {
         if constexpr (E4M3) {
             int64_t at = pc.row[0];
 #pragma unroll
             for (int g = 1; g < S::kPieces; ++g) {
-                const int64_t x = pc.row[g];
+                const uint32_t x = pc.row[g];
                 at = wave == g ? x : at;
             }
             const char* kp = p.c.k + (at + r8) * D + 16 * c8;
@@ -323,7 +346,7 @@ __global__ __launch_bounds__(256, 2) void paged_attn_many_kernel(const AttnJob j
     // ---- first tile, queries
     uint32_t valid = 0;  // of the tile that is about to be used: which of its pieces exist
     if (vt0 < vt1) {
-        const Pieces pc = pieces_of(vt0);
+        const Pieces<S::kPieces> pc = pages.tile<S::kPieces>(key0_of(vt0));
         valid = pc.valid;
         if constexpr (E4M3) issue8(pc);
         else issue16(pc, 0);
@@ -362,13 +385,24 @@ __global__ __launch_bounds__(256, 2) void paged_attn_many_kernel(const AttnJob j
             for (int e = 0; e < 16; ++e) sacc[kk][e] = 0.0f;
         uint32_t kb = tile_base + get_k;
         asm volatile("" : "+v"(kb));
+        // (fragments three steps ahead of their use; consecutive products alternate between the two accumulators)
+        auto k_frag = [&](int s, int kk) { return *lds<const u16x8>((kb ^ (s << 5)) + kk * 32 * kRowBytes); };
+        u16x8 kf[3][2];
 #pragma unroll
-        for (int s = 0; s < D / 16; ++s)
-#pragma unroll
-            for (int kk = 0; kk < 2; ++kk) {
-                const u16x8 kf = *lds<const u16x8>((kb ^ (s << 5)) + kk * 32 * kRowBytes);
-                sacc[kk] = mfma32<F16>(kf, qf[s], sacc[kk]);
+        for (int s = 0; s < 3; ++s) {
+            kf[s][0] = k_frag(s, 0);
+            kf[s][1] = k_frag(s, 1);
+        }
+        static_for<D / 16>([&](auto sc) {
+            constexpr int T = decltype(sc)::value;
+            sacc[0] = mfma32<F16>(kf[T % 3][0], qf[T], sacc[0]);
+            sacc[1] = mfma32<F16>(kf[T % 3][1], qf[T], sacc[1]);
+            if constexpr (T + 3 < D / 16) {
+                kf[T % 3][0] = k_frag(T + 3, 0);
+                kf[T % 3][1] = k_frag(T + 3, 1);
             }
+            __builtin_amdgcn_sched_barrier(0);
+        });
         if constexpr (edge) {
 #pragma unroll
             for (int kk = 0; kk < 2; ++kk)
@@ -402,8 +436,7 @@ __global__ __launch_bounds__(256, 2) void paged_attn_many_kernel(const AttnJob j
         }
         float psum = 0.0f;
         u32x4 pf[2][2];
-#pragma unroll
-        for (int kk = 0; kk < 2; ++kk)
+        auto weigh = [&](int kk) __attribute__((always_inline)) {
 #pragma unroll
             for (int s2 = 0; s2 < 2; ++s2)
 #pragma unroll
@@ -413,11 +446,7 @@ __global__ __launch_bounds__(256, 2) void paged_attn_many_kernel(const AttnJob j
                     psum += a + b;
                     pf[kk][s2][j / 2] = pack_elem2<F16>(a, b);
                 }
-        l_run = l_run * alpha + psum;
-#pragma unroll
-        for (int kk = 0; kk < 2; ++kk)
-#pragma unroll
-            for (int s2 = 0; s2 < 2; ++s2) asm volatile("" : "+v"(pf[kk][s2]));  // (packed here: not in 32 bits up to their use)
+        };
         uint32_t vb = tile_base + kTile + get_v;
         asm volatile("" : "+v"(vb));
         auto v_frag = [&](int kk, int s2, int mt) {  // rows 8 x + 4 h + q of the 16: the swizzle turns by 2 x, the channels by 4 mt
@@ -430,6 +459,13 @@ __global__ __launch_bounds__(256, 2) void paged_attn_many_kernel(const AttnJob j
         using O = OddValues<F16>;
         bool special = false;
         if constexpr (edge) {
+            weigh(0);
+            weigh(1);
+            l_run = l_run * alpha + psum;
+#pragma unroll
+            for (int kk = 0; kk < 2; ++kk)
+#pragma unroll
+                for (int s2 = 0; s2 < 2; ++s2) asm volatile("" : "+v"(pf[kk][s2]));  // (packed here: not in 32 bits up to their use)
             uint32_t any = 0;
 #pragma unroll
             for (int kk = 0; kk < 2; ++kk)
@@ -442,12 +478,16 @@ __global__ __launch_bounds__(256, 2) void paged_attn_many_kernel(const AttnJob j
             special = __any((any & O::kSign) != 0);
         }
         if (!special) {
+            // (inside the mask: the products of one half of the keys have the exponentials of the other to overlap with)
 #pragma unroll
-            for (int kk = 0; kk < 2; ++kk)
+            for (int kk = 0; kk < 2; ++kk) {
+                if constexpr (!edge) weigh(kk);
 #pragma unroll
                 for (int s2 = 0; s2 < 2; ++s2)
 #pragma unroll
                     for (int mt = 0; mt < kMt; ++mt) oacc[mt] = times(v_frag(kk, s2, mt), pf[kk][s2], oacc[mt]);
+            }
+            if constexpr (!edge) l_run = l_run * alpha + psum;
         } else {
 #pragma unroll
             for (int kk = 0; kk < 2; ++kk)
@@ -471,26 +511,39 @@ __global__ __launch_bounds__(256, 2) void paged_attn_many_kernel(const AttnJob j
         }
     };
 
-    int buf = 0;
-    for (int vt = vt0; vt < vt1; ++vt) {
+    // Tiles [inner0, inner1) lie inside every row's mask.  They run in a loop of their own: with both kinds in one loop the
+    // accumulators would be copied between them, 64 registers a tile.
+    const int first_row = ts.row0 / p.group, last_row = (ts.row0 + S::kRowTile - 1 < ts.n_rows ? ts.row0 + S::kRowTile - 1 : ts.n_rows - 1) / p.group;
+    const int all_lo = lo_of(ts.pos0 + last_row), from = (all_lo + kKeys - 1) / kKeys - ts.first;
+    const int inner0 = ts.sink_tiles + (from > 0 ? from : 0), to = ts.sink_tiles + hi_of(ts.pos0 + first_row) / kKeys - ts.first;
+    const int inner1 = to < vt1 ? to : vt1;
+    constexpr uint32_t kAll = (1u << S::kPieces) - 1;
+    int buf = 0, vt = vt0;
+    auto turn = [&](auto edge_c) __attribute__((always_inline)) {
+        constexpr bool edge = decltype(edge_c)::value;
         if constexpr (E4M3) put8(lds0 + buf * 2 * kTile);
         else asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // this wave's loads of the tile are in
         __syncthreads();  // and all others'; and no wave reads the other buffer any more
         const uint32_t now = valid;
         if (vt + 1 < vt1) {
-            const Pieces pc = pieces_of(vt + 1);
+            const Pieces<S::kPieces> pc = pages.tile<S::kPieces>(key0_of(vt + 1));
             valid = pc.valid;
             if constexpr (E4M3) issue8(pc);
             else issue16(pc, buf ^ 1);
         }
         const int key0 = key0_of(vt);
-        // (a tile may be hidden from every row of a wave: the keys behind a prompt's first rows, the window of its last ones)
-        if (has_rows && key0 < w_hi_max && (key0 + kKeys > w_lo_min || key0 < p.sinks)) {
-            const bool inside = key0 + kKeys <= w_hi_min && (key0 >= w_lo_max || key0 + kKeys <= p.sinks) && now == (1u << S::kPieces) - 1;
-            if (inside) compute(lds0 + buf * 2 * kTile, key0, now, std::false_type{});
-            else compute(lds0 + buf * 2 * kTile, key0, now, std::true_type{});
-        }
+        // (an edge tile may be hidden from every row of a wave: the keys behind a prompt's first rows, the window of its last)
+        if (!edge || (has_rows && key0 < w_hi_max && (key0 + kKeys > w_lo_min || key0 < p.sinks))) compute(lds0 + buf * 2 * kTile, key0, now, edge_c);
         buf ^= 1;
+        ++vt;
+    };
+    while (vt < vt1) {
+        if (vt >= inner0 && vt < inner1 && valid == kAll) {
+            do turn(std::false_type{});
+            while (vt < inner1 && valid == kAll);
+        } else {
+            turn(std::true_type{});
+        }
     }
 
     // ---- results: lane (l31, h) holds of its row the channels 32 mt + 8 (e >> 2) + 4 h + (e & 3)
@@ -595,27 +648,8 @@ __global__ __launch_bounds__(64 * KW, (NQ == 1 ? 2 : 1)) void paged_attn_few_ker
     }
 
     // ---- key tiles
-    const const_i32 table = (const_i32)(p.c.block_table + static_cast<int64_t>(ts.b) * p.c.table_stride);
-    const int page_mask = (1 << p.c.page_shift) - 1;
+    const PageWalk pages(p.c, ts.b, kvh);
     auto key0_of = [&](int vt) { return (vt < ts.sink_tiles ? vt : ts.first + vt - ts.sink_tiles) * kKeys; };
-    struct Pieces {
-        int64_t row[2];
-        uint32_t valid;
-    };
-    auto pieces_of = [&](int vt) {
-        Pieces r;
-        r.valid = 0;
-        const int key0 = key0_of(vt);
-#pragma unroll
-        for (int u = 0; u < 2; ++u) {
-            const int key = key0 + 16 * u, i = key >> p.c.page_shift;
-            const int page = table[i < p.c.table_stride ? i : p.c.table_stride - 1];
-            const bool ok = i < p.c.table_stride && page >= 0 && page < p.c.n_pages;
-            r.valid |= ok ? 1u << u : 0u;
-            r.row[u] = ((static_cast<int64_t>(ok ? page : 0) * p.c.n_heads + kvh) << p.c.page_shift) + (key & page_mask);
-        }
-        return r;
-    };
     const uint32_t own_base = __builtin_amdgcn_readfirstlane(lds_addr_of(smem + wave * S::kBufs * kTile));
     const int lrow = lane / kChunks, lchunk = lane % kChunks;
     uint32_t voff_v[E4M3 ? 1 : S::kVar];
@@ -636,10 +670,10 @@ __global__ __launch_bounds__(64 * KW, (NQ == 1 ? 2 : 1)) void paged_attn_few_ker
         u32x4 w[2][kKs];
         uint32_t exp[2];
     };
-    auto issue = [&](const Pieces& pc, Keys& k, int buf) __attribute__((always_inline)) {
+    auto issue = [&](const Pieces<2>& pc, Keys& k, int buf) __attribute__((always_inline)) {
         if constexpr (E4M3) {
-            const int64_t even = pc.row[0], odd = pc.row[1];
-            const int64_t at = (r8 & 16 ? odd : even) + (r8 & 15);
+            const uint32_t even = pc.row[0], odd = pc.row[1];
+            const int64_t at = static_cast<int64_t>(r8 & 16 ? odd : even) + (r8 & 15);
             const char* vp = p.c.v + at * D + 16 * c8;
 #pragma unroll
             for (int i = 0; i < kLoads8; ++i) v8[i] = *reinterpret_cast<const u32x4*>(vp + i * D);
@@ -649,12 +683,12 @@ __global__ __launch_bounds__(64 * KW, (NQ == 1 ? 2 : 1)) void paged_attn_few_ker
             const uint32_t dst = __builtin_amdgcn_readfirstlane(own_base + buf * kTile);
             static_for<S::kLoads>([&](auto ic) {
                 constexpr int I = decltype(ic)::value;
-                lds_dma16(uniform(p.c.v + pc.row[I * S::kRpi / 16] * kRowBytes), voff_v[I % S::kVar], dst + I * 1024);
+                lds_dma16(uniform(p.c.v + static_cast<int64_t>(pc.row[I * S::kRpi / 16]) * kRowBytes), voff_v[I % S::kVar], dst + I * 1024);
             });
         }
 #pragma unroll
         for (int u = 0; u < 2; ++u) {
-            const char* kp = uniform(p.c.k + pc.row[u] * kStored);
+            const char* kp = uniform(p.c.k + static_cast<int64_t>(pc.row[u]) * kStored);
 #pragma unroll
             for (int s = 0; s < kKs; ++s) k.w[u][s] = *reinterpret_cast<const u32x4*>(kp + voff_k + 64 * s);
             if constexpr (E4M3) k.exp[u] = reinterpret_cast<const uint8_t*>(uniform(reinterpret_cast<const char*>(p.c.k_exp) + pc.row[u]))[static_cast<uint32_t>(col)];
@@ -786,7 +820,7 @@ __global__ __launch_bounds__(64 * KW, (NQ == 1 ? 2 : 1)) void paged_attn_few_ker
     uint32_t valid = 0;  // of the tile that is about to be used: which of its pieces exist
     Keys ka, kb;
     if (vt < vt1) {
-        const Pieces pc = pieces_of(vt);
+        const Pieces<2> pc = pages.tile<2>(key0_of(vt));
         valid = pc.valid;
         issue(pc, ka, 0);
     }
@@ -812,7 +846,7 @@ __global__ __launch_bounds__(64 * KW, (NQ == 1 ? 2 : 1)) void paged_attn_few_ker
         const uint32_t now = valid;
         const int next = vt + KW, key0 = key0_of(vt);
         if (next < vt1) {
-            const Pieces pc = pieces_of(next);
+            const Pieces<2> pc = pages.tile<2>(key0_of(next));
             valid = pc.valid;
             issue(pc, next_k, E4M3 ? 0 : buf ^ 1);
         }
