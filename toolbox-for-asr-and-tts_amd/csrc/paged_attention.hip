@@ -28,11 +28,13 @@ namespace asrfe {
 typedef short v4s __attribute__((ext_vector_type(4)));
 typedef const __attribute__((address_space(4))) int32_t* const_i32;
 
-// The same address in scalar registers, for a value that is the same in every lane.
-__device__ __forceinline__ const char* uniform(const char* p) {
+// The same address in scalar registers, for a value that is the same in every lane.  (In the global address space: loads
+// through a pointer made of a number would be flat ones, which the LDS counter waits for, too.)
+typedef const __attribute__((address_space(1))) char* global_ptr;
+__device__ __forceinline__ global_ptr uniform(const char* p) {
     const uint64_t a = reinterpret_cast<uint64_t>(p);
     const uint32_t lo = __builtin_amdgcn_readfirstlane(static_cast<uint32_t>(a)), hi = __builtin_amdgcn_readfirstlane(static_cast<uint32_t>(a >> 32));
-    return reinterpret_cast<const char*>(static_cast<uint64_t>(hi) << 32 | lo);
+    return (global_ptr)(static_cast<uint64_t>(hi) << 32 | lo);
 }
 
 // Two results in 16 bits.  A mean of fp16 values can leave their range by its rounding errors only: it stays inside;
@@ -224,6 +226,30 @@ struct PageWalk {
     }
 };
 
+// What one row sees: positions [lo, hi) and the first `sinks`, of pieces that exist.  N scores of a lane in runs of four
+// positions, run e / 4 of them at first(e / 4), in the piece of the same number that piece(e / 4) gives.
+struct RowMask {
+    int lo, hi, sinks;
+    template <int N, class First, class Piece, class Score>
+    __device__ __forceinline__ void hide(int key0, uint32_t valid, uint32_t all, First&& first, Piece&& piece, Score&& score) const {
+        const uint32_t n = static_cast<uint32_t>(hi > lo ? hi - lo : 0);
+        const int base = key0 - lo;
+        const bool sink_tile = key0 < sinks;  // (the same in every lane)
+#pragma unroll
+        for (int e = 0; e < N; ++e) {
+            const int at = first(e / 4) + (e & 3);
+            bool see = static_cast<uint32_t>(base + at) < n;
+            if (sink_tile) see = see | ((key0 + at < sinks) & (key0 + at < hi));
+            score(e) = see ? score(e) : -INFINITY;
+        }
+        if (valid != all) {
+#pragma unroll
+            for (int e = 0; e < N; ++e)
+                if (!((valid >> piece(e / 4)) & 1)) score(e) = -INFINITY;
+        }
+    }
+};
+
 // ---- many rows: prompts ------------------------------------------------------------------------------------------------
 // Four waves with 32 rows each share key tiles of 64 positions in the LDS: tile t + 1 arrives while tile t is used.
 template <int D, bool E4M3>
@@ -237,10 +263,13 @@ struct ManyShape {
 };
 
 template <int D, bool F16, bool E4M3>
-__global__ __launch_bounds__(256, 2) void paged_attn_many_kernel(const AttnJob job) {
+__global__ __launch_bounds__(256, (D == 64 && !E4M3 ? 3 : 2)) void paged_attn_many_kernel(const AttnJob job) {
     using S = ManyShape<D, E4M3>;
     constexpr int kKeys = S::kKeys, kRowBytes = S::kRowBytes, kTile = S::kTile, kChunks = kRowBytes / 16, kMt = D / 32;
+    constexpr uint32_t kAll = (1u << S::kPieces) - 1;
+    using O = OddValues<F16>;
     __shared__ __attribute__((aligned(1024))) char smem[4 * kTile];
+    __shared__ int odd_tile;  // the last edge tile in whose V an infinity or NaN was found
     // (no saturate_fp16_conversions here: in that mode the matrix instructions lose infinities and NaN in their accumulators)
     const PagedAttnParams& p = job.p;
     const int tid = threadIdx.x, lane = tid & 63, l31 = lane & 31, h = lane >> 5;
@@ -291,8 +320,8 @@ __global__ __launch_bounds__(256, 2) void paged_attn_many_kernel(const AttnJob j
             } else {
                 at = pc.row[I];
             }
-            lds_dma16(uniform(p.c.k + at * kRowBytes), voff_k, dst + I * 4096);
-            lds_dma16(uniform(p.c.v + at * kRowBytes), voff_v, dst + kTile + I * 4096);
+            lds_dma16((const void*)uniform(p.c.k + at * kRowBytes), voff_k, dst + I * 4096);
+            lds_dma16((const void*)uniform(p.c.v + at * kRowBytes), voff_v, dst + kTile + I * 4096);
         });
     };
     // e4m3, through registers: a wave takes a piece, a lane 16 codes of each of kLoads8 consecutive rows, so that their
@@ -376,7 +405,7 @@ __global__ __launch_bounds__(256, 2) void paged_attn_many_kernel(const AttnJob j
         for (int e = 0; e < 16; ++e) oacc[mt][e] = 0.0f;
     float mc = -INFINITY, l_run = 0.0f;  // running maximum (scaled, base 2) and sum of this lane's half of the keys
 
-    auto compute = [&](uint32_t tile_base, int key0, uint32_t exist, auto edge_c) __attribute__((always_inline)) {
+    auto compute = [&](uint32_t tile_base, int key0, uint32_t exist, bool special, auto edge_c) __attribute__((always_inline)) {
         constexpr bool edge = decltype(edge_c)::value;
         f32x16 sacc[2];
 #pragma unroll
@@ -403,15 +432,28 @@ __global__ __launch_bounds__(256, 2) void paged_attn_many_kernel(const AttnJob j
             }
             __builtin_amdgcn_sched_barrier(0);
         });
+        uint32_t vb = tile_base + kTile + get_v;
+        asm volatile("" : "+v"(vb));
+        auto v_frag = [&](int kk, int s2, int mt) {  // rows 8 x + 4 h + q of the 16: the swizzle turns by 2 x, the channels by 4 mt
+            const uint32_t at = vb ^ (mt * 64);
+            const v4s a = __builtin_amdgcn_ds_read_tr16_b64_v4i16(lds<v4s>(at + (kk * 32 + s2 * 16) * kRowBytes));
+            const v4s b = __builtin_amdgcn_ds_read_tr16_b64_v4i16(lds<v4s>((at ^ 32) + (kk * 32 + s2 * 16 + 8) * kRowBytes));
+            return __builtin_bit_cast(u32x4, __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7));
+        };
+        // the products' steps: 32-position half kk, 16 positions s2 of it, 32 channels mt; fragments are read four steps ahead
+        constexpr int kSteps = 4 * kMt, kRing = 4;
+        u32x4 vf[kRing];
+        auto v_step = [&](auto tc) __attribute__((always_inline)) {
+            constexpr int T = decltype(tc)::value;
+            vf[T % kRing] = v_frag(T / (2 * kMt), (T / kMt) & 1, T % kMt);
+        };
+        if constexpr (!edge) static_for<kRing>([&](auto tc) { v_step(tc); });
         if constexpr (edge) {
+            const RowMask mask{lo, hi, p.sinks};
 #pragma unroll
             for (int kk = 0; kk < 2; ++kk)
-#pragma unroll
-                for (int e = 0; e < 16; ++e) {
-                    const int j = key0 + kk * 32 + (e & 3) + 8 * (e >> 2) + 4 * h;
-                    const bool see = (j < hi) & ((j >= lo) | (j < p.sinks)) & (((exist >> (kk * 2 + (e >> 3))) & 1) != 0);
-                    sacc[kk][e] = see ? sacc[kk][e] : -INFINITY;
-                }
+                mask.hide<16>(key0, exist, kAll, [&](int r) { return kk * 32 + 8 * r + 4 * h; }, [&](int r) { return 2 * kk + (r >> 1); },
+                              [&](int e) -> float& { return reinterpret_cast<float*>(&sacc[kk])[e]; });
         }
         float rmax = sacc[0][0];
 #pragma unroll
@@ -436,58 +478,43 @@ __global__ __launch_bounds__(256, 2) void paged_attn_many_kernel(const AttnJob j
         }
         float psum = 0.0f;
         u32x4 pf[2][2];
-        auto weigh = [&](int kk) __attribute__((always_inline)) {
-#pragma unroll
-            for (int s2 = 0; s2 < 2; ++s2)
-#pragma unroll
-                for (int j = 0; j < 8; j += 2) {
-                    const float a = __builtin_amdgcn_exp2f(fmaf(sacc[kk][8 * s2 + j], c, -sub));
-                    const float b = __builtin_amdgcn_exp2f(fmaf(sacc[kk][8 * s2 + j + 1], c, -sub));
-                    psum += a + b;
-                    pf[kk][s2][j / 2] = pack_elem2<F16>(a, b);
-                }
-        };
-        uint32_t vb = tile_base + kTile + get_v;
-        asm volatile("" : "+v"(vb));
-        auto v_frag = [&](int kk, int s2, int mt) {  // rows 8 x + 4 h + q of the 16: the swizzle turns by 2 x, the channels by 4 mt
-            const uint32_t at = vb ^ (mt * 64);
-            const v4s a = __builtin_amdgcn_ds_read_tr16_b64_v4i16(lds<v4s>(at + (kk * 32 + s2 * 16) * kRowBytes));
-            const v4s b = __builtin_amdgcn_ds_read_tr16_b64_v4i16(lds<v4s>((at ^ 32) + (kk * 32 + s2 * 16 + 8) * kRowBytes));
-            return __builtin_bit_cast(u32x4, __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7));
+        auto weigh = [&](auto qc) __attribute__((always_inline)) {  // two scores: pair Q of the 16 of a lane
+            constexpr int Q = decltype(qc)::value, kk = Q / 8, e = 2 * (Q % 8);
+            const float a = __builtin_amdgcn_exp2f(fmaf(sacc[kk][e], c, -sub));
+            const float b = __builtin_amdgcn_exp2f(fmaf(sacc[kk][e + 1], c, -sub));
+            psum += a + b;
+            pf[kk][e / 8][(e % 8) / 2] = pack_elem2<F16>(a, b);
         };
         auto times = [&](const u32x4 v, const u32x4 w, const f32x16 acc) { return mfma32<F16>(__builtin_bit_cast(u16x8, v), __builtin_bit_cast(u16x8, w), acc); };
-        using O = OddValues<F16>;
-        bool special = false;
         if constexpr (edge) {
-            weigh(0);
-            weigh(1);
+            static_for<16>([&](auto qc) { weigh(qc); });
             l_run = l_run * alpha + psum;
 #pragma unroll
             for (int kk = 0; kk < 2; ++kk)
 #pragma unroll
                 for (int s2 = 0; s2 < 2; ++s2) asm volatile("" : "+v"(pf[kk][s2]));  // (packed here: not in 32 bits up to their use)
-            uint32_t any = 0;
-#pragma unroll
-            for (int kk = 0; kk < 2; ++kk)
-#pragma unroll
-                for (int s2 = 0; s2 < 2; ++s2) {
-#pragma unroll
-                    for (int mt = 0; mt < kMt; ++mt) any |= O::any(v_frag(kk, s2, mt));
-                    __builtin_amdgcn_sched_barrier(0);
-                }
-            special = __any((any & O::kSign) != 0);
         }
         if (!special) {
-            // (inside the mask: the products of one half of the keys have the exponentials of the other to overlap with)
+            if constexpr (edge) {
 #pragma unroll
-            for (int kk = 0; kk < 2; ++kk) {
-                if constexpr (!edge) weigh(kk);
+                for (int kk = 0; kk < 2; ++kk)
 #pragma unroll
-                for (int s2 = 0; s2 < 2; ++s2)
+                    for (int s2 = 0; s2 < 2; ++s2)
 #pragma unroll
-                    for (int mt = 0; mt < kMt; ++mt) oacc[mt] = times(v_frag(kk, s2, mt), pf[kk][s2], oacc[mt]);
+                        for (int mt = 0; mt < kMt; ++mt) oacc[mt] = times(v_frag(kk, s2, mt), pf[kk][s2], oacc[mt]);
+            } else {
+                // the products of the first half of the keys have the exponentials of the second between them
+                static_for<8>([&](auto qc) { weigh(qc); });
+                static_for<kSteps>([&](auto tc) {
+                    constexpr int T = decltype(tc)::value, kk = T / (2 * kMt), s2 = (T / kMt) & 1, mt = T % kMt;
+                    const u32x4 v = vf[T % kRing];
+                    if constexpr (T + kRing < kSteps) v_step(IC<T + kRing>{});
+                    oacc[mt] = times(v, pf[kk][s2], oacc[mt]);
+                    if constexpr (kk == 0) static_for<4 / kMt>([&](auto xc) { weigh(IC<8 + T * (4 / kMt) + decltype(xc)::value>{}); });
+                    __builtin_amdgcn_sched_barrier(0);
+                });
+                l_run = l_run * alpha + psum;
             }
-            if constexpr (!edge) l_run = l_run * alpha + psum;
         } else {
 #pragma unroll
             for (int kk = 0; kk < 2; ++kk)
@@ -517,8 +544,8 @@ __global__ __launch_bounds__(256, 2) void paged_attn_many_kernel(const AttnJob j
     const int all_lo = lo_of(ts.pos0 + last_row), from = (all_lo + kKeys - 1) / kKeys - ts.first;
     const int inner0 = ts.sink_tiles + (from > 0 ? from : 0), to = ts.sink_tiles + hi_of(ts.pos0 + first_row) / kKeys - ts.first;
     const int inner1 = to < vt1 ? to : vt1;
-    constexpr uint32_t kAll = (1u << S::kPieces) - 1;
     int buf = 0, vt = vt0;
+    if (tid == 0) odd_tile = -1;  // (every use of it lies behind a barrier)
     auto turn = [&](auto edge_c) __attribute__((always_inline)) {
         constexpr bool edge = decltype(edge_c)::value;
         if constexpr (E4M3) put8(lds0 + buf * 2 * kTile);
@@ -532,8 +559,18 @@ __global__ __launch_bounds__(256, 2) void paged_attn_many_kernel(const AttnJob j
             else issue16(pc, buf ^ 1);
         }
         const int key0 = key0_of(vt);
+        // In an edge tile a hidden value may meet a weight of zero: every wave looks through 16 of its rows of V.
+        bool special = false;
+        if constexpr (edge) {
+            uint32_t any = 0;
+#pragma unroll
+            for (int i = 0; i < 16 * kRowBytes / 1024; ++i) any |= O::any(*lds<const u32x4>(lds0 + (2 * buf + 1) * kTile + (wave * 16 * kRowBytes + i * 1024) + lane * 16));
+            if (__any((any & O::kSign) != 0)) odd_tile = vt;
+            __syncthreads();
+            special = __builtin_amdgcn_readfirstlane(odd_tile) == vt;
+        }
         // (an edge tile may be hidden from every row of a wave: the keys behind a prompt's first rows, the window of its last)
-        if (!edge || (has_rows && key0 < w_hi_max && (key0 + kKeys > w_lo_min || key0 < p.sinks))) compute(lds0 + buf * 2 * kTile, key0, now, edge_c);
+        if (!edge || (has_rows && key0 < w_hi_max && (key0 + kKeys > w_lo_min || key0 < p.sinks))) compute(lds0 + buf * 2 * kTile, key0, now, special, edge_c);
         buf ^= 1;
         ++vt;
     };
@@ -683,15 +720,15 @@ __global__ __launch_bounds__(64 * KW, (NQ == 1 ? 2 : 1)) void paged_attn_few_ker
             const uint32_t dst = __builtin_amdgcn_readfirstlane(own_base + buf * kTile);
             static_for<S::kLoads>([&](auto ic) {
                 constexpr int I = decltype(ic)::value;
-                lds_dma16(uniform(p.c.v + static_cast<int64_t>(pc.row[I * S::kRpi / 16]) * kRowBytes), voff_v[I % S::kVar], dst + I * 1024);
+                lds_dma16((const void*)uniform(p.c.v + static_cast<int64_t>(pc.row[I * S::kRpi / 16]) * kRowBytes), voff_v[I % S::kVar], dst + I * 1024);
             });
         }
 #pragma unroll
         for (int u = 0; u < 2; ++u) {
-            const char* kp = uniform(p.c.k + static_cast<int64_t>(pc.row[u]) * kStored);
+            const global_ptr kp = uniform(p.c.k + static_cast<int64_t>(pc.row[u]) * kStored);
 #pragma unroll
-            for (int s = 0; s < kKs; ++s) k.w[u][s] = *reinterpret_cast<const u32x4*>(kp + voff_k + 64 * s);
-            if constexpr (E4M3) k.exp[u] = reinterpret_cast<const uint8_t*>(uniform(reinterpret_cast<const char*>(p.c.k_exp) + pc.row[u]))[static_cast<uint32_t>(col)];
+            for (int s = 0; s < kKs; ++s) k.w[u][s] = *(const __attribute__((address_space(1))) u32x4*)(kp + voff_k + 64 * s);
+            if constexpr (E4M3) k.exp[u] = (uint8_t)uniform(reinterpret_cast<const char*>(p.c.k_exp) + pc.row[u])[static_cast<uint32_t>(col)];
         }
     };
     const uint32_t put_v = r8 * kRowBytes + ((2 * c8) ^ swz_v<D>(r8)) * 16;
@@ -737,14 +774,9 @@ __global__ __launch_bounds__(64 * KW, (NQ == 1 ? 2 : 1)) void paged_attn_few_ker
 #pragma unroll
         for (int n = 0; n < NQ; ++n) {
             if constexpr (edge) {
-#pragma unroll
-                for (int u = 0; u < 2; ++u)
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        const int j = key0 + 16 * u + 4 * g + i;
-                        const bool see = (j < hi[n]) & ((j >= lo[n]) | (j < p.sinks)) & (((valid >> u) & 1) != 0);
-                        sacc[n][u][i] = see ? sacc[n][u][i] : -INFINITY;
-                    }
+                const RowMask mask{lo[n], hi[n], p.sinks};
+                mask.hide<8>(key0, valid, 3, [&](int u) { return 16 * u + 4 * g; }, [&](int u) { return u; },
+                             [&](int e) -> float& { return reinterpret_cast<float*>(&sacc[n][e >> 2])[e & 3]; });
             }
             float rmax = sacc[n][0][0];
 #pragma unroll
