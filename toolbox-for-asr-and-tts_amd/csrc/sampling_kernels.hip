@@ -81,6 +81,14 @@ struct SampleLds {
     int total;
 };
 
+// (a function's own variable, so that every access is known to be one of the LDS: through a reference kept in an object
+// they would be flat ones)
+template <int NT>
+__device__ __forceinline__ SampleLds<NT>& sample_lds() {
+    __shared__ SampleLds<NT> s;
+    return s;
+}
+
 template <int DT, int NT>
 struct Sampler {
     static constexpr int kWaves = NT / 64;
@@ -88,15 +96,14 @@ struct Sampler {
     static constexpr int kSub = 1024 / NT;  // partial maxima of a thread
 
     const SampleParams& p;
-    SampleLds<NT>& s;
     const int tid, lane, wave;
     const char* row;
     int head, n_vec, n_steps;  // elements before the first 16-byte boundary, 16-byte pieces, steps of 64 of them
     float top, low;            // largest logit, least logit with a weight
     double a;                  // log2(e) / T
 
-    __device__ Sampler(const SampleParams& p_, SampleLds<NT>& s_, int r)
-        : p(p_), s(s_), tid(threadIdx.x), lane(threadIdx.x & 63), wave(__builtin_amdgcn_readfirstlane(threadIdx.x >> 6)) {
+    __device__ __forceinline__ Sampler(const SampleParams& p_, int r)
+        : p(p_), tid(threadIdx.x), lane(threadIdx.x & 63), wave(__builtin_amdgcn_readfirstlane(threadIdx.x >> 6)) {
         constexpr int kSize = DT == ASRFE_DT_F32 ? 4 : 2;
         row = static_cast<const char*>(p.logits) + static_cast<int64_t>(r) * p.ld * kSize;
         head = static_cast<int>((16 - (reinterpret_cast<uintptr_t>(row) & 15)) & 15) / kSize;
@@ -105,94 +112,70 @@ struct Sampler {
         n_steps = (n_vec + 63) / 64;
     }
 
-    __device__ float one(int i) const {
-        if constexpr (DT == ASRFE_DT_F32) return reinterpret_cast<const float*>(row)[i];
-        else if constexpr (DT == ASRFE_DT_F16) return static_cast<float>(reinterpret_cast<const _Float16*>(row)[i]);
-        else return __uint_as_float(static_cast<uint32_t>(reinterpret_cast<const uint16_t*>(row)[i]) << 16);
-    }
-    __device__ static void widen(const uint4 w, float (&x)[kVec]) {
-        if constexpr (DT == ASRFE_DT_F32) {
-            x[0] = __uint_as_float(w.x); x[1] = __uint_as_float(w.y); x[2] = __uint_as_float(w.z); x[3] = __uint_as_float(w.w);
-        } else {
-            constexpr bool kF16 = DT == ASRFE_DT_F16;
-            unpack_elem2<kF16>(w.x, x[0], x[1]);
-            unpack_elem2<kF16>(w.y, x[2], x[3]);
-            unpack_elem2<kF16>(w.z, x[4], x[5]);
-            unpack_elem2<kF16>(w.w, x[6], x[7]);
-        }
-    }
     // The row in steps: step 0 is the head (one element per lane), then the pieces, then what is left behind the last one.
-    // f(x, i0): this lane's elements i0, i0 + 1, ... (NaN where it has none: no comparison holds for them).
-    template <class F>
-    __device__ void step(int t, F&& f) const {
-        float x[kVec];
+    // This lane's 16 bytes of step t; NaN where it has no elements: no comparison holds for them, and they have no weight.
+    static constexpr uint32_t kNan = DT == ASRFE_DT_F32 ? 0x7fc00000u : DT == ASRFE_DT_F16 ? 0x7e007e00u : 0x7fc07fc0u;
+    __device__ __forceinline__ int first_of(int t) const {  // its first element
+        return t == 0 ? lane : t <= n_steps ? head + ((t - 1) * 64 + lane) * kVec : head + n_vec * kVec + lane;
+    }
+    __device__ __forceinline__ u32x4 load(int t) const {
+        u32x4 w = {kNan, kNan, kNan, kNan};
+        const int i = first_of(t);
         if (t > 0 && t <= n_steps) {
-            const int v = (t - 1) * 64 + lane;
-            const int i0 = head + v * kVec;
-            if (v < n_vec) {
-                widen(*reinterpret_cast<const uint4*>(row + static_cast<int64_t>(i0) * (DT == ASRFE_DT_F32 ? 4 : 2)), x);
-            } else {
+            if (i < head + n_vec * kVec) w = *reinterpret_cast<const u32x4*>(row + static_cast<int64_t>(i) * (16 / kVec));
+        } else if (i < (t == 0 ? head : p.vocab) && t < steps()) {
+            if constexpr (DT == ASRFE_DT_F32) w[0] = reinterpret_cast<const uint32_t*>(row)[i];
+            else w[0] = (kNan & 0xffff0000u) | reinterpret_cast<const uint16_t*>(row)[i];
+        }
+        return w;
+    }
+    __device__ __forceinline__ static void widen(const u32x4 w, float (&x)[kVec]) {
 #pragma unroll
-                for (int e = 0; e < kVec; ++e) x[e] = __builtin_nanf("");
-            }
-            f(x, i0);
-        } else {
-            const int i0 = t == 0 ? lane : head + n_vec * kVec + lane, end = t == 0 ? head : p.vocab;
-#pragma unroll
-            for (int e = 1; e < kVec; ++e) x[e] = __builtin_nanf("");
-            x[0] = i0 < end ? one(i0) : __builtin_nanf("");
-            f(x, i0);
+        for (int i = 0; i < 4; ++i) {
+            if constexpr (DT == ASRFE_DT_F32) x[i] = __uint_as_float(w[i]);
+            else unpack_elem2<DT == ASRFE_DT_F16>(w[i], x[2 * i], x[2 * i + 1]);
         }
     }
-    __device__ int steps() const { return n_steps + 2; }
+    __device__ __forceinline__ int steps() const { return n_steps + 2; }
+    // f(x, i0) for steps t0, t0 + by, ... below t1: this lane's elements i0, i0 + 1, ...  Three loads are in flight.
     template <class F>
-    __device__ void steps_of(int t0, int t1, int by, F&& f) const {
+    __device__ __forceinline__ void steps_of(int t0, int t1, int by, F&& f) const {
+        u32x4 w0 = load(t0), w1 = load(t0 + by), w2;
         for (int t = t0; t < t1; t += by) {
-            if (t + 3 * by < t1 && t > 0 && t + 3 * by < n_steps) {  // four full steps at once: four loads in flight
-                uint4 w[4];
-#pragma unroll
-                for (int k = 0; k < 4; ++k) {
-                    const int i0 = head + ((t + k * by - 1) * 64 + lane) * kVec;
-                    w[k] = *reinterpret_cast<const uint4*>(row + static_cast<int64_t>(i0) * (DT == ASRFE_DT_F32 ? 4 : 2));
-                }
-#pragma unroll
-                for (int k = 0; k < 4; ++k) {
-                    float x[kVec];
-                    widen(w[k], x);
-                    f(x, head + ((t + k * by - 1) * 64 + lane) * kVec);
-                }
-                t += 3 * by;
-            } else {
-                step(t, f);
-            }
+            w2 = load(t + 2 * by);
+            float x[kVec];
+            widen(w0, x);
+            f(x, first_of(t));
+            w0 = w1;
+            w1 = w2;
         }
     }
     // this wave's run of steps: runs follow each other in the order of the vocabulary
-    __device__ int run_of(int w) const {
+    __device__ __forceinline__ int run_of(int w) const {
         const int per = (steps() + kWaves - 1) / kWaves, t = w * per;
         return t < steps() ? t : steps();
     }
     template <class F>
-    __device__ void walk(F&& f) const { steps_of(run_of(wave), run_of(wave + 1), 1, f); }
+    __device__ __forceinline__ void walk(F&& f) const { steps_of(run_of(wave), run_of(wave + 1), 1, f); }
 
-    // weight in multiples of 2^-44; v is at least `low`
-    __device__ u64 fixed(float v) const {
-        const double t = fmax((static_cast<double>(fminf(v, 3.402823466e38f)) - static_cast<double>(fminf(top, 3.402823466e38f))) * a, -200.0);
+    // Weight in multiples of 2^-44.  Below `low`, and for NaN, it comes out as zero: the median of three takes the least.
+    __device__ __forceinline__ u64 weight(float v) const {
+        const double t = fmax((static_cast<double>(__builtin_amdgcn_fmed3f(v, low, top)) - static_cast<double>(top)) * (a * 32.0), -6400.0);
         constexpr double kMagic = 6755399441055744.0;  // 1.5 * 2^52: the sum's low bits are the nearest whole number
-        const double d = t * 32.0 + kMagic;
+        const double d = t + kMagic;
         const int k = static_cast<int>(__builtin_bit_cast(u64, d));
-        const double f = fma(d - kMagic, -1.0 / 32.0, t);  // |f| <= 1 / 64
-        // 2^f = sum (f ln 2)^n / n!, up to n = 4: the next term is below 2e-12
-        double y = fma(f, 0.009618129107628477, 0.05550410866482158);
-        y = fma(f, y, 0.2402265069591007);
-        y = fma(f, y, 0.6931471805599453);
-        y = fma(f, y, 1.0) * s.table[k & 31];
+        const double f = t - (d - kMagic);  // |f| <= 1 / 2, in units of 1 / 32
+        // 2^(f / 32) = sum (f ln 2 / 32)^n / n!, up to n = 4: the next term is below 2e-12
+        double y = fma(f, 9.172562701156919e-09, 1.6938509724835576e-06);
+        y = fma(f, y, 0.00023459619820224656);
+        y = fma(f, y, 0.021660849392498292);
+        y = fma(f, y, 1.0) * sample_lds<NT>().table[k & 31];
         const double scale = __builtin_bit_cast(double, static_cast<u64>(1023 + 44 + (k >> 5)) << 52);
         return __builtin_bit_cast(u64, fma(y, scale, 0x1p52)) & 0xfffffffffffffull;
     }
-    __device__ u64 weight(float v) const { return v >= low ? fixed(v) : 0; }
 
-    __device__ u64 block_sum(u64 v) {
+    __device__ __forceinline__ u64 block_sum(u64 v) {
+        SampleLds<NT>& s = sample_lds<NT>();
         v = wave_sum(v);
         __syncthreads();
         if (lane == 0) s.a[wave] = v;
@@ -205,38 +188,44 @@ struct Sampler {
 
     // Finds the value at which a running sum over falling values first reaches `want` (1 <= want <= the sum of all):
     // the sum over larger values is below `want`, the sum with that value's elements is not.  MASS: sums of weights, else of
-    // elements.
+    // elements.  want = 0: `share` of the sum of all, rounded up.
     template <bool MASS>
-    __device__ float reach(u64 want, u64& before) {
+    __device__ __forceinline__ float reach(u64& want, float share, u64& before) {
+        SampleLds<NT>& s = sample_lds<NT>();
         const float least = MASS ? low : -3.402823466e38f;
         const float span = static_cast<float>(kOctaves / a);  // logits per kOctaves octaves of weight
         const float scale = fminf(static_cast<float>(kBins) / span, 3e38f);
         auto bin1 = [&](float v) {
-            const float d = (top - v) * scale;
-            return static_cast<int>(d < kBins - 1 ? d : (d == d ? kBins - 1.0f : 0.0f));  // (inf - inf: the top itself)
+            const float d = fmaxf((top - v) * scale, 0.0f);  // (0 * inf: the top itself)
+            return static_cast<int>(fminf(d, kBins - 1.0f));
         };
         before = 0;
-        uint32_t lo = 0, hi = 0;  // keys among which the value is, after the first pass
+        float from = least, to = top;  // the value lies among these
+        uint32_t lo = 0, hi = 0;       // and, after the first pass, among these keys
         int shift = -1;
         for (;;) {
             __syncthreads();
             for (int i = tid; i < kBins; i += NT) s.hist[i] = 0;
             __syncthreads();
-            walk([&](const float (&x)[kVec], int) {
+            if (shift < 0) {
+                walk([&](const float (&x)[kVec], int) {
+                    u64 w[kVec];
 #pragma unroll
-                for (int e = 0; e < kVec; ++e) {
-                    if (!(x[e] >= least)) continue;
-                    int b;
-                    if (shift < 0) {
-                        b = bin1(x[e]);
-                    } else {
-                        const uint32_t k = key_of<DT>(x[e]);
-                        if (k < lo || k > hi) continue;
-                        b = static_cast<int>((hi - k) >> shift);
+                    for (int e = 0; e < kVec; ++e) {
+                        w[e] = MASS ? weight(x[e]) : u64{x[e] >= least};
+                        if (e % 4 == 3) __builtin_amdgcn_sched_barrier(0);
                     }
-                    atomicAdd(&s.hist[b], MASS ? fixed(x[e]) : u64{1});
-                }
-            });
+#pragma unroll
+                    for (int e = 0; e < kVec; ++e)
+                        if (w[e] != 0) atomicAdd(&s.hist[bin1(x[e])], w[e]);
+                });
+            } else {
+                walk([&](const float (&x)[kVec], int) {
+#pragma unroll
+                    for (int e = 0; e < kVec; ++e)
+                        if (x[e] >= from && x[e] <= to) atomicAdd(&s.hist[(hi - key_of<DT>(x[e])) >> shift], MASS ? weight(x[e]) : u64{1});
+                });
+            }
             __syncthreads();
             // the bin where `want` is reached: every thread a run of bins
             constexpr int kPer = kBins / NT;
@@ -246,7 +235,16 @@ struct Sampler {
             u64 sum = wave_scan(mine);
             if (lane == 63) s.a[wave] = sum;
             __syncthreads();
-            for (int i = 0; i < wave; ++i) sum += s.a[i];
+            u64 all = 0;
+            for (int i = 0; i < kWaves; ++i) {
+                sum += i < wave ? s.a[i] : 0;
+                all += s.a[i];
+            }
+            if (want == 0) {
+                const double x = ceil(static_cast<double>(share) * static_cast<double>(all));
+                want = x >= 1.0 ? static_cast<u64>(x) : 1;
+                want = want > all ? all : want;
+            }
             sum += before - mine;
             if (sum < want && want <= sum + mine) {
                 int b = tid * kPer;
@@ -285,21 +283,23 @@ struct Sampler {
             lo = __builtin_amdgcn_readfirstlane(lo);
             hi = __builtin_amdgcn_readfirstlane(hi);
             if (lo >= hi) return value_of<DT>(hi);
+            from = value_of<DT>(lo);
+            to = value_of<DT>(hi);
             shift = 0;
             while (((hi - lo) >> shift) >= static_cast<uint32_t>(kBins)) ++shift;
         }
     }
 
     // id and log-probability: v its logit, total the kept weight
-    __device__ void put(int r, int id, float v, u64 total) const {
+    __device__ __forceinline__ void put(int r, int id, float v, u64 total) const {
         p.ids[r] = id;
         if (p.logprobs) {
-            const double t = (static_cast<double>(fminf(v, 3.402823466e38f)) - static_cast<double>(fminf(top, 3.402823466e38f))) * a;
+            const double t = v == top ? 0.0 : (static_cast<double>(v) - static_cast<double>(top)) * a;
             p.logprobs[r] = static_cast<float>(t * 0.6931471805599453 - log(static_cast<double>(total) * 0x1p-44));
         }
     }
     // sums are whole, so a sum exceeds u * total where it exceeds its whole part; a number outside [0, 1) takes an end
-    __device__ u64 target_of(int r, u64 total) const {
+    __device__ __forceinline__ u64 target_of(int r, u64 total) const {
         const double at = fmax(0.0, static_cast<double>(p.u[r])) * static_cast<double>(total);
         if (!(at < static_cast<double>(total))) return total - 1;
         const u64 t = static_cast<u64>(at);
@@ -307,7 +307,8 @@ struct Sampler {
     }
 
     // ---- few candidates: those at or above `bound`; false if there are too many
-    __device__ bool from_list(int r, float bound, int top_k, float top_p, float min_p, bool need_all) {
+    __device__ __forceinline__ bool from_list(int r, float bound, int top_k, float top_p, float min_p, bool need_all) {
+        SampleLds<NT>& s = sample_lds<NT>();
         __syncthreads();
         int n = 0;  // of this wave
         u64 all = 0;
@@ -317,7 +318,10 @@ struct Sampler {
             for (int e = 0; e < kVec; ++e) take |= x[e] >= bound ? 1u << e : 0u;
             if (need_all) {
 #pragma unroll
-                for (int e = 0; e < kVec; ++e) all += weight(x[e]);
+                for (int e = 0; e < kVec; ++e) {
+                    all += weight(x[e]);
+                    if (e % 4 == 3) __builtin_amdgcn_sched_barrier(0);
+                }
             }
             if (__any(take != 0)) {
                 const int c = __builtin_popcount(take);
@@ -391,9 +395,9 @@ struct Sampler {
         return true;
     }
 
-    // ---- the number in the running sum over the vocabulary of what the cut keeps
-    __device__ void from_cut(int r, float cut, u64 ties) {
-        const u64 each = weight(cut);
+    // ---- the number in the running sum over the vocabulary of what the cut keeps; each: the weight at the cut
+    __device__ __forceinline__ void from_cut(int r, float cut, u64 ties, u64 each) {
+        SampleLds<NT>& s = sample_lds<NT>();
         int t0 = 0, t1 = steps();
         u64 target = 0, total = 0, ties_left = ties;
         // the run of steps in which the sum is reached, first of the whole row, then inside that run
@@ -404,8 +408,10 @@ struct Sampler {
             steps_of(w0, w1, 1, [&](const float (&x)[kVec], int) {
 #pragma unroll
                 for (int e = 0; e < kVec; ++e) {
-                    if (x[e] > cut) above += weight(x[e]);
+                    const u64 w = weight(x[e]);
+                    above += x[e] > cut ? w : 0;
                     same += x[e] == cut;
+                    if (e % 4 == 3) __builtin_amdgcn_sched_barrier(0);
                 }
             });
             above = wave_sum(above);
@@ -442,12 +448,17 @@ struct Sampler {
         if (wave != 0) return;
         for (int t = t0; t < t1; ++t) {
             bool done = false;
-            step(t, [&](const float (&x)[kVec], int i0) {
+            float x[kVec];
+            widen(load(t), x);
+            const int i0 = first_of(t);
+            {
                 u64 above = 0, same = 0;
 #pragma unroll
                 for (int e = 0; e < kVec; ++e) {
-                    if (x[e] > cut) above += weight(x[e]);
+                    const u64 w = weight(x[e]);
+                    above += x[e] > cut ? w : 0;
                     same += x[e] == cut;
+                    if (e % 4 == 3) __builtin_amdgcn_sched_barrier(0);
                 }
                 const u64 same_to = wave_scan(same), same_before = same_to - same;
                 const u64 taken = same_before >= ties_left ? 0 : (same < ties_left - same_before ? same : ties_left - same_before);
@@ -474,12 +485,13 @@ struct Sampler {
                     const u64 n = __shfl(same_to, 63);
                     ties_left -= n < ties_left ? n : ties_left;
                 }
-            });
+            }
             if (done) return;
         }
     }
 
-    __device__ void run(int r) {
+    __device__ __forceinline__ void run(int r) {
+        SampleLds<NT>& s = sample_lds<NT>();
         if (tid < 32) s.table[tid] = exp2(tid / 32.0);
         const float temp = p.temperature ? p.temperature[r] : 1.0f;
         const bool greedy = !(temp > 0.0f);
@@ -493,13 +505,16 @@ struct Sampler {
         if (greedy) {
             steps_of(wave, steps(), kWaves, [&](const float (&x)[kVec], int i0) {
 #pragma unroll
-                for (int e = 0; e < kVec; ++e)
-                    if (x[e] > part[0]) { part[0] = x[e]; where = i0 + e; }
+                for (int e = 0; e < kVec; ++e) {
+                    const bool up = x[e] > part[0];
+                    part[0] = up ? x[e] : part[0];
+                    where = up ? i0 + e : where;
+                }
             });
         } else {
             steps_of(wave, steps(), kWaves, [&](const float (&x)[kVec], int) {
 #pragma unroll
-                for (int e = 0; e < kVec; ++e) part[e % kSub] = fmaxf(part[e % kSub], x[e]);
+                for (int e = 0; e < kVec; ++e) part[e % kSub] = x[e] > part[e % kSub] ? x[e] : part[e % kSub];
             });
         }
         top = part[0];
@@ -532,50 +547,76 @@ struct Sampler {
             return;
         }
         a = 1.4426950408889634 / static_cast<double>(temp);
-        const float reachable = static_cast<float>(kOctaves / a);
-        low = top == INFINITY ? INFINITY : fmaxf(top - reachable, -3.402823466e38f);
+        // far enough below the top for no weight even after its rounding, and below the top in any case
+        const uint32_t tb = __float_as_uint(top);
+        const float below = __uint_as_float(tb == 0 || tb == 0x80000000u ? 0x80000001u : (tb & 0x80000000u) ? tb + 1 : tb - 1);
+        low = fminf(top - static_cast<float>(2.0 * kOctaves / a), below);
+        float cut;
+        u64 ties = ~0ull >> 1, each = 0;
+        const bool some_k = top_k > 0 && top_k < p.vocab;
+        if (top == INFINITY) {
+            // +inf logits share all the weight: a share of them by number, from the lowest index
+            u64 n = 0;
+            walk([&](const float (&x)[kVec], int) {
+#pragma unroll
+                for (int e = 0; e < kVec; ++e) n += x[e] == INFINITY;
+            });
+            n = block_sum(n);
+            if (some_k && n > static_cast<u64>(top_k)) n = static_cast<u64>(top_k);
+            if (top_p < 1.0f) n = static_cast<u64>(fmax(1.0, ceil(static_cast<double>(top_p) * static_cast<double>(n))));
+            cut = INFINITY;
+            ties = min_p > 1.0f ? 1 : n;
+            each = 1ull << 44;
+        } else if (!filtered(r, top_k, top_p, min_p, part, cut, ties, each)) {
+            return;  // chosen from a list
+        }
+        from_cut(r, cut, ties, each);
+    }
+
+    // The cut of the three filters; false if the token was chosen from a list of candidates instead.
+    __device__ __forceinline__ bool filtered(int r, int top_k, float top_p, float min_p, const float (&part)[kSub], float& cut, u64& ties, u64& each) {
+        SampleLds<NT>& s = sample_lds<NT>();
+        const bool some_k = top_k > 0 && top_k < p.vocab;
+        u64 before = 0;
         // ---- a bound that all that can be kept lies at or above
         float bound = -INFINITY;
         if (top_k > 0 && top_k <= kTopKList) {
-            // the top_k-th largest partial maximum, to within a few parts in 10^5 of their range: every round tries 64 keys
+            // the top_k-th largest partial maximum, or a little below it
             __syncthreads();
 #pragma unroll
             for (int i = 0; i < kSub; ++i) s.maxima[tid * kSub + i] = key_of<ASRFE_DT_F32>(part[i]);
             __syncthreads();
-            uint32_t mine[16];
+            uint32_t mine[16];  // (the upper halves of the keys will do)
 #pragma unroll
-            for (int i = 0; i < 16; ++i) mine[i] = s.maxima[i * 64 + lane];
-            uint32_t l = key_of<ASRFE_DT_F32>(-3.402823466e38f), h = key_of<ASRFE_DT_F32>(top);  // at least top_k at or above l?
+            for (int i = 0; i < 16; ++i) mine[i] = s.maxima[i * 64 + lane] >> 16;
             auto count = [&](uint32_t k) {
                 int c = 0;
 #pragma unroll
                 for (int i = 0; i < 16; ++i) c += __builtin_popcountll(__ballot(mine[i] >= k));
                 return c;
             };
+            uint32_t l = key_of<ASRFE_DT_F32>(-3.402823466e38f) >> 16, h = key_of<ASRFE_DT_F32>(top) >> 16;
             if (count(l) >= top_k) {
                 while (l < h) {
                     const uint32_t mid = l + (h - l) / 2 + 1;
                     if (count(mid) >= top_k) l = mid;
                     else h = mid - 1;
                 }
-                bound = value_of<ASRFE_DT_F32>(l);
+                bound = fmaxf(value_of<ASRFE_DT_F32>(l << 16), -3.402823466e38f);
             }
         }
         // (top_p measures against all that top_k leaves: the list has to hold that, whatever min_p drops afterwards)
-        const bool some_k = top_k > 0 && top_k < p.vocab;
         if (min_p > 0.0f && !(some_k && top_p < 1.0f)) {
             // l >= max + log2(min_p) / a, and a little below: the candidates' own weights decide
             const double edge = static_cast<double>(top) + log2(fmin(static_cast<double>(min_p), 1.0)) / a;
-            if (top < INFINITY) bound = fmaxf(bound, static_cast<float>(edge - 1e-6 * (fabs(edge) + fabs(static_cast<double>(top))) - 1e-30));
+            bound = fmaxf(bound, static_cast<float>(edge - 1e-6 * (fabs(edge) + fabs(static_cast<double>(top))) - 1e-30));
         }
         if (bound > -INFINITY) {
             bound = fminf(bound, top);
-            if (from_list(r, bound, top_k, top_p, min_p, top_p < 1.0f && !some_k)) return;
+            if (from_list(r, bound, top_k, top_p, min_p, top_p < 1.0f && !some_k)) return false;
         }
         // ---- the general way
-        float cut = low;   // without a filter all that has a weight is kept
-        u64 ties = ~0ull >> 1, before = 0;
-        u64 all = 0;
+        cut = low;  // without a filter all that has a weight is kept
         if (some_k) {
             u64 n = 0;
             walk([&](const float (&x)[kVec], int) {
@@ -584,28 +625,33 @@ struct Sampler {
             });
             n = block_sum(n);
             if (n > static_cast<u64>(top_k)) {
-                cut = reach<false>(static_cast<u64>(top_k), before);
-                ties = static_cast<u64>(top_k) - before;
+                u64 want = static_cast<u64>(top_k);
+                cut = reach<false>(want, 0.0f, before);
+                ties = want - before;
             }
         }
         if (top_p < 1.0f) {
-            u64 n = 0, same = 0;
-            walk([&](const float (&x)[kVec], int) {
+            u64 want = 0;
+            if (some_k) {  // a share of what top_k leaves
+                u64 n = 0, same = 0;
+                walk([&](const float (&x)[kVec], int) {
 #pragma unroll
-                for (int e = 0; e < kVec; ++e) {
-                    if (x[e] > cut) n += weight(x[e]);
-                    same += x[e] == cut;
-                }
-            });
-            all = block_sum(n);
-            same = block_sum(same);
-            all += (same < ties ? same : ties) * weight(cut);
-            const double want = static_cast<double>(top_p) * static_cast<double>(all);
-            u64 want_n = want > 0.0 ? static_cast<u64>(ceil(want)) : 1;
-            want_n = want_n < 1 ? 1 : (want_n > all ? all : want_n);
-            cut = reach<true>(want_n, before);
-            const u64 each = weight(cut);
-            ties = (want_n - before + each - 1) / each;
+                    for (int e = 0; e < kVec; ++e) {
+                        const u64 w = weight(x[e]);
+                        n += x[e] > cut ? w : 0;
+                        same += x[e] == cut;
+                    }
+                });
+                n = block_sum(n);
+                same = block_sum(same);
+                n += (same < ties ? same : ties) * weight(cut);
+                const double x = ceil(static_cast<double>(top_p) * static_cast<double>(n));
+                want = x >= 1.0 ? static_cast<u64>(x) : 1;
+                want = want > n ? n : want;
+            }
+            cut = reach<true>(want, top_p, before);
+            each = weight(cut);
+            ties = (want - before + each - 1) / each;
         }
         if (min_p > 0.0f) {
             // the least value whose weight is at least min_p
@@ -622,13 +668,13 @@ struct Sampler {
                 ties = min_p > 1.0f ? 1 : ~0ull >> 1;
             }
         }
-        from_cut(r, cut, ties);
+        each = weight(cut);
+        return true;
     }
 };
 
 template <int DT, int NT>
 __global__ __launch_bounds__(NT) void sample_kernel(const SampleParams p) {
-    __shared__ SampleLds<NT> s;
     const int r = blockIdx.x;
     if (p.token_num && r % p.rows_per >= p.token_num[r / p.rows_per]) {
         if (threadIdx.x == 0) {
@@ -637,8 +683,7 @@ __global__ __launch_bounds__(NT) void sample_kernel(const SampleParams p) {
         }
         return;
     }
-    Sampler<DT, NT> sampler(p, s, r);
-    sampler.run(r);
+    Sampler<DT, NT>(p, r).run(r);
 }
 
 int32_t launch_sample(asrfe_ctx* ctx, const SampleParams& p, int dtype, hipStream_t s) {
