@@ -224,6 +224,14 @@ def load() -> C.CDLL:
     return _lib
 
 
+def raw_stream(index: int) -> int:
+    """The current stream of a device as the C ABI takes it (without the Stream object that torch.cuda.current_stream builds
+    around it: 0.1 us instead of 2.7 us a call)."""
+    import torch
+
+    return torch._C._cuda_getCurrentRawStream(index)
+
+
 def default_config() -> Config:
     cfg = Config()
     rc = load().asrfe_default_config(C.byref(cfg))

@@ -49,7 +49,7 @@ class PagedKvCache:
             raise ValueError("PagedKvCache: buffers must be 16-byte aligned")
         self.ctx, self.k, self.v, self.k_exp, self.v_exp = ctx, k, v, k_exp, v_exp
         self.n_pages, self.n_heads, self.page_size, self.head_dim = k.shape
-        self.dtype, self.device = k.dtype, k.device
+        self.dtype, self.device, self._index = k.dtype, k.device, k.get_device()
         self._c = _lib.KvCache(k.data_ptr(), v.data_ptr(), k_exp.data_ptr() if e4m3 else None, v_exp.data_ptr() if e4m3 else None,
                                *k.shape[:1], self.page_size, self.n_heads, self.head_dim,
                                _lib.DT_E4M3 if e4m3 else _DT[k.dtype])
@@ -66,56 +66,64 @@ class PagedKvCache:
             return cls(ctx, k, v)
         return cls(ctx, k.view(dtype), v.view(dtype), *(torch.full(shape[:3], 127, dtype=torch.uint8, device=device) for _ in range(2)))
 
-    # ---- checks ----------------------------------------------------------------------------
-    def _plan(self, who, lens, table, cu=None):
-        for name, t, dim in (("kv_lens", lens, 1), ("block_table", table, 2), ("cu_q", cu, 1)):
-            if t is None and name == "cu_q":
-                continue
-            if not isinstance(t, torch.Tensor) or t.dtype != torch.int32 or t.dim() != dim or t.device != self.device \
-                    or not t.is_contiguous():
-                raise ValueError(f"PagedKvCache.{who}: {name} must be a contiguous int32 tensor of {dim} dimension(s) on {self.device}")
-        if table.shape[0] != lens.shape[0] or (cu is not None and cu.shape[0] != lens.shape[0] + 1):
+    # ---- checks (in the order of what is cheap to ask: small calls are bound by the host) -------------------
+    def _plan(self, who, lens, table, cu):
+        i32, index = torch.int32, self._index
+        for t, dim in ((lens, 1), (table, 2), (cu, 1)):
+            if t.dtype is not i32 or t.dim() != dim or t.get_device() != index or not t.is_contiguous():
+                raise ValueError(f"PagedKvCache.{who}: cu_q, kv_lens and block_table must be contiguous int32 tensors [B + 1], [B] and "
+                                 f"[B, n] on {self.device}")
+        if table.shape[0] != lens.shape[0] or (cu is not lens and cu.shape[0] != lens.shape[0] + 1):
             raise ValueError(f"PagedKvCache.{who}: one length and one row of the table per sequence, cu_q one entry more")
 
     def _rows(self, who, name, t, heads):
-        """One [n, heads, head_dim] operand: its rows lie anywhere, their elements side by side."""
-        if not isinstance(t, torch.Tensor) or t.device != self.device or t.dtype not in _DT or t.dim() != 3 \
-                or t.shape[2] != self.head_dim or (heads is not None and t.shape[1] != heads):
+        """One [n, heads, head_dim] operand: its rows lie anywhere, their elements side by side.  -> token and head stride"""
+        dtype, shape = t.dtype, t.shape
+        if dtype not in _DT or len(shape) != 3 or shape[2] != self.head_dim or (heads is not None and shape[1] != heads) \
+                or t.get_device() != self._index:
             raise ValueError(f"PagedKvCache.{who}: {name} must be a float16 or bfloat16 tensor [n, {heads or 'heads'}, {self.head_dim}] "
                              f"on {self.device}")
-        if self.dtype in _DT and t.dtype != self.dtype:
+        if dtype is not self.dtype and self.dtype in _DT:
             raise ValueError(f"PagedKvCache.{who}: {name} must be {self.dtype}, as the cache is")
-        if t.numel() and (t.stride(2) != 1 or t.stride(0) % 8 or t.stride(1) % 8 or t.data_ptr() % 16):
+        ts, hs, es = t.stride()
+        if (es != 1 or ts & 7 or hs & 7 or t.data_ptr() & 15) and t.numel():
             raise ValueError(f"PagedKvCache.{who}: {name} needs rows of contiguous elements, 16-byte aligned (strides in multiples of 8)")
+        return ts, hs
+
+    def _call(self, fn, *args):
+        """fn(context, cache, *args, stream) on the cache's device."""
+        if torch.cuda.current_device() != self._index:
+            with torch.cuda.device(self._index):
+                return self._call(fn, *args)
+        rc = fn(self.ctx.handle, self._ref, *args, _lib.raw_stream(self._index))
+        if rc:
+            self.ctx.check(rc)
 
     # ---- operators ---------------------------------------------------------------------------
     def append(self, k: torch.Tensor, v: torch.Tensor, cu_q: torch.Tensor, kv_lens: torch.Tensor, block_table: torch.Tensor) -> None:
         """Writes the new rows' keys and values k, v [n, n_heads, head_dim] into their pages (quantised as they are written in
         an e4m3 cache).  Slices of a fused projection may be passed as they are."""
         self._plan("append", kv_lens, block_table, cu_q)
-        self._rows("append", "k", k, self.n_heads)
-        self._rows("append", "v", v, self.n_heads)
-        if k.shape != v.shape or k.dtype != v.dtype:
+        kts, khs = self._rows("append", "k", k, self.n_heads)
+        vts, vhs = self._rows("append", "v", v, self.n_heads)
+        n = k.shape[0]
+        if v.shape[0] != n or v.dtype is not k.dtype:
             raise ValueError("PagedKvCache.append: k and v must agree in shape and type")
-        with torch.cuda.device(self.device):
-            self.ctx.check(self.ctx.lib.asrfe_kv_append(
-                self.ctx.handle, self._ref, k.data_ptr(), v.data_ptr(), _DT[k.dtype], k.stride(0), k.stride(1), v.stride(0),
-                v.stride(1), k.shape[0], cu_q.data_ptr(), kv_lens.data_ptr(), block_table.data_ptr(), block_table.shape[1],
-                kv_lens.shape[0], torch.cuda.current_stream().cuda_stream))
+        self._call(self.ctx.lib.asrfe_kv_append, k.data_ptr(), v.data_ptr(), _DT[k.dtype], kts, khs, vts, vhs, n, cu_q.data_ptr(),
+                   kv_lens.data_ptr(), block_table.data_ptr(), block_table.shape[1], kv_lens.shape[0])
 
     def read(self, kv_lens: torch.Tensor, block_table: torch.Tensor, t_max: int, dtype: torch.dtype | None = None):
         """-> k, v [B, t_max, n_heads, head_dim]: positions 0 .. t_max - 1 of every sequence, zero at and past kv_lens[b] and
         where there is no page.  ``dtype``: of the copies (the cache's own for 16-bit caches; float16 unless given for e4m3)."""
-        self._plan("read", kv_lens, block_table)
+        self._plan("read", kv_lens, block_table, kv_lens)
         dtype = dtype or (self.dtype if self.dtype in _DT else torch.float16)
         if dtype not in _DT or (self.dtype in _DT and dtype != self.dtype):
             raise ValueError("PagedKvCache.read: dtype must be the cache's own, float16 or bfloat16 for an e4m3 cache")
-        k, v = (torch.empty((kv_lens.shape[0], t_max, self.n_heads, self.head_dim), dtype=dtype, device=self.device) for _ in range(2))
-        if k.numel():
-            with torch.cuda.device(self.device):
-                self.ctx.check(self.ctx.lib.asrfe_kv_read(
-                    self.ctx.handle, self._ref, kv_lens.data_ptr(), block_table.data_ptr(), block_table.shape[1], kv_lens.shape[0],
-                    t_max, k.data_ptr(), v.data_ptr(), _DT[dtype], torch.cuda.current_stream().cuda_stream))
+        batch = kv_lens.shape[0]
+        k, v = torch.empty((2, batch, t_max, self.n_heads, self.head_dim), dtype=dtype, device=self.device).unbind(0)
+        if batch and t_max:
+            self._call(self.ctx.lib.asrfe_kv_read, kv_lens.data_ptr(), block_table.data_ptr(), block_table.shape[1], batch, t_max,
+                       k.data_ptr(), v.data_ptr(), _DT[dtype])
         return k, v
 
     def attend(self, q: torch.Tensor, cu_q: torch.Tensor, kv_lens: torch.Tensor, block_table: torch.Tensor, window: int = 0,
@@ -128,33 +136,29 @@ class PagedKvCache:
         defaults to 1 / sqrt(head_dim); ``max_kv`` bounds kv_lens (the table's width unless given: a tighter bound shapes
         the launch better)."""
         self._plan("attend", kv_lens, block_table, cu_q)
-        self._rows("attend", "q", q, None)
-        n, heads, _ = q.shape
+        qts, qhs = self._rows("attend", "q", q, None)
+        n, heads, dim = q.shape
         if heads < 1 or heads % self.n_heads:
             raise ValueError(f"PagedKvCache.attend: the heads of q must be a multiple of the cache's {self.n_heads}")
         if window < 0 or sinks < 0:
             raise ValueError("PagedKvCache.attend: window and sinks must not be negative")
         if out is None:
-            out = torch.empty((n, heads, self.head_dim), dtype=q.dtype, device=q.device)
+            out = torch.empty((n, heads, dim), dtype=q.dtype, device=self.device)
+            ots, ohs = heads * dim, dim
         else:
-            self._rows("attend", "out", out, heads)
-            if out.shape != q.shape or out.dtype != q.dtype:
+            ots, ohs = self._rows("attend", "out", out, heads)
+            if out.shape[0] != n or out.dtype is not q.dtype:
                 raise ValueError("PagedKvCache.attend: out must have q's shape and type")
         if not n:
             return out
-        batch = kv_lens.shape[0]
-        max_kv = block_table.shape[1] * self.page_size if max_kv is None else int(max_kv)
-        scale = 1.0 / math.sqrt(self.head_dim) if scale is None else float(scale)
-        lib, h = self.ctx.lib, self.ctx.handle
-        nbytes = int(lib.asrfe_paged_attention_workspace_bytes(h, self._ref, n, heads, batch, max_kv))
+        batch, width = block_table.shape
+        max_kv = width * self.page_size if max_kv is None else int(max_kv)
+        nbytes = self.ctx.lib.asrfe_paged_attention_workspace_bytes(self.ctx.handle, self._ref, n, heads, batch, max_kv)
         if nbytes < 0:
             raise ValueError("PagedKvCache.attend: bad sizes")
-        with torch.cuda.device(self.device):
-            # from the allocator of the current stream, so calls on several streams and captured graphs never share one
-            ws = torch.empty((nbytes,), dtype=torch.uint8, device=q.device) if nbytes else None
-            self.ctx.check(lib.asrfe_paged_attention(
-                h, self._ref, q.data_ptr(), _DT[q.dtype], q.stride(0), q.stride(1), n, heads, cu_q.data_ptr(), kv_lens.data_ptr(),
-                block_table.data_ptr(), block_table.shape[1], batch, max_kv, window, sinks, 1 if causal else 0, scale,
-                out.data_ptr(), out.stride(0), out.stride(1), ws.data_ptr() if nbytes else None, nbytes,
-                torch.cuda.current_stream().cuda_stream))
+        # from the allocator of the current stream, so calls on several streams and captured graphs never share one
+        ws = torch.empty((nbytes,), dtype=torch.uint8, device=self.device) if nbytes else None
+        self._call(self.ctx.lib.asrfe_paged_attention, q.data_ptr(), _DT[q.dtype], qts, qhs, n, heads, cu_q.data_ptr(), kv_lens.data_ptr(),
+                   block_table.data_ptr(), width, batch, max_kv, window, sinks, 1 if causal else 0,
+                   1.0 / math.sqrt(dim) if scale is None else scale, out.data_ptr(), ots, ohs, ws.data_ptr() if nbytes else None, nbytes)
         return out

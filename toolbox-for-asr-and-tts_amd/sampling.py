@@ -14,15 +14,19 @@ _DT = {torch.float32: _lib.DT_F32, torch.float16: _lib.DT_F16, torch.bfloat16: _
 MAX_VOCAB = 1 << 18
 
 
-def _per_row(name, value, rows, dtype, device):
+def _per_row(name, value, rows, dtype, index, device):
     """A setting for every row: a tensor [rows], one number for all, or None."""
     if value is None:
         return None
     if not isinstance(value, torch.Tensor):
         return torch.full((rows,), value, dtype=dtype, device=device)
-    if value.dtype != dtype or value.shape != (rows,) or value.device != device or not value.is_contiguous():
+    if value.dtype is not dtype or value.dim() != 1 or value.shape[0] != rows or value.get_device() != index or not value.is_contiguous():
         raise ValueError(f"sample_tokens: {name} must be one number or a contiguous {dtype} tensor [{rows}] on {device}")
     return value
+
+
+def _ptr(t):
+    return None if t is None else t.data_ptr()
 
 
 def sample_tokens(ctx: _lib.Context, logits: torch.Tensor, u: torch.Tensor, temperature=None, top_k=None, top_p=None, min_p=None,
@@ -34,35 +38,40 @@ def sample_tokens(ctx: _lib.Context, logits: torch.Tensor, u: torch.Tensor, temp
     are kept (<= 0: all), of those the shortest prefix with at least ``top_p`` of their weight, of those the ones with at
     least ``min_p`` of the largest weight, and always the first; the id is the lowest one at which the running sum of the
     kept weights exceeds ``u`` times their sum.  A temperature that is not above zero takes the arg-max.  Every setting is one
-    number, a tensor [rows] or None.  NaN logits count as -inf; a row with nothing above -inf gives id 0 and logprob -inf.
+    number (u, too), a tensor [rows] or None.  NaN logits count as -inf; a row with nothing above -inf gives id 0 and logprob -inf.
     ``token_num`` [rows / n] int32: of every n rows the ones behind an utterance's tokens get id -1 and logprob 0."""
     if not logits.is_cuda or logits.dtype not in _DT or logits.dim() != 2 or not 1 <= logits.shape[1] <= MAX_VOCAB:
         raise ValueError(f"sample_tokens: logits must be a float32, float16 or bfloat16 CUDA tensor [rows, 1 .. {MAX_VOCAB}]")
     rows, vocab = logits.shape
-    dev = logits.device
-    if rows and vocab > 1 and logits.stride(1) != 1 or rows > 1 and logits.stride(0) < vocab:
+    stride, step = logits.stride()
+    index, dev = logits.get_device(), logits.device
+    if rows and vocab > 1 and step != 1 or rows > 1 and stride < vocab:
         raise ValueError("sample_tokens: every row's logits must lie side by side, rows must not overlap")
-    if not isinstance(u, torch.Tensor) or u.dtype != torch.float32 or u.shape != (rows,) or u.device != dev or not u.is_contiguous():
-        raise ValueError(f"sample_tokens: u must be a contiguous float32 tensor [{rows}] on {dev}")
-    temperature, top_p, min_p = (_per_row(n, x, rows, torch.float32, dev)
-                                 for n, x in (("temperature", temperature), ("top_p", top_p), ("min_p", min_p)))
-    top_k = _per_row("top_k", top_k, rows, torch.int32, dev)
+    u = _per_row("u", u, rows, torch.float32, index, dev)
+    temperature = _per_row("temperature", temperature, rows, torch.float32, index, dev)
+    top_k = _per_row("top_k", top_k, rows, torch.int32, index, dev)
+    top_p = _per_row("top_p", top_p, rows, torch.float32, index, dev)
+    min_p = _per_row("min_p", min_p, rows, torch.float32, index, dev)
+    if u is None:
+        raise ValueError("sample_tokens: u is needed")
     rows_per = 0
     if token_num is not None:
-        if token_num.dtype != torch.int32 or token_num.dim() != 1 or token_num.device != dev or not token_num.is_contiguous() \
+        if token_num.dtype != torch.int32 or token_num.dim() != 1 or token_num.get_device() != index or not token_num.is_contiguous() \
                 or not token_num.shape[0] or rows % token_num.shape[0] or not rows:
             raise ValueError("sample_tokens: token_num must be a contiguous int32 tensor whose length divides the rows")
         rows_per = rows // token_num.shape[0]
     if ids is None:
         ids = torch.empty((rows,), dtype=torch.int32, device=dev)
-    elif ids.dtype != torch.int32 or ids.shape != (rows,) or ids.device != dev or not ids.is_contiguous():
+    elif ids.dtype != torch.int32 or ids.shape != (rows,) or ids.get_device() != index or not ids.is_contiguous():
         raise ValueError(f"sample_tokens: ids must be a contiguous int32 tensor [{rows}] on {dev}")
     logprobs = torch.empty((rows,), dtype=torch.float32, device=dev)
     if rows:
-        ptr = lambda t: t.data_ptr() if t is not None else None  # noqa: E731
-        with torch.cuda.device(dev):
-            ctx.check(ctx.lib.asrfe_sample_tokens(
-                ctx.handle, logits.data_ptr(), _DT[logits.dtype], logits.stride(0) if rows > 1 else vocab, rows, vocab, u.data_ptr(),
-                ptr(temperature), ptr(top_k), ptr(top_p), ptr(min_p), ptr(token_num), rows_per, ids.data_ptr(), logprobs.data_ptr(),
-                torch.cuda.current_stream().cuda_stream))
+        if torch.cuda.current_device() != index:
+            with torch.cuda.device(index):
+                return sample_tokens(ctx, logits, u, temperature, top_k, top_p, min_p, token_num, ids)
+        rc = ctx.lib.asrfe_sample_tokens(
+            ctx.handle, logits.data_ptr(), _DT[logits.dtype], stride if rows > 1 else vocab, rows, vocab, u.data_ptr(), _ptr(temperature),
+            _ptr(top_k), _ptr(top_p), _ptr(min_p), _ptr(token_num), rows_per, ids.data_ptr(), logprobs.data_ptr(), _lib.raw_stream(index))
+        if rc:
+            ctx.check(rc)
     return ids, logprobs
