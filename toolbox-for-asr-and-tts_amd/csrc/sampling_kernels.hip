@@ -1,17 +1,17 @@
 // Choice of a token per row of logits: temperature, top-k, top-p, min-p and one random number.
 //
 //   One workgroup per row (256 threads for small vocabularies, else 1024).  Weights w = 2^((l - max) log2(e) / T) are formed
-//   in double precision (a table of 2^(j / 32) and a polynomial: relative error below 1e-11; double FMAs issue at the rate
-//   of single ones here) and summed as whole multiples of 2^-44, so a sum is the same in any order and atomics may form
+//   in double precision (a table of 2^(j / 1024) and a polynomial: relative error below 1e-11; double FMAs issue at the
+//   rate of single ones here) and summed as whole multiples of 2^-44, so a sum is the same in any order and atomics may form
 //   it.  What is kept is a prefix of the order (falling logit, rising index), described by the value of its last element,
 //   `cut`, and the number of elements of that value that belong to it, `ties`.
 //
 //   The row is read from memory once for its maximum and, from the caches, once or a few times more:
-//     * few candidates (a small top_k, or min_p): the k-th largest of 1024 partial maxima is a lower bound of the k-th
+//     * few candidates (a small top_k, or min_p): the k-th largest of 4096 (2048) partial maxima is a lower bound of the k-th
 //       largest logit; what is at or above it goes into a list in the LDS, in the order of the vocabulary, and every
 //       filter is settled there by counting (256 entries at most; more take the way below);
 //     * else a cut is found by histograms in the LDS, first over (max - l) / T, then over the keys of the values left in
-//       the bin where the cut lies, 2048 bins at a time, until one value is left;
+//       the bin where the cut lies, until one value is left;
 //     * the number is then looked up in the running sum over the vocabulary: per wave, per step of that wave, per lane.
 #include "elem.h"
 #include "paged_device.h"
@@ -20,7 +20,6 @@ namespace asrfe {
 
 typedef unsigned long long u64;
 
-constexpr int kBins = 2048;
 constexpr int kList = 256;        // candidates the list path takes
 constexpr int kTopKList = 200;    // largest top_k that tries it: the list holds ties and near misses too
 constexpr double kOctaves = 46.0; // weights below 2^-45 are zero in multiples of 2^-44
@@ -61,20 +60,27 @@ __device__ __forceinline__ u64 wave_scan(u64 v) {  // sum up to and with this la
 template <int NT>
 struct SampleLds {
     static constexpr int kWaves = NT / 64;
-    double table[32];
+    // (256 rows of 131072 in 32 bits under top_p: 156 to 160 us with 4096 bins, 154 with 16384, which short rows take 1 us to clear)
+    static constexpr int kBins = NT == 1024 ? 4096 : 2048, kPer = kBins / NT;
+    // place of a bin: a thread sums kPer neighbours, one place of padding behind them keeps threads on banks of their own
+    __device__ __forceinline__ static int slot(int bin) { return bin + bin / kPer; }
+    double table[1024];  // 2^(j / 1024)
     u64 a[kWaves], b[kWaves];
     union {
-        u64 hist[kBins];
-        uint32_t maxima[1024];
+        u64 hist[kBins + kBins / kPer];
         struct {
             float value[kWaves][kList];
             int index[kWaves][kList];
         } found;
     };
     struct {
+        struct {
+            u64 order;   // key, then the place in the list from behind: unique, larger ones come first
+            u64 weight;
+        } entry[kList];
         float value[kList];
-        int index[kList];
-        u64 weight[kList];
+        int index[kList], rank[kList];
+        u64 before[kList];
     } list;
     u64 res[4];
     int n[kWaves];
@@ -92,18 +98,21 @@ __device__ __forceinline__ SampleLds<NT>& sample_lds() {
 template <int DT, int NT>
 struct Sampler {
     static constexpr int kWaves = NT / 64;
+    static constexpr int kBins = SampleLds<NT>::kBins, kPer = SampleLds<NT>::kPer;
+    __device__ __forceinline__ static int slot(int bin) { return SampleLds<NT>::slot(bin); }
     static constexpr int kVec = DT == ASRFE_DT_F32 ? 4 : 8;
-    static constexpr int kSub = 1024 / NT;  // partial maxima of a thread
+    static constexpr int kSub = NT == 1024 ? 4 : 8;  // partial maxima of a thread
 
     const SampleParams& p;
     const int tid, lane, wave;
     const char* row;
     int head, n_vec, n_steps;  // elements before the first 16-byte boundary, 16-byte pieces, steps of 64 of them
+    bool flat;                 // all that counts has the same logit, one without a scale (+inf, or the least there is)
     float top, low;            // largest logit, least logit with a weight
-    double a;                  // log2(e) / T
+    double a, a_units;         // log2(e) / T, and 1024 times as much, for weight()
 
     __device__ __forceinline__ Sampler(const SampleParams& p_, int r)
-        : p(p_), tid(threadIdx.x), lane(threadIdx.x & 63), wave(__builtin_amdgcn_readfirstlane(threadIdx.x >> 6)) {
+        : p(p_), tid(threadIdx.x), lane(threadIdx.x & 63), wave(__builtin_amdgcn_readfirstlane(threadIdx.x >> 6)), flat(false) {
         constexpr int kSize = DT == ASRFE_DT_F32 ? 4 : 2;
         row = static_cast<const char*>(p.logits) + static_cast<int64_t>(r) * p.ld * kSize;
         head = static_cast<int>((16 - (reinterpret_cast<uintptr_t>(row) & 15)) & 15) / kSize;
@@ -137,17 +146,23 @@ struct Sampler {
         }
     }
     __device__ __forceinline__ int steps() const { return n_steps + 2; }
-    // f(x, i0) for steps t0, t0 + by, ... below t1: this lane's elements i0, i0 + 1, ...  Three loads are in flight.
+    // f(x, i0, t) for the n steps t0, t0 + by, ..., from the one of number `from` around to the one before it: this lane's
+    // elements i0, i0 + 1, ...  Three loads are in flight.
     template <class F>
-    __device__ __forceinline__ void steps_of(int t0, int t1, int by, F&& f) const {
-        u32x4 w0 = load(t0), w1 = load(t0 + by), w2;
-        for (int t = t0; t < t1; t += by) {
-            w2 = load(t + 2 * by);
+    __device__ __forceinline__ void steps_of(int t0, int n, int by, int from, F&& f) const {
+        if (n <= 0) return;
+        int i0 = from, i1 = from + 1 < n ? from + 1 : 0;
+        u32x4 w0 = load(t0 + i0 * by), w1 = load(t0 + i1 * by), w2;
+        for (int k = 0; k < n; ++k) {
+            const int i2 = i1 + 1 < n ? i1 + 1 : 0;
+            w2 = load(t0 + i2 * by);
             float x[kVec];
             widen(w0, x);
-            f(x, first_of(t));
+            f(x, first_of(t0 + i0 * by), t0 + i0 * by);
             w0 = w1;
             w1 = w2;
+            i0 = i1;
+            i1 = i2;
         }
     }
     // this wave's run of steps: runs follow each other in the order of the vocabulary
@@ -156,23 +171,31 @@ struct Sampler {
         return t < steps() ? t : steps();
     }
     template <class F>
-    __device__ __forceinline__ void walk(F&& f) const { steps_of(run_of(wave), run_of(wave + 1), 1, f); }
+    __device__ __forceinline__ void walk(F&& f) const {
+        // (every wave begins elsewhere in its run: all at the same distance from their runs' starts ask the same few memory
+        // channels at once: 256 rows of 131072 under top_p 115 us, this way 105 us)
+        const int t0 = run_of(wave), n = run_of(wave + 1) - t0;
+        steps_of(t0, n, 1, n > 0 ? wave % n : 0, f);
+    }
 
-    // Weight in multiples of 2^-44.  Below `low`, and for NaN, it comes out as zero: the median of three takes the least.
-    __device__ __forceinline__ u64 weight(float v) const {
-        const double t = fmax((static_cast<double>(__builtin_amdgcn_fmed3f(v, low, top)) - static_cast<double>(top)) * (a * 32.0), -6400.0);
+    // Weight in multiples of 2^-44, with kOffset added (a sum over n values takes it off n times; whole numbers may wrap).
+    // Below `low`, and for NaN, the median of three takes `low`, whose weight is zero.
+    static constexpr u64 kOffset = 0x4330000000000000ull;  // bits of 2^52, whose unit is one
+    __device__ __forceinline__ u64 weight_bits(float v) const {
+        const double t = (static_cast<double>(__builtin_amdgcn_fmed3f(v, low, top)) - static_cast<double>(top)) * a_units;
         constexpr double kMagic = 6755399441055744.0;  // 1.5 * 2^52: the sum's low bits are the nearest whole number
         const double d = t + kMagic;
         const int k = static_cast<int>(__builtin_bit_cast(u64, d));
-        const double f = t - (d - kMagic);  // |f| <= 1 / 2, in units of 1 / 32
-        // 2^(f / 32) = sum (f ln 2 / 32)^n / n!, up to n = 4: the next term is below 2e-12
-        double y = fma(f, 9.172562701156919e-09, 1.6938509724835576e-06);
-        y = fma(f, y, 0.00023459619820224656);
-        y = fma(f, y, 0.021660849392498292);
-        y = fma(f, y, 1.0) * sample_lds<NT>().table[k & 31];
-        const double scale = __builtin_bit_cast(double, static_cast<u64>(1023 + 44 + (k >> 5)) << 52);
-        return __builtin_bit_cast(u64, fma(y, scale, 0x1p52)) & 0xfffffffffffffull;
+        const double f = t - (d - kMagic);  // |f| <= 1 / 2, in units of 1 / 1024
+        // 2^(f / 1024) = 1 + f ln 2 / 1024 + (f ln 2 / 1024)^2 / 2: the next term is below 7e-12.  (A table of 32 entries, which
+        // meets no bank conflicts, and two terms more: 5 % slower.)
+        const double e = f * fma(f, 2.2909787910375658e-07, 0.0006769015435155716);
+        const double tab = sample_lds<NT>().table[k & 1023];
+        // (its exponent moved by k / 1024 and 44)
+        const double w = __builtin_bit_cast(double, __builtin_bit_cast(u64, tab) + (static_cast<u64>(static_cast<uint32_t>((k >> 10) + 44)) << 52));
+        return __builtin_bit_cast(u64, fma(w, e, w + 0x1p52));
     }
+    __device__ __forceinline__ u64 weight(float v) const { return weight_bits(v) - kOffset; }
 
     __device__ __forceinline__ u64 block_sum(u64 v) {
         SampleLds<NT>& s = sample_lds<NT>();
@@ -184,6 +207,28 @@ struct Sampler {
 #pragma unroll
         for (int i = 0; i < kWaves; ++i) t += s.a[i];
         return t;
+    }
+
+    // The bin of the histogram at which a sum that starts at `before` reaches `want`, in s.res[1] (left as it is where none does),
+    // and the sum before it in `before`.  Every thread takes a run of bins.
+    __device__ __forceinline__ void find_bin(u64 want, u64& before) {
+        SampleLds<NT>& s = sample_lds<NT>();
+        u64 mine = 0;
+#pragma unroll
+        for (int i = 0; i < kPer; ++i) mine += s.hist[slot(tid * kPer) + i];
+        u64 sum = wave_scan(mine);
+        if (lane == 63) s.b[wave] = sum;
+        __syncthreads();
+        for (int i = 0; i < wave; ++i) sum += s.b[i];
+        sum += before - mine;
+        if (sum < want && want <= sum + mine) {
+            int b = tid * kPer;
+            while (sum + s.hist[slot(b)] < want) sum += s.hist[slot(b++)];
+            s.res[0] = sum;
+            s.res[1] = b;
+        }
+        __syncthreads();
+        before = s.res[0];
     }
 
     // Finds the value at which a running sum over falling values first reaches `want` (1 <= want <= the sum of all):
@@ -205,10 +250,10 @@ struct Sampler {
         int shift = -1;
         for (;;) {
             __syncthreads();
-            for (int i = tid; i < kBins; i += NT) s.hist[i] = 0;
+            for (int i = tid; i < kBins + kBins / kPer; i += NT) s.hist[i] = 0;
             __syncthreads();
             if (shift < 0) {
-                walk([&](const float (&x)[kVec], int) {
+                walk([&](const float (&x)[kVec], int, int) {
                     u64 w[kVec];
 #pragma unroll
                     for (int e = 0; e < kVec; ++e) {
@@ -217,43 +262,26 @@ struct Sampler {
                     }
 #pragma unroll
                     for (int e = 0; e < kVec; ++e)
-                        if (w[e] != 0) atomicAdd(&s.hist[bin1(x[e])], w[e]);
+                        if (w[e] != 0) atomicAdd(&s.hist[slot(bin1(x[e]))], w[e]);
                 });
             } else {
-                walk([&](const float (&x)[kVec], int) {
+                walk([&](const float (&x)[kVec], int, int) {
 #pragma unroll
                     for (int e = 0; e < kVec; ++e)
-                        if (x[e] >= from && x[e] <= to) atomicAdd(&s.hist[(hi - key_of<DT>(x[e])) >> shift], MASS ? weight(x[e]) : u64{1});
+                        if (x[e] >= from && x[e] <= to) atomicAdd(&s.hist[slot((hi - key_of<DT>(x[e])) >> shift)], MASS ? weight(x[e]) : u64{1});
                 });
             }
             __syncthreads();
-            // the bin where `want` is reached: every thread a run of bins
-            constexpr int kPer = kBins / NT;
-            u64 mine = 0;
-#pragma unroll
-            for (int i = 0; i < kPer; ++i) mine += s.hist[tid * kPer + i];
-            u64 sum = wave_scan(mine);
-            if (lane == 63) s.a[wave] = sum;
-            __syncthreads();
-            u64 all = 0;
-            for (int i = 0; i < kWaves; ++i) {
-                sum += i < wave ? s.a[i] : 0;
-                all += s.a[i];
-            }
             if (want == 0) {
+                u64 mine = 0;
+#pragma unroll
+                for (int i = 0; i < kPer; ++i) mine += s.hist[slot(tid * kPer) + i];
+                const u64 all = block_sum(mine);
                 const double x = ceil(static_cast<double>(share) * static_cast<double>(all));
                 want = x >= 1.0 ? static_cast<u64>(x) : 1;
                 want = want > all ? all : want;
             }
-            sum += before - mine;
-            if (sum < want && want <= sum + mine) {
-                int b = tid * kPer;
-                while (sum + s.hist[b] < want) sum += s.hist[b++];
-                s.res[0] = sum;
-                s.res[1] = b;
-            }
-            __syncthreads();
-            before = s.res[0];
+            find_bin(want, before);
             const int b = static_cast<int>(s.res[1]);
             if (shift < 0) {
                 // keys of the bin's values: the ends are found by trying 64 keys at a time (bins fall as keys rise)
@@ -294,7 +322,7 @@ struct Sampler {
     __device__ __forceinline__ void put(int r, int id, float v, u64 total) const {
         p.ids[r] = id;
         if (p.logprobs) {
-            const double t = v == top ? 0.0 : (static_cast<double>(v) - static_cast<double>(top)) * a;
+            const double t = flat ? 0.0 : (static_cast<double>(v) - static_cast<double>(top)) * a;
             p.logprobs[r] = static_cast<float>(t * 0.6931471805599453 - log(static_cast<double>(total) * 0x1p-44));
         }
     }
@@ -310,9 +338,11 @@ struct Sampler {
     __device__ __forceinline__ bool from_list(int r, float bound, int top_k, float top_p, float min_p, bool need_all) {
         SampleLds<NT>& s = sample_lds<NT>();
         __syncthreads();
-        int n = 0;  // of this wave
+        int n = 0, early = 0;  // of this wave; those found before its run began anew at its first step
         u64 all = 0;
-        walk([&](const float (&x)[kVec], int i0) {
+        const int first_step = run_of(wave);
+        walk([&](const float (&x)[kVec], int i0, int t) {
+            if (t == first_step) early = n;
             uint32_t take = 0;
 #pragma unroll
             for (int e = 0; e < kVec; ++e) take |= x[e] >= bound ? 1u << e : 0u;
@@ -353,27 +383,42 @@ struct Sampler {
             total_n += s.n[i];
         }
         if (total_n > kList) return false;
-        for (int i = lane; i < n; i += 64) {
+        for (int i = lane; i < n; i += 64) {  // (what was found early lies behind the rest in the order of the vocabulary)
             const float v = s.found.value[wave][i];
-            s.list.value[start + i] = v;
-            s.list.index[start + i] = s.found.index[wave][i];
-            s.list.weight[start + i] = weight(v);
+            const int at = start + (i < early ? i + n - early : i - early);
+            s.list.value[at] = v;
+            s.list.index[at] = s.found.index[wave][i];
+            s.list.entry[at].order = static_cast<u64>(key_of<ASRFE_DT_F32>(v)) << 32 | static_cast<uint32_t>(kList - at);
+            s.list.entry[at].weight = weight(v);
+            s.list.rank[at] = 0;
+            s.list.before[at] = 0;
         }
         __syncthreads();
         // every candidate counts what comes before it in the order
         const bool on = tid < total_n;
         const float v = on ? s.list.value[tid] : 0.0f;
-        const u64 w = on ? s.list.weight[tid] : 0;
-        int rank = 0;
-        u64 before = 0;
-        if (wave * 64 < total_n) {
-            for (int j = 0; j < total_n; ++j) {
-                const float vj = s.list.value[j];
-                const bool ahead = vj > v || (vj == v && j < tid);
+        const u64 w = on ? s.list.entry[tid].weight : 0;
+        // (64 candidates a wave, and the list cut among the waves that have the same ones)
+        const int blocks = total_n <= 64 ? 1 : total_n <= 128 ? 2 : 4, cuts = kWaves / blocks, per = (total_n + cuts - 1) / cuts;
+        {
+            const int i = wave % blocks * 64 + lane, j0 = wave / blocks * per, j1 = min(total_n, j0 + per);
+            const u64 order = s.list.entry[i].order;  // (behind the end: what is there, for nobody)
+            int rank = 0;
+            u64 before = 0;
+#pragma unroll 8
+            for (int j = j0; j < j1; ++j) {
+                const bool ahead = s.list.entry[j].order > order;
                 rank += ahead;
-                before += ahead ? s.list.weight[j] : 0;
+                before += ahead ? s.list.entry[j].weight : 0;
+            }
+            if (i < total_n && rank) {
+                atomicAdd(&s.list.rank[i], rank);
+                atomicAdd(&s.list.before[i], before);
             }
         }
+        __syncthreads();
+        const int rank = on ? s.list.rank[tid] : 0;
+        const u64 before = on ? s.list.before[tid] : 0;
         const bool in_k = on && (top_k <= 0 || rank < top_k);
         if (!need_all) all = block_sum(in_k ? w : 0);
         bool keep = in_k;
@@ -405,16 +450,15 @@ struct Sampler {
             const int per = (t1 - t0 + kWaves - 1) / kWaves;
             const int w0 = t0 + wave * per < t1 ? t0 + wave * per : t1, w1 = w0 + per < t1 ? w0 + per : t1;
             u64 above = 0, same = 0;
-            steps_of(w0, w1, 1, [&](const float (&x)[kVec], int) {
+            steps_of(w0, w1 - w0, 1, w1 > w0 ? wave % (w1 - w0) : 0, [&](const float (&x)[kVec], int, int) {
 #pragma unroll
                 for (int e = 0; e < kVec; ++e) {
-                    const u64 w = weight(x[e]);
-                    above += x[e] > cut ? w : 0;
+                    above += weight_bits(x[e] > cut ? x[e] : low);
                     same += x[e] == cut;
                     if (e % 4 == 3) __builtin_amdgcn_sched_barrier(0);
                 }
             });
-            above = wave_sum(above);
+            above = wave_sum(above - kOffset * static_cast<u64>((w1 - w0) * kVec));
             same = wave_sum(same);
             __syncthreads();
             if (lane == 0) {
@@ -455,11 +499,11 @@ struct Sampler {
                 u64 above = 0, same = 0;
 #pragma unroll
                 for (int e = 0; e < kVec; ++e) {
-                    const u64 w = weight(x[e]);
-                    above += x[e] > cut ? w : 0;
+                    above += weight_bits(x[e] > cut ? x[e] : low);
                     same += x[e] == cut;
                     if (e % 4 == 3) __builtin_amdgcn_sched_barrier(0);
                 }
+                above -= kOffset * kVec;
                 const u64 same_to = wave_scan(same), same_before = same_to - same;
                 const u64 taken = same_before >= ties_left ? 0 : (same < ties_left - same_before ? same : ties_left - same_before);
                 const u64 mine = above + taken * each, upto = wave_scan(mine);
@@ -492,8 +536,8 @@ struct Sampler {
 
     __device__ __forceinline__ void run(int r) {
         SampleLds<NT>& s = sample_lds<NT>();
-        if (tid < 32) s.table[tid] = exp2(tid / 32.0);
-        const float temp = p.temperature ? p.temperature[r] : 1.0f;
+        for (int i = tid; i < 1024; i += NT) s.table[i] = exp2(i / 1024.0);
+        const float temp = fminf(p.temperature ? p.temperature[r] : 1.0f, 1e30f);  // (beyond it all weights are one as well)
         const bool greedy = !(temp > 0.0f);
         const int top_k = p.top_k ? p.top_k[r] : 0;
         const float top_p = p.top_p ? p.top_p[r] : 1.0f, min_p = p.min_p ? p.min_p[r] : 0.0f;
@@ -503,7 +547,7 @@ struct Sampler {
         for (int i = 0; i < kSub; ++i) part[i] = -INFINITY;
         int where = 0x7fffffff;
         if (greedy) {
-            steps_of(wave, steps(), kWaves, [&](const float (&x)[kVec], int i0) {
+            steps_of(wave, (steps() - wave + kWaves - 1) / kWaves, kWaves, 0, [&](const float (&x)[kVec], int i0, int) {
 #pragma unroll
                 for (int e = 0; e < kVec; ++e) {
                     const bool up = x[e] > part[0];
@@ -512,9 +556,17 @@ struct Sampler {
                 }
             });
         } else {
-            steps_of(wave, steps(), kWaves, [&](const float (&x)[kVec], int) {
+            steps_of(wave, (steps() - wave + kWaves - 1) / kWaves, kWaves, 0, [&](const float (&x)[kVec], int, int) {
 #pragma unroll
                 for (int e = 0; e < kVec; ++e) part[e % kSub] = x[e] > part[e % kSub] ? x[e] : part[e % kSub];
+                if constexpr (kVec < kSub) {  // the other half's turn
+#pragma unroll
+                    for (int e = 0; e < kVec; ++e) {
+                        const float y = part[e];
+                        part[e] = part[e + kVec];
+                        part[e + kVec] = y;
+                    }
+                }
             });
         }
         top = part[0];
@@ -551,22 +603,28 @@ struct Sampler {
         const uint32_t tb = __float_as_uint(top);
         const float below = __uint_as_float(tb == 0 || tb == 0x80000000u ? 0x80000001u : (tb & 0x80000000u) ? tb + 1 : tb - 1);
         low = fminf(top - static_cast<float>(2.0 * kOctaves / a), below);
+        // (where logits are so large that nothing lies between `low` and the top, a power the exponent can hold will do)
+        a_units = 1024.0 * fmin(a, 4.0 * kOctaves / (static_cast<double>(top) - static_cast<double>(low)));
         float cut;
         u64 ties = ~0ull >> 1, each = 0;
         const bool some_k = top_k > 0 && top_k < p.vocab;
-        if (top == INFINITY) {
-            // +inf logits share all the weight: a share of them by number, from the lowest index
+        if (low < -3.402823466e38f || top == INFINITY) {
+            // a share by number, from the lowest index
             u64 n = 0;
-            walk([&](const float (&x)[kVec], int) {
+            walk([&](const float (&x)[kVec], int, int) {
 #pragma unroll
-                for (int e = 0; e < kVec; ++e) n += x[e] == INFINITY;
+                for (int e = 0; e < kVec; ++e) n += x[e] == top;
             });
             n = block_sum(n);
             if (some_k && n > static_cast<u64>(top_k)) n = static_cast<u64>(top_k);
             if (top_p < 1.0f) n = static_cast<u64>(fmax(1.0, ceil(static_cast<double>(top_p) * static_cast<double>(n))));
-            cut = INFINITY;
+            cut = top;
             ties = min_p > 1.0f ? 1 : n;
             each = 1ull << 44;
+            flat = true;
+            top = 0.0f;  // (for the weights of what is not chosen: none)
+            low = -1.0f;
+            a_units = 1024.0 * 2.0 * kOctaves;
         } else if (!filtered(r, top_k, top_p, min_p, part, cut, ties, each)) {
             return;  // chosen from a list
         }
@@ -581,29 +639,22 @@ struct Sampler {
         // ---- a bound that all that can be kept lies at or above
         float bound = -INFINITY;
         if (top_k > 0 && top_k <= kTopKList) {
-            // the top_k-th largest partial maximum, or a little below it
+            // The top_k-th largest partial maximum, or a little below it: by number, over the upper halves of the keys, from the
+            // top down.  (Where it lies more than kBins of them down there is no bound, and the general way is taken.)
+            const uint32_t high = key_of<ASRFE_DT_F32>(top) >> 16;
+            for (int i = tid; i < kBins + kBins / kPer; i += NT) s.hist[i] = 0;
             __syncthreads();
 #pragma unroll
-            for (int i = 0; i < kSub; ++i) s.maxima[tid * kSub + i] = key_of<ASRFE_DT_F32>(part[i]);
-            __syncthreads();
-            uint32_t mine[16];  // (the upper halves of the keys will do)
-#pragma unroll
-            for (int i = 0; i < 16; ++i) mine[i] = s.maxima[i * 64 + lane] >> 16;
-            auto count = [&](uint32_t k) {
-                int c = 0;
-#pragma unroll
-                for (int i = 0; i < 16; ++i) c += __builtin_popcountll(__ballot(mine[i] >= k));
-                return c;
-            };
-            uint32_t l = key_of<ASRFE_DT_F32>(-3.402823466e38f) >> 16, h = key_of<ASRFE_DT_F32>(top) >> 16;
-            if (count(l) >= top_k) {
-                while (l < h) {
-                    const uint32_t mid = l + (h - l) / 2 + 1;
-                    if (count(mid) >= top_k) l = mid;
-                    else h = mid - 1;
-                }
-                bound = fmaxf(value_of<ASRFE_DT_F32>(l << 16), -3.402823466e38f);
+            for (int i = 0; i < kSub; ++i) {
+                const uint32_t down = high - (key_of<ASRFE_DT_F32>(part[i]) >> 16);
+                if (down < static_cast<uint32_t>(kBins) && part[i] >= -3.402823466e38f) atomicAdd(&s.hist[slot(down)], u64{1});
             }
+            if (tid == 0) s.res[1] = kBins;
+            __syncthreads();
+            u64 sum = 0;
+            find_bin(static_cast<u64>(top_k), sum);
+            const uint32_t down = static_cast<uint32_t>(s.res[1]);
+            if (down < static_cast<uint32_t>(kBins)) bound = fmaxf(value_of<ASRFE_DT_F32>((high - down) << 16), -3.402823466e38f);
         }
         // (top_p measures against all that top_k leaves: the list has to hold that, whatever min_p drops afterwards)
         if (min_p > 0.0f && !(some_k && top_p < 1.0f)) {
@@ -619,7 +670,7 @@ struct Sampler {
         cut = low;  // without a filter all that has a weight is kept
         if (some_k) {
             u64 n = 0;
-            walk([&](const float (&x)[kVec], int) {
+            walk([&](const float (&x)[kVec], int, int) {
 #pragma unroll
                 for (int e = 0; e < kVec; ++e) n += x[e] >= -3.402823466e38f;
             });
@@ -634,7 +685,7 @@ struct Sampler {
             u64 want = 0;
             if (some_k) {  // a share of what top_k leaves
                 u64 n = 0, same = 0;
-                walk([&](const float (&x)[kVec], int) {
+                walk([&](const float (&x)[kVec], int, int) {
 #pragma unroll
                     for (int e = 0; e < kVec; ++e) {
                         const u64 w = weight(x[e]);
@@ -688,8 +739,8 @@ __global__ __launch_bounds__(NT) void sample_kernel(const SampleParams p) {
 
 int32_t launch_sample(asrfe_ctx* ctx, const SampleParams& p, int dtype, hipStream_t s) {
     const dim3 grid(p.rows);
-    // small vocabularies: eight rows of a compute unit at once instead of two
-    const bool small = p.vocab <= 16384;
+    // small vocabularies: several rows of a compute unit at once, where there are more rows than compute units
+    const bool small = p.vocab <= 16384 && p.rows > ctx->num_cus;
 #define SAMPLE(DT)                                                                                 \
     do {                                                                                           \
         if (small) hipLaunchKernelGGL((sample_kernel<DT, 256>), grid, dim3(256), 0, s, p);         \
