@@ -147,7 +147,7 @@ struct Sampler {
     }
     __device__ __forceinline__ int steps() const { return n_steps + 2; }
     // f(x, i0, t) for the n steps t0, t0 + by, ..., from the one of number `from` around to the one before it: this lane's
-    // elements i0, i0 + 1, ...  Three loads are in flight.
+    // elements i0, i0 + 1, ...  Three loads are in flight (eight: 5 % slower; a row's time is its compute unit's arithmetic).
     template <class F>
     __device__ __forceinline__ void steps_of(int t0, int n, int by, int from, F&& f) const {
         if (n <= 0) return;
@@ -233,9 +233,10 @@ struct Sampler {
 
     // Finds the value at which a running sum over falling values first reaches `want` (1 <= want <= the sum of all):
     // the sum over larger values is below `want`, the sum with that value's elements is not.  MASS: sums of weights, else of
-    // elements.  want = 0: `share` of the sum of all, rounded up.
-    template <bool MASS>
-    __device__ __forceinline__ float reach(u64& want, float share, u64& before) {
+    // elements.  want = 0: `share` of the sum of all, rounded up.  `settle(from, all)` may end the search when a bin of values
+    // not below `from` is known to hold the end: it says whether it did (all: zero, or that sum).
+    template <bool MASS, class F>
+    __device__ __forceinline__ float reach(u64& want, float share, u64& before, bool& settled, F&& settle) {
         SampleLds<NT>& s = sample_lds<NT>();
         const float least = MASS ? low : -3.402823466e38f;
         const float span = static_cast<float>(kOctaves / a);  // logits per kOctaves octaves of weight
@@ -245,6 +246,7 @@ struct Sampler {
             return static_cast<int>(fminf(d, kBins - 1.0f));
         };
         before = 0;
+        u64 all = 0;
         float from = least, to = top;  // the value lies among these
         uint32_t lo = 0, hi = 0;       // and, after the first pass, among these keys
         int shift = -1;
@@ -276,7 +278,7 @@ struct Sampler {
                 u64 mine = 0;
 #pragma unroll
                 for (int i = 0; i < kPer; ++i) mine += s.hist[slot(tid * kPer) + i];
-                const u64 all = block_sum(mine);
+                all = block_sum(mine);
                 const double x = ceil(static_cast<double>(share) * static_cast<double>(all));
                 want = x >= 1.0 ? static_cast<u64>(x) : 1;
                 want = want > all ? all : want;
@@ -310,8 +312,12 @@ struct Sampler {
             }
             lo = __builtin_amdgcn_readfirstlane(lo);
             hi = __builtin_amdgcn_readfirstlane(hi);
-            if (lo >= hi) return value_of<DT>(hi);
             from = value_of<DT>(lo);
+            if (shift < 0 && settle(from, all)) {
+                settled = true;
+                return from;
+            }
+            if (lo >= hi) return value_of<DT>(hi);
             to = value_of<DT>(hi);
             shift = 0;
             while (((hi - lo) >> shift) >= static_cast<uint32_t>(kBins)) ++shift;
@@ -334,12 +340,12 @@ struct Sampler {
         return t < total ? t : total - 1;
     }
 
-    // ---- few candidates: those at or above `bound`; false if there are too many
-    __device__ __forceinline__ bool from_list(int r, float bound, int top_k, float top_p, float min_p, bool need_all) {
+    // ---- few candidates: those at or above `bound`; false if there are too many.  top_p is measured against `all`: known
+    // (not zero), or summed over the row (need_all), or what top_k leaves.
+    __device__ __forceinline__ bool from_list(int r, float bound, int top_k, float top_p, float min_p, u64 all, bool need_all) {
         SampleLds<NT>& s = sample_lds<NT>();
         __syncthreads();
         int n = 0, early = 0;  // of this wave; those found before its run began anew at its first step
-        u64 all = 0;
         const int first_step = run_of(wave);
         walk([&](const float (&x)[kVec], int i0, int t) {
             if (t == first_step) early = n;
@@ -420,7 +426,7 @@ struct Sampler {
         const int rank = on ? s.list.rank[tid] : 0;
         const u64 before = on ? s.list.before[tid] : 0;
         const bool in_k = on && (top_k <= 0 || rank < top_k);
-        if (!need_all) all = block_sum(in_k ? w : 0);
+        if (all == 0) all = block_sum(in_k ? w : 0);
         bool keep = in_k;
         if (top_p < 1.0f) keep = keep && static_cast<double>(before) < static_cast<double>(top_p) * static_cast<double>(all);
         if (min_p > 0.0f) keep = keep && static_cast<double>(w) >= static_cast<double>(min_p) * 0x1p44;
@@ -639,22 +645,24 @@ struct Sampler {
         // ---- a bound that all that can be kept lies at or above
         float bound = -INFINITY;
         if (top_k > 0 && top_k <= kTopKList) {
-            // The top_k-th largest partial maximum, or a little below it: by number, over the upper halves of the keys, from the
-            // top down.  (Where it lies more than kBins of them down there is no bound, and the general way is taken.)
-            const uint32_t high = key_of<ASRFE_DT_F32>(top) >> 16;
+            // The top_k-th largest partial maximum, or a little below it: by number, over the distance from the top, in
+            // bins of a hundredth of it or so (its upper bits, from 2^-16 on).  d < e is l > top - e, exactly: e has few bits,
+            // and roundings keep the order.  (Where it lies 2^16 and more down there is no bound: the general way.)
+            constexpr int kFine = 23 - (kBins == 4096 ? 7 : 6);
+            constexpr uint32_t kLeast = 111u << 23;  // 2^-16
             for (int i = tid; i < kBins + kBins / kPer; i += NT) s.hist[i] = 0;
             __syncthreads();
 #pragma unroll
             for (int i = 0; i < kSub; ++i) {
-                const uint32_t down = high - (key_of<ASRFE_DT_F32>(part[i]) >> 16);
-                if (down < static_cast<uint32_t>(kBins) && part[i] >= -3.402823466e38f) atomicAdd(&s.hist[slot(down)], u64{1});
+                const uint32_t d = __float_as_uint(fmaxf(top - part[i], 0.0f)), b = d < kLeast ? 0 : (d - kLeast) >> kFine;
+                if (b < static_cast<uint32_t>(kBins) && part[i] >= -3.402823466e38f) atomicAdd(&s.hist[slot(static_cast<int>(b))], u64{1});
             }
             if (tid == 0) s.res[1] = kBins;
             __syncthreads();
             u64 sum = 0;
             find_bin(static_cast<u64>(top_k), sum);
-            const uint32_t down = static_cast<uint32_t>(s.res[1]);
-            if (down < static_cast<uint32_t>(kBins)) bound = fmaxf(value_of<ASRFE_DT_F32>((high - down) << 16), -3.402823466e38f);
+            const uint32_t b = static_cast<uint32_t>(s.res[1]);
+            if (b < static_cast<uint32_t>(kBins)) bound = fmaxf(top - __uint_as_float(kLeast + ((b + 1) << kFine)), -3.402823466e38f);
         }
         // (top_p measures against all that top_k leaves: the list has to hold that, whatever min_p drops afterwards)
         if (min_p > 0.0f && !(some_k && top_p < 1.0f)) {
@@ -664,8 +672,11 @@ struct Sampler {
         }
         if (bound > -INFINITY) {
             bound = fminf(bound, top);
-            if (from_list(r, bound, top_k, top_p, min_p, top_p < 1.0f && !some_k)) return false;
+            if (from_list(r, bound, top_k, top_p, min_p, 0, top_p < 1.0f && !some_k)) return false;
         }
+        float most[kSub / 4];
+#pragma unroll
+        for (int i = 0; i < kSub / 4; ++i) most[i] = fmaxf(fmaxf(part[4 * i], part[4 * i + 1]), fmaxf(part[4 * i + 2], part[4 * i + 3]));
         // ---- the general way
         cut = low;  // without a filter all that has a weight is kept
         if (some_k) {
@@ -677,12 +688,13 @@ struct Sampler {
             n = block_sum(n);
             if (n > static_cast<u64>(top_k)) {
                 u64 want = static_cast<u64>(top_k);
-                cut = reach<false>(want, 0.0f, before);
+                bool never = false;
+                cut = reach<false>(want, 0.0f, before, never, [](float, u64) { return false; });
                 ties = want - before;
             }
         }
         if (top_p < 1.0f) {
-            u64 want = 0;
+            u64 want = 0, left = 0;
             if (some_k) {  // a share of what top_k leaves
                 u64 n = 0, same = 0;
                 walk([&](const float (&x)[kVec], int, int) {
@@ -699,8 +711,18 @@ struct Sampler {
                 const double x = ceil(static_cast<double>(top_p) * static_cast<double>(n));
                 want = x >= 1.0 ? static_cast<u64>(x) : 1;
                 want = want > n ? n : want;
+                left = n;
             }
-            cut = reach<true>(want, top_p, before);
+            bool settled = false;
+            cut = reach<true>(want, top_p, before, settled, [&](float from, u64 all) {
+                // Few values go into a list.  How many there are is not known, but most of few are maxima of a thread: 256 are
+                // 226 of 1024 maxima, or 201 of 512, where they lie anywhere.
+                int many = 0;
+#pragma unroll
+                for (int i = 0; i < kSub / 4; ++i) many += most[i] >= from;
+                return block_sum(static_cast<u64>(many)) <= kList / 8 * 7 && from_list(r, from, top_k, top_p, min_p, some_k ? left : all, false);
+            });
+            if (settled) return false;
             each = weight(cut);
             ties = (want - before + each - 1) / each;
         }
@@ -725,7 +747,7 @@ struct Sampler {
 };
 
 template <int DT, int NT>
-__global__ __launch_bounds__(NT) void sample_kernel(const SampleParams p) {
+__global__ __launch_bounds__(NT, 4) void sample_kernel(const SampleParams p) {
     const int r = blockIdx.x;
     if (p.token_num && r % p.rows_per >= p.token_num[r / p.rows_per]) {
         if (threadIdx.x == 0) {
