@@ -19,6 +19,7 @@
 namespace asrfe {
 
 typedef unsigned long long u64;
+typedef u64 u64x2 __attribute__((ext_vector_type(2)));
 
 constexpr int kList = 256;        // candidates the list path takes
 constexpr int kTopKList = 200;    // largest top_k that tries it: the list holds ties and near misses too
@@ -60,21 +61,22 @@ __device__ __forceinline__ u64 wave_scan(u64 v) {  // sum up to and with this la
 template <int NT>
 struct SampleLds {
     static constexpr int kWaves = NT / 64;
-    // (256 rows of 131072 in 32 bits under top_p: 156 to 160 us with 4096 bins, 154 with 16384, which short rows take 1 us to clear)
-    static constexpr int kBins = NT == 1024 ? 4096 : 2048, kPer = kBins / NT;
-    // place of a bin: a thread sums kPer neighbours, one place of padding behind them keeps threads on banks of their own
-    __device__ __forceinline__ static int slot(int bin) { return bin + bin / kPer; }
+    // A histogram of its own per wave, so that the mass a cut leaves to every wave's run of the vocabulary is known with the
+    // cut.  Their bins of weights are 2^kBinBits / 1024 octaves wide.
+    static constexpr int kBinBits = NT == 1024 ? 6 : 7, kBins = static_cast<int>(kOctaves * 1024) >> kBinBits;
+    static constexpr int kNear = NT == 1024 ? 4096 : 2048;  // bins of the search for a bound
     double table[1024];  // 2^(j / 1024)
     u64 a[kWaves], b[kWaves];
     union {
-        u64 hist[kBins + kBins / kPer];
+        u64 hist[kWaves * kBins];
+        uint32_t near[kNear];
         struct {
             float value[kWaves][kList];
             int index[kWaves][kList];
         } found;
     };
     struct {
-        struct {
+        struct alignas(16) {
             u64 order;   // key, then the place in the list from behind: unique, larger ones come first
             u64 weight;
         } entry[kList];
@@ -98,15 +100,15 @@ __device__ __forceinline__ SampleLds<NT>& sample_lds() {
 template <int DT, int NT>
 struct Sampler {
     static constexpr int kWaves = NT / 64;
-    static constexpr int kBins = SampleLds<NT>::kBins, kPer = SampleLds<NT>::kPer;
-    __device__ __forceinline__ static int slot(int bin) { return SampleLds<NT>::slot(bin); }
+    static constexpr int kBins = SampleLds<NT>::kBins, kNear = SampleLds<NT>::kNear;
     static constexpr int kVec = DT == ASRFE_DT_F32 ? 4 : 8;
     static constexpr int kSub = NT == 1024 ? 4 : 8;  // partial maxima of a thread
 
     const SampleParams& p;
     const int tid, lane, wave;
-    const char* row;
-    int head, n_vec, n_steps;  // elements before the first 16-byte boundary, 16-byte pieces, steps of 64 of them
+    typedef __attribute__((address_space(1))) const char Global;  // (flat loads would wait for every access of the LDS, and it for them)
+    Global* row;
+    int lead, last, n_steps;   // elements of the first 16-byte piece before the row, last piece, steps of 64 pieces
     bool flat;                 // all that counts has the same logit, one without a scale (+inf, or the least there is)
     float top, low;            // largest logit, least logit with a weight
     double a, a_units;         // log2(e) / T, and 1024 times as much, for weight()
@@ -114,55 +116,59 @@ struct Sampler {
     __device__ __forceinline__ Sampler(const SampleParams& p_, int r)
         : p(p_), tid(threadIdx.x), lane(threadIdx.x & 63), wave(__builtin_amdgcn_readfirstlane(threadIdx.x >> 6)), flat(false) {
         constexpr int kSize = DT == ASRFE_DT_F32 ? 4 : 2;
-        row = static_cast<const char*>(p.logits) + static_cast<int64_t>(r) * p.ld * kSize;
-        head = static_cast<int>((16 - (reinterpret_cast<uintptr_t>(row) & 15)) & 15) / kSize;
-        head = head < p.vocab ? head : p.vocab;
-        n_vec = (p.vocab - head) / kVec;
-        n_steps = (n_vec + 63) / 64;
+        row = (Global*)p.logits + static_cast<int64_t>(r) * p.ld * kSize;
+        lead = static_cast<int>(reinterpret_cast<uintptr_t>(row) & 15) / kSize;
+        row -= lead * kSize;
+        last = (lead + p.vocab - 1) / kVec;
+        n_steps = last / 64 + 1;
     }
 
-    // The row in steps: step 0 is the head (one element per lane), then the pieces, then what is left behind the last one.
-    // This lane's 16 bytes of step t; NaN where it has no elements: no comparison holds for them, and they have no weight.
-    static constexpr uint32_t kNan = DT == ASRFE_DT_F32 ? 0x7fc00000u : DT == ASRFE_DT_F16 ? 0x7e007e00u : 0x7fc07fc0u;
-    __device__ __forceinline__ int first_of(int t) const {  // its first element
-        return t == 0 ? lane : t <= n_steps ? head + ((t - 1) * 64 + lane) * kVec : head + n_vec * kVec + lane;
-    }
+    // The row in steps of 64 aligned pieces of 16 bytes.  The first and the last piece may hold elements that are not the row's (a
+    // piece with one of the row's lies inside its allocation's granule), and lanes behind the last piece read that one again:
+    // at() makes them all NaN, for which no comparison holds, and which has no weight.  Loads take no branch, so they stay in
+    // flight while other pieces are worked on.
+    __device__ __forceinline__ int steps() const { return n_steps; }
+    __device__ __forceinline__ int first_of(int t) const { return (t * 64 + lane) * kVec - lead; }  // this lane's first element
     __device__ __forceinline__ u32x4 load(int t) const {
-        u32x4 w = {kNan, kNan, kNan, kNan};
-        const int i = first_of(t);
-        if (t > 0 && t <= n_steps) {
-            if (i < head + n_vec * kVec) w = *reinterpret_cast<const u32x4*>(row + static_cast<int64_t>(i) * (16 / kVec));
-        } else if (i < (t == 0 ? head : p.vocab) && t < steps()) {
-            if constexpr (DT == ASRFE_DT_F32) w[0] = reinterpret_cast<const uint32_t*>(row)[i];
-            else w[0] = (kNan & 0xffff0000u) | reinterpret_cast<const uint16_t*>(row)[i];
-        }
-        return w;
+        const uint32_t piece = static_cast<uint32_t>(min(t * 64 + lane, last));
+        return *reinterpret_cast<__attribute__((address_space(1))) const u32x4*>(row + piece * 16);
     }
-    __device__ __forceinline__ static void widen(const u32x4 w, float (&x)[kVec]) {
+    __device__ __forceinline__ void at(int t, const u32x4 w, float (&x)[kVec]) const {
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
             if constexpr (DT == ASRFE_DT_F32) x[i] = __uint_as_float(w[i]);
             else unpack_elem2<DT == ASRFE_DT_F16>(w[i], x[2 * i], x[2 * i + 1]);
         }
+        if (t == 0 || t == n_steps - 1) {
+            const int i0 = first_of(t);
+#pragma unroll
+            for (int e = 0; e < kVec; ++e) x[e] = static_cast<unsigned>(i0 + e) < static_cast<unsigned>(p.vocab) ? x[e] : __builtin_nanf("");
+        }
     }
-    __device__ __forceinline__ int steps() const { return n_steps + 2; }
     // f(x, i0, t) for the n steps t0, t0 + by, ..., from the one of number `from` around to the one before it: this lane's
-    // elements i0, i0 + 1, ...  Three loads are in flight (eight: 5 % slower; a row's time is its compute unit's arithmetic).
-    template <class F>
+    // elements i0, i0 + 1, ...  AHEAD loads are in flight (each in registers of its own: moving them would wait for them).
+    template <int AHEAD, class F>
     __device__ __forceinline__ void steps_of(int t0, int n, int by, int from, F&& f) const {
         if (n <= 0) return;
-        int i0 = from, i1 = from + 1 < n ? from + 1 : 0;
-        u32x4 w0 = load(t0 + i0 * by), w1 = load(t0 + i1 * by), w2;
-        for (int k = 0; k < n; ++k) {
-            const int i2 = i1 + 1 < n ? i1 + 1 : 0;
-            w2 = load(t0 + i2 * by);
-            float x[kVec];
-            widen(w0, x);
-            f(x, first_of(t0 + i0 * by), t0 + i0 * by);
-            w0 = w1;
-            w1 = w2;
-            i0 = i1;
-            i1 = i2;
+        u32x4 w[AHEAD];
+        int next = from, now = from;
+#pragma unroll
+        for (int j = 0; j < AHEAD; ++j) {
+            w[j] = load(t0 + next * by);
+            next = next + 1 < n ? next + 1 : 0;
+        }
+        for (int k = 0; k < n; k += AHEAD) {
+#pragma unroll
+            for (int j = 0; j < AHEAD; ++j) {
+                if (k + j >= n) break;
+                float x[kVec];
+                const int t = t0 + now * by;
+                at(t, w[j], x);
+                w[j] = load(t0 + next * by);
+                f(x, first_of(t), t);
+                now = now + 1 < n ? now + 1 : 0;
+                next = next + 1 < n ? next + 1 : 0;
+            }
         }
     }
     // this wave's run of steps: runs follow each other in the order of the vocabulary
@@ -170,22 +176,31 @@ struct Sampler {
         const int per = (steps() + kWaves - 1) / kWaves, t = w * per;
         return t < steps() ? t : steps();
     }
-    template <class F>
+    template <int AHEAD, class F>
     __device__ __forceinline__ void walk(F&& f) const {
         // (every wave begins elsewhere in its run: all at the same distance from their runs' starts ask the same few memory
         // channels at once: 256 rows of 131072 under top_p 115 us, this way 105 us)
         const int t0 = run_of(wave), n = run_of(wave + 1) - t0;
-        steps_of(t0, n, 1, n > 0 ? wave % n : 0, f);
+        steps_of<AHEAD>(t0, n, 1, n > 0 ? wave % n : 0, f);
     }
 
     // Weight in multiples of 2^-44, with kOffset added (a sum over n values takes it off n times; whole numbers may wrap).
     // Below `low`, and for NaN, the median of three takes `low`, whose weight is zero.
     static constexpr u64 kOffset = 0x4330000000000000ull;  // bits of 2^52, whose unit is one
     __device__ __forceinline__ u64 weight_bits(float v) const {
+        int k;
+        return weight_bits(v, k);
+    }
+    // and k, its logarithm in units of 1 / 1024 octave (zero or below)
+    __device__ __forceinline__ int log_weight(float v) const {
         const double t = (static_cast<double>(__builtin_amdgcn_fmed3f(v, low, top)) - static_cast<double>(top)) * a_units;
-        constexpr double kMagic = 6755399441055744.0;  // 1.5 * 2^52: the sum's low bits are the nearest whole number
+        return static_cast<int>(__builtin_bit_cast(u64, t + kMagic));
+    }
+    static constexpr double kMagic = 6755399441055744.0;  // 1.5 * 2^52: a sum's low bits are the nearest whole number
+    __device__ __forceinline__ u64 weight_bits(float v, int& k) const {
+        const double t = (static_cast<double>(__builtin_amdgcn_fmed3f(v, low, top)) - static_cast<double>(top)) * a_units;
         const double d = t + kMagic;
-        const int k = static_cast<int>(__builtin_bit_cast(u64, d));
+        k = static_cast<int>(__builtin_bit_cast(u64, d));
         const double f = t - (d - kMagic);  // |f| <= 1 / 2, in units of 1 / 1024
         // 2^(f / 1024) = 1 + f ln 2 / 1024 + (f ln 2 / 1024)^2 / 2: the next term is below 7e-12.  (A table of 32 entries, which
         // meets no bank conflicts, and two terms more: 5 % slower.)
@@ -209,23 +224,38 @@ struct Sampler {
         return t;
     }
 
-    // The bin of the histogram at which a sum that starts at `before` reaches `want`, in s.res[1] (left as it is where none does),
-    // and the sum before it in `before`.  Every thread takes a run of bins.
-    __device__ __forceinline__ void find_bin(u64 want, u64& before) {
+    // The bin at which a sum over bins that starts at `before` reaches `want`, in s.res[1] (left as it is where none does), and
+    // the sum before it in `before`.  Every thread takes a run of N / NT bins, each the sum of ROWS.
+    template <int ROWS, int N, class T>
+    __device__ __forceinline__ void find_bin(const T* hist, u64 want, u64& before) {
         SampleLds<NT>& s = sample_lds<NT>();
-        u64 mine = 0;
+        constexpr int kPer = (N + NT - 1) / NT;
+        u64 bin[kPer], mine = 0;
 #pragma unroll
-        for (int i = 0; i < kPer; ++i) mine += s.hist[slot(tid * kPer) + i];
+        for (int i = 0; i < kPer; ++i) {
+            bin[i] = 0;
+            const int at = tid * kPer + i;
+            if (at < N) {
+#pragma unroll
+                for (int j = 0; j < ROWS; ++j) bin[i] += hist[j * N + at];
+            }
+            mine += bin[i];
+        }
         u64 sum = wave_scan(mine);
         if (lane == 63) s.b[wave] = sum;
         __syncthreads();
         for (int i = 0; i < wave; ++i) sum += s.b[i];
         sum += before - mine;
         if (sum < want && want <= sum + mine) {
-            int b = tid * kPer;
-            while (sum + s.hist[slot(b)] < want) sum += s.hist[slot(b++)];
+            int b = 0;
+#pragma unroll
+            for (int i = 0; i + 1 < kPer; ++i)
+                if (b == i && sum + bin[i] < want) {
+                    sum += bin[i];
+                    ++b;
+                }
             s.res[0] = sum;
-            s.res[1] = b;
+            s.res[1] = tid * kPer + b;
         }
         __syncthreads();
         before = s.res[0];
@@ -234,14 +264,19 @@ struct Sampler {
     // Finds the value at which a running sum over falling values first reaches `want` (1 <= want <= the sum of all):
     // the sum over larger values is below `want`, the sum with that value's elements is not.  MASS: sums of weights, else of
     // elements.  want = 0: `share` of the sum of all, rounded up.  `settle(from, all)` may end the search when a bin of values
-    // not below `from` is known to hold the end: it says whether it did (all: zero, or that sum).
+    // not below `from` is known to hold the end: it says whether it did (all: zero, or that sum).  mine: what this wave's
+    // run of the vocabulary has above the value, and of it.
+    struct Mine {
+        u64 above, same;
+    };
     template <bool MASS, class F>
-    __device__ __forceinline__ float reach(u64& want, float share, u64& before, bool& settled, F&& settle) {
+    __device__ __forceinline__ float reach(u64& want, float share, u64& before, Mine& mine_run, bool& settled, F&& settle) {
         SampleLds<NT>& s = sample_lds<NT>();
         const float least = MASS ? low : -3.402823466e38f;
         const float span = static_cast<float>(kOctaves / a);  // logits per kOctaves octaves of weight
         const float scale = fminf(static_cast<float>(kBins) / span, 3e38f);
         auto bin1 = [&](float v) {
+            if (MASS) return -log_weight(v) >> SampleLds<NT>::kBinBits;
             const float d = fmaxf((top - v) * scale, 0.0f);  // (0 * inf: the top itself)
             return static_cast<int>(fminf(d, kBins - 1.0f));
         };
@@ -252,39 +287,51 @@ struct Sampler {
         int shift = -1;
         for (;;) {
             __syncthreads();
-            for (int i = tid; i < kBins + kBins / kPer; i += NT) s.hist[i] = 0;
+            for (int i = tid; i < kWaves * kBins; i += NT) s.hist[i] = 0;
             __syncthreads();
             if (shift < 0) {
-                walk([&](const float (&x)[kVec], int, int) {
+                walk<2>([&](const float (&x)[kVec], int, int) {
                     u64 w[kVec];
+                    int at[kVec];
 #pragma unroll
                     for (int e = 0; e < kVec; ++e) {
-                        w[e] = MASS ? weight(x[e]) : u64{x[e] >= least};
+                        if (MASS) {
+                            w[e] = weight_bits(x[e], at[e]) - kOffset;
+                            at[e] = -at[e] >> SampleLds<NT>::kBinBits;
+                        } else {
+                            w[e] = x[e] >= least;
+                            at[e] = bin1(x[e]);
+                        }
                         if (e % 4 == 3) __builtin_amdgcn_sched_barrier(0);
                     }
 #pragma unroll
                     for (int e = 0; e < kVec; ++e)
-                        if (w[e] != 0) atomicAdd(&s.hist[slot(bin1(x[e]))], w[e]);
+                        if (w[e] != 0) atomicAdd(&s.hist[wave * kBins + at[e]], w[e]);
                 });
             } else {
-                walk([&](const float (&x)[kVec], int, int) {
+                walk<2>([&](const float (&x)[kVec], int, int) {
 #pragma unroll
                     for (int e = 0; e < kVec; ++e)
-                        if (x[e] >= from && x[e] <= to) atomicAdd(&s.hist[slot((hi - key_of<DT>(x[e])) >> shift)], MASS ? weight(x[e]) : u64{1});
+                        if (x[e] >= from && x[e] <= to) atomicAdd(&s.hist[wave * kBins + ((hi - key_of<DT>(x[e])) >> shift)], MASS ? weight(x[e]) : u64{1});
                 });
             }
             __syncthreads();
             if (want == 0) {
                 u64 mine = 0;
-#pragma unroll
-                for (int i = 0; i < kPer; ++i) mine += s.hist[slot(tid * kPer) + i];
+                for (int i = tid; i < kWaves * kBins; i += NT) mine += s.hist[i];
                 all = block_sum(mine);
                 const double x = ceil(static_cast<double>(share) * static_cast<double>(all));
                 want = x >= 1.0 ? static_cast<u64>(x) : 1;
                 want = want > all ? all : want;
             }
-            find_bin(want, before);
+            find_bin<kWaves, kBins>(s.hist, want, before);
             const int b = static_cast<int>(s.res[1]);
+            if (MASS) {
+                u64 mine = 0;
+                for (int i = lane; i < b; i += 64) mine += s.hist[wave * kBins + i];
+                mine_run.above += wave_sum(mine);
+                mine_run.same = s.hist[wave * kBins + b];
+            }
             if (shift < 0) {
                 // keys of the bin's values: the ends are found by trying 64 keys at a time (bins fall as keys rise)
                 const uint32_t k0 = key_of<DT>(least), k1 = key_of<DT>(top);
@@ -347,7 +394,7 @@ struct Sampler {
         __syncthreads();
         int n = 0, early = 0;  // of this wave; those found before its run began anew at its first step
         const int first_step = run_of(wave);
-        walk([&](const float (&x)[kVec], int i0, int t) {
+        walk<3>([&](const float (&x)[kVec], int i0, int t) {
             if (t == first_step) early = n;
             uint32_t take = 0;
 #pragma unroll
@@ -413,9 +460,10 @@ struct Sampler {
             u64 before = 0;
 #pragma unroll 8
             for (int j = j0; j < j1; ++j) {
-                const bool ahead = s.list.entry[j].order > order;
+                const u64x2 at = *reinterpret_cast<const u64x2*>(&s.list.entry[j]);
+                const bool ahead = at[0] > order;
                 rank += ahead;
-                before += ahead ? s.list.entry[j].weight : 0;
+                before += ahead ? at[1] : 0;
             }
             if (i < total_n && rank) {
                 atomicAdd(&s.list.rank[i], rank);
@@ -447,7 +495,7 @@ struct Sampler {
     }
 
     // ---- the number in the running sum over the vocabulary of what the cut keeps; each: the weight at the cut
-    __device__ __forceinline__ void from_cut(int r, float cut, u64 ties, u64 each) {
+    __device__ __forceinline__ void from_cut(int r, float cut, u64 ties, u64 each, const Mine& mine_run, bool known) {
         SampleLds<NT>& s = sample_lds<NT>();
         int t0 = 0, t1 = steps();
         u64 target = 0, total = 0, ties_left = ties;
@@ -455,17 +503,21 @@ struct Sampler {
         for (int level = 0; level < 2; ++level) {
             const int per = (t1 - t0 + kWaves - 1) / kWaves;
             const int w0 = t0 + wave * per < t1 ? t0 + wave * per : t1, w1 = w0 + per < t1 ? w0 + per : t1;
-            u64 above = 0, same = 0;
-            steps_of(w0, w1 - w0, 1, w1 > w0 ? wave % (w1 - w0) : 0, [&](const float (&x)[kVec], int, int) {
+            u64 above = mine_run.above, same = mine_run.same;
+            if (level > 0 || !known) {
+                above = 0;
+                int equal = 0;
+                steps_of<2>(w0, w1 - w0, 1, w1 > w0 ? wave % (w1 - w0) : 0, [&](const float (&x)[kVec], int, int) {
 #pragma unroll
-                for (int e = 0; e < kVec; ++e) {
-                    above += weight_bits(x[e] > cut ? x[e] : low);
-                    same += x[e] == cut;
-                    if (e % 4 == 3) __builtin_amdgcn_sched_barrier(0);
-                }
-            });
-            above = wave_sum(above - kOffset * static_cast<u64>((w1 - w0) * kVec));
-            same = wave_sum(same);
+                    for (int e = 0; e < kVec; ++e) {
+                        above += weight_bits(x[e] > cut ? x[e] : low);
+                        equal += x[e] == cut;
+                        if (e % 4 == 3) __builtin_amdgcn_sched_barrier(0);
+                    }
+                });
+                above = wave_sum(above - kOffset * static_cast<u64>((w1 - w0) * kVec));
+                same = wave_sum(static_cast<u64>(equal));
+            }
             __syncthreads();
             if (lane == 0) {
                 s.a[wave] = above;
@@ -499,7 +551,7 @@ struct Sampler {
         for (int t = t0; t < t1; ++t) {
             bool done = false;
             float x[kVec];
-            widen(load(t), x);
+            at(t, load(t), x);
             const int i0 = first_of(t);
             {
                 u64 above = 0, same = 0;
@@ -553,7 +605,7 @@ struct Sampler {
         for (int i = 0; i < kSub; ++i) part[i] = -INFINITY;
         int where = 0x7fffffff;
         if (greedy) {
-            steps_of(wave, (steps() - wave + kWaves - 1) / kWaves, kWaves, 0, [&](const float (&x)[kVec], int i0, int) {
+            steps_of<4>(wave, (steps() - wave + kWaves - 1) / kWaves, kWaves, 0, [&](const float (&x)[kVec], int i0, int) {
 #pragma unroll
                 for (int e = 0; e < kVec; ++e) {
                     const bool up = x[e] > part[0];
@@ -562,7 +614,7 @@ struct Sampler {
                 }
             });
         } else {
-            steps_of(wave, (steps() - wave + kWaves - 1) / kWaves, kWaves, 0, [&](const float (&x)[kVec], int, int) {
+            steps_of<4>(wave, (steps() - wave + kWaves - 1) / kWaves, kWaves, 0, [&](const float (&x)[kVec], int, int) {
 #pragma unroll
                 for (int e = 0; e < kVec; ++e) part[e % kSub] = x[e] > part[e % kSub] ? x[e] : part[e % kSub];
                 if constexpr (kVec < kSub) {  // the other half's turn
@@ -613,11 +665,13 @@ struct Sampler {
         a_units = 1024.0 * fmin(a, 4.0 * kOctaves / (static_cast<double>(top) - static_cast<double>(low)));
         float cut;
         u64 ties = ~0ull >> 1, each = 0;
+        Mine mine{};
+        bool known = false;  // `mine` is
         const bool some_k = top_k > 0 && top_k < p.vocab;
         if (low < -3.402823466e38f || top == INFINITY) {
             // a share by number, from the lowest index
             u64 n = 0;
-            walk([&](const float (&x)[kVec], int, int) {
+            walk<2>([&](const float (&x)[kVec], int, int) {
 #pragma unroll
                 for (int e = 0; e < kVec; ++e) n += x[e] == top;
             });
@@ -631,14 +685,15 @@ struct Sampler {
             top = 0.0f;  // (for the weights of what is not chosen: none)
             low = -1.0f;
             a_units = 1024.0 * 2.0 * kOctaves;
-        } else if (!filtered(r, top_k, top_p, min_p, part, cut, ties, each)) {
+        } else if (!filtered(r, top_k, top_p, min_p, part, cut, ties, each, mine, known)) {
             return;  // chosen from a list
         }
-        from_cut(r, cut, ties, each);
+        from_cut(r, cut, ties, each, mine, known);
     }
 
     // The cut of the three filters; false if the token was chosen from a list of candidates instead.
-    __device__ __forceinline__ bool filtered(int r, int top_k, float top_p, float min_p, const float (&part)[kSub], float& cut, u64& ties, u64& each) {
+    __device__ __forceinline__ bool filtered(int r, int top_k, float top_p, float min_p, const float (&part)[kSub], float& cut, u64& ties, u64& each,
+                                             Mine& mine, bool& known) {
         SampleLds<NT>& s = sample_lds<NT>();
         const bool some_k = top_k > 0 && top_k < p.vocab;
         u64 before = 0;
@@ -648,21 +703,21 @@ struct Sampler {
             // The top_k-th largest partial maximum, or a little below it: by number, over the distance from the top, in
             // bins of a hundredth of it or so (its upper bits, from 2^-16 on).  d < e is l > top - e, exactly: e has few bits,
             // and roundings keep the order.  (Where it lies 2^16 and more down there is no bound: the general way.)
-            constexpr int kFine = 23 - (kBins == 4096 ? 7 : 6);
+            constexpr int kFine = 23 - (kNear == 4096 ? 7 : 6);
             constexpr uint32_t kLeast = 111u << 23;  // 2^-16
-            for (int i = tid; i < kBins + kBins / kPer; i += NT) s.hist[i] = 0;
+            for (int i = tid; i < kNear; i += NT) s.near[i] = 0;
             __syncthreads();
 #pragma unroll
             for (int i = 0; i < kSub; ++i) {
                 const uint32_t d = __float_as_uint(fmaxf(top - part[i], 0.0f)), b = d < kLeast ? 0 : (d - kLeast) >> kFine;
-                if (b < static_cast<uint32_t>(kBins) && part[i] >= -3.402823466e38f) atomicAdd(&s.hist[slot(static_cast<int>(b))], u64{1});
+                if (b < static_cast<uint32_t>(kNear) && part[i] >= -3.402823466e38f) atomicAdd(&s.near[b], 1u);
             }
-            if (tid == 0) s.res[1] = kBins;
+            if (tid == 0) s.res[1] = kNear;
             __syncthreads();
             u64 sum = 0;
-            find_bin(static_cast<u64>(top_k), sum);
+            find_bin<1, kNear>(s.near, static_cast<u64>(top_k), sum);
             const uint32_t b = static_cast<uint32_t>(s.res[1]);
-            if (b < static_cast<uint32_t>(kBins)) bound = fmaxf(top - __uint_as_float(kLeast + ((b + 1) << kFine)), -3.402823466e38f);
+            if (b < static_cast<uint32_t>(kNear)) bound = fmaxf(top - __uint_as_float(kLeast + ((b + 1) << kFine)), -3.402823466e38f);
         }
         // (top_p measures against all that top_k leaves: the list has to hold that, whatever min_p drops afterwards)
         if (min_p > 0.0f && !(some_k && top_p < 1.0f)) {
@@ -681,7 +736,7 @@ struct Sampler {
         cut = low;  // without a filter all that has a weight is kept
         if (some_k) {
             u64 n = 0;
-            walk([&](const float (&x)[kVec], int, int) {
+            walk<2>([&](const float (&x)[kVec], int, int) {
 #pragma unroll
                 for (int e = 0; e < kVec; ++e) n += x[e] >= -3.402823466e38f;
             });
@@ -689,7 +744,8 @@ struct Sampler {
             if (n > static_cast<u64>(top_k)) {
                 u64 want = static_cast<u64>(top_k);
                 bool never = false;
-                cut = reach<false>(want, 0.0f, before, never, [](float, u64) { return false; });
+                Mine none{};
+                cut = reach<false>(want, 0.0f, before, none, never, [](float, u64) { return false; });
                 ties = want - before;
             }
         }
@@ -697,7 +753,7 @@ struct Sampler {
             u64 want = 0, left = 0;
             if (some_k) {  // a share of what top_k leaves
                 u64 n = 0, same = 0;
-                walk([&](const float (&x)[kVec], int, int) {
+                walk<2>([&](const float (&x)[kVec], int, int) {
 #pragma unroll
                     for (int e = 0; e < kVec; ++e) {
                         const u64 w = weight(x[e]);
@@ -714,7 +770,7 @@ struct Sampler {
                 left = n;
             }
             bool settled = false;
-            cut = reach<true>(want, top_p, before, settled, [&](float from, u64 all) {
+            cut = reach<true>(want, top_p, before, mine, settled, [&](float from, u64 all) {
                 // Few values go into a list.  How many there are is not known, but most of few are maxima of a thread: 256 are
                 // 226 of 1024 maxima, or 201 of 512, where they lie anywhere.
                 int many = 0;
@@ -725,6 +781,8 @@ struct Sampler {
             if (settled) return false;
             each = weight(cut);
             ties = (want - before + each - 1) / each;
+            mine.same /= each;
+            known = true;
         }
         if (min_p > 0.0f) {
             // the least value whose weight is at least min_p
@@ -737,6 +795,7 @@ struct Sampler {
             }
             const float c = value_of<DT>(l);
             if (c > cut) {
+                known = false;
                 cut = c;
                 ties = min_p > 1.0f ? 1 : ~0ull >> 1;
             }
