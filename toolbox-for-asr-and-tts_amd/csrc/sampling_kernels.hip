@@ -65,7 +65,7 @@ struct SampleLds {
     // cut.  Their bins of weights are 2^kBinBits / 1024 octaves wide.
     static constexpr int kBinBits = NT == 1024 ? 6 : 7, kBins = static_cast<int>(kOctaves * 1024) >> kBinBits;
     static constexpr int kNear = NT == 1024 ? 4096 : 2048;  // bins of the search for a bound
-    double table[1024];  // 2^(j / 1024)
+    double table[1024];  // 2^(44 + j / 1024)
     u64 a[kWaves], b[kWaves];
     union {
         u64 hist[kWaves * kBins];
@@ -192,23 +192,23 @@ struct Sampler {
         return weight_bits(v, k);
     }
     // and k, its logarithm in units of 1 / 1024 octave (zero or below)
-    __device__ __forceinline__ int log_weight(float v) const {
-        const double t = (static_cast<double>(__builtin_amdgcn_fmed3f(v, low, top)) - static_cast<double>(top)) * a_units;
-        return static_cast<int>(__builtin_bit_cast(u64, t + kMagic));
-    }
     static constexpr double kMagic = 6755399441055744.0;  // 1.5 * 2^52: a sum's low bits are the nearest whole number
+    __device__ __forceinline__ double below_top(float v) const {
+        return static_cast<double>(__builtin_amdgcn_fmed3f(v, low, top)) - static_cast<double>(top);
+    }
+    __device__ __forceinline__ int log_weight(float v) const { return static_cast<int>(__builtin_bit_cast(u64, __builtin_fma(below_top(v), a_units, kMagic))); }
     __device__ __forceinline__ u64 weight_bits(float v, int& k) const {
-        const double t = (static_cast<double>(__builtin_amdgcn_fmed3f(v, low, top)) - static_cast<double>(top)) * a_units;
-        const double d = t + kMagic;
+        const double x = below_top(v), d = __builtin_fma(x, a_units, kMagic);
         k = static_cast<int>(__builtin_bit_cast(u64, d));
-        const double f = t - (d - kMagic);  // |f| <= 1 / 2, in units of 1 / 1024
+        const double f = __builtin_fma(x, a_units, kMagic - d);  // |f| <= 1 / 2, in units of 1 / 1024
         // 2^(f / 1024) = 1 + f ln 2 / 1024 + (f ln 2 / 1024)^2 / 2: the next term is below 7e-12.  (A table of 32 entries, which
         // meets no bank conflicts, and two terms more: 5 % slower.)
-        const double e = f * fma(f, 2.2909787910375658e-07, 0.0006769015435155716);
-        const double tab = sample_lds<NT>().table[k & 1023];
-        // (its exponent moved by k / 1024 and 44)
-        const double w = __builtin_bit_cast(double, __builtin_bit_cast(u64, tab) + (static_cast<u64>(static_cast<uint32_t>((k >> 10) + 44)) << 52));
-        return __builtin_bit_cast(u64, fma(w, e, w + 0x1p52));
+        const double e = f * __builtin_fma(f, 2.2909787910375658e-07, 0.0006769015435155716);
+        const u64 tab = __builtin_bit_cast(u64, sample_lds<NT>().table[k & 1023]);  // 2^44 times the power
+        // (its exponent moved by k / 1024)
+        const uint32_t high = static_cast<uint32_t>(tab >> 32) + (static_cast<uint32_t>(k & ~1023) << 10);
+        const double w = __builtin_bit_cast(double, static_cast<u64>(high) << 32 | static_cast<uint32_t>(tab));
+        return __builtin_bit_cast(u64, __builtin_fma(w, e, w + 0x1p52));
     }
     __device__ __forceinline__ u64 weight(float v) const { return weight_bits(v) - kOffset; }
 
@@ -306,13 +306,22 @@ struct Sampler {
                     }
 #pragma unroll
                     for (int e = 0; e < kVec; ++e)
-                        if (w[e] != 0) atomicAdd(&s.hist[wave * kBins + at[e]], w[e]);
+                        if (MASS ? at[e] < kBins : w[e] != 0) atomicAdd(&s.hist[wave * kBins + at[e]], w[e]);
                 });
             } else {
+                // few lanes have one and fewer have two: one of each lane at a time
                 walk<2>([&](const float (&x)[kVec], int, int) {
+                    uint32_t take = 0;
 #pragma unroll
-                    for (int e = 0; e < kVec; ++e)
-                        if (x[e] >= from && x[e] <= to) atomicAdd(&s.hist[wave * kBins + ((hi - key_of<DT>(x[e])) >> shift)], MASS ? weight(x[e]) : u64{1});
+                    for (int e = 0; e < kVec; ++e) take |= x[e] >= from && x[e] <= to ? 1u << e : 0u;
+                    while (__any(take != 0)) {
+                        const int e = __builtin_ctz(take | 1u << kVec);
+                        float v = x[0];
+#pragma unroll
+                        for (int i = 1; i < kVec; ++i) v = e == i ? x[i] : v;
+                        if (take != 0) atomicAdd(&s.hist[wave * kBins + ((hi - key_of<DT>(v)) >> shift)], MASS ? weight(v) : u64{1});
+                        take &= take - 1;
+                    }
                 });
             }
             __syncthreads();
@@ -594,9 +603,10 @@ struct Sampler {
 
     __device__ __forceinline__ void run(int r) {
         SampleLds<NT>& s = sample_lds<NT>();
-        for (int i = tid; i < 1024; i += NT) s.table[i] = exp2(i / 1024.0);
         const float temp = fminf(p.temperature ? p.temperature[r] : 1.0f, 1e30f);  // (beyond it all weights are one as well)
         const bool greedy = !(temp > 0.0f);
+        if (!greedy)
+            for (int i = tid; i < 1024; i += NT) s.table[i] = exp2(i / 1024.0) * 0x1p44;
         const int top_k = p.top_k ? p.top_k[r] : 0;
         const float top_p = p.top_p ? p.top_p[r] : 1.0f, min_p = p.min_p ? p.min_p[r] : 0.0f;
         // ---- the maximum, and partial maxima of kSub places per thread; for the arg-max its first index, too
