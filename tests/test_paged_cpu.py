@@ -2,6 +2,8 @@
 device, and the oracle against independent statements (torch's own e4m3 conversion, its softmax, known answers)."""
 import ctypes as C
 import os
+import re
+import subprocess
 import sys
 
 import numpy as np
@@ -199,3 +201,26 @@ def test_oracle_sampling_known_answers():
     assert po.sample_row(np.array([np.nan, -np.inf, 2.0]), 0.9)[0] == 2
     assert po.sample_row(np.array([1.0, np.inf, 3.0, np.inf]), 0.6)[0] == 3
     assert po.sample_row(l, 0.9, temperature=0.0)[0] == 1
+
+
+# ---- the generated code ---------------------------------------------------------------------------------------------------
+HIPCC = "/opt/rocm/bin/hipcc"
+
+
+@pytest.mark.skipif(not os.path.exists(HIPCC), reason="needs hipcc to generate the kernels' assembly")
+@pytest.mark.parametrize("source", ["paged_kernels.hip", "paged_attention.hip", "sampling_kernels.hip"])
+def test_generated_code(tmp_path, source):
+    """With the Makefile's flags: no packed fp32 arithmetic, no flat access of memory (the LDS counter would wait for it), and
+    LDS-DMA loads that keep their distance from the M0 write in front of them."""
+    from tools import check_vm_queue as cq
+
+    csrc = os.path.join(ROOT, "toolbox-for-asr-and-tts_amd", "csrc")
+    path = str(tmp_path / "kernels.s")
+    subprocess.check_call([HIPCC, "-O3", "-std=c++17", "--offload-arch=gfx950", "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops",
+                           "-I" + os.path.join(ROOT, "include"), "-I" + csrc, "-S", "--cuda-device-only", "-o", path,
+                           os.path.join(csrc, source)], stderr=subprocess.DEVNULL)
+    text = open(path).read()
+    assert not re.findall(r"\bv_pk_(?:add|mul|fma)_f32", text)
+    if source == "paged_attention.hip":
+        assert cq.check_m0(path) == []
+    assert not re.findall(r"\bflat_(?:load|store)", text)
