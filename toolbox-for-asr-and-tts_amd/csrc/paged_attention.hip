@@ -136,12 +136,11 @@ __device__ __forceinline__ int first_tile(const PagedAttnParams& p, int b, int c
     return static_cast<int>(static_cast<int64_t>(cu) * p.group / RT) + b;
 }
 
-// What row tile `tile` covers of sequence b; false if none of its rows.
+// What row tile `tile` covers of a sequence; false if none of its rows.
 template <int RT, int TK>
-__device__ __forceinline__ bool span_of(const PagedAttnParams& p, int b, int tile, TileSpan& s) {
-    s.b = b;
-    const int cu0 = __builtin_amdgcn_readfirstlane(p.c.cu_q[s.b]), cu1 = __builtin_amdgcn_readfirstlane(p.c.cu_q[s.b + 1]);
-    const int kv = __builtin_amdgcn_readfirstlane(p.c.kv_lens[s.b]);
+__device__ __forceinline__ bool span_of(const PagedAttnParams& p, const Sequence& seq, int tile, TileSpan& s) {
+    s.b = seq.b;
+    const int cu0 = seq.cu0, cu1 = seq.cu1, kv = seq.len;
     const int64_t n_rows = static_cast<int64_t>((cu1 < p.n_tokens ? cu1 : p.n_tokens) - cu0) * p.group;
     const int64_t row0 = (static_cast<int64_t>(tile) - first_tile<RT>(p, s.b, cu0)) * RT;
     if (cu0 < 0 || row0 < 0 || row0 >= n_rows) return false;
@@ -165,23 +164,10 @@ __device__ __forceinline__ bool span_of(const PagedAttnParams& p, int b, int til
     return true;
 }
 
-// Row tile `tile` -> its sequence: a search of 64 sequences per step.
 template <int RT, int TK>
 __device__ __forceinline__ bool tile_span(const PagedAttnParams& p, int tile, TileSpan& s) {
-    const int lane = threadIdx.x & 63;
-    int lo = 0, span = p.c.batch, step = 1;
-    while (step * 64 < span) step *= 64;
-    for (;; step >>= 6) {
-        const int i = lo + lane * step;
-        const bool below = i < lo + span && first_tile<RT>(p, i, p.c.cu_q[i]) <= tile;
-        const int c = __builtin_popcountll(__ballot(below));
-        if (c == 0) return false;
-        lo += (c - 1) * step;
-        const int left = span - (c - 1) * step;
-        span = left < step ? left : step;
-        if (step == 1) break;
-    }
-    return span_of<RT, TK>(p, __builtin_amdgcn_readfirstlane(lo), tile, s);
+    Sequence seq;
+    return find_sequence(p.c, seq, [&](int i, int cu) { return first_tile<RT>(p, i, cu) <= tile; }) && span_of<RT, TK>(p, seq, tile, s);
 }
 
 template <int D>
@@ -991,12 +977,11 @@ __global__ __launch_bounds__(256) void paged_join_kernel(const AttnJob job) {
     __shared__ float red[8];
     const PagedAttnParams& p = job.p;
     const int t = blockIdx.x / p.n_q_heads, hq = blockIdx.x % p.n_q_heads, kvh = hq / p.group, tid = threadIdx.x;
-    const int b = __builtin_amdgcn_readfirstlane(find_sequence(p.c.cu_q, p.c.batch, t));
-    if (b < 0) return;
-    const int cu0 = p.c.cu_q[b], row = (t - cu0) * p.group + hq % p.group, r = row % RT;
-    const int tile = first_tile<RT>(p, b, cu0) + row / RT;
+    Sequence seq;
+    if (!sequence_of(p.c, t, seq)) return;
+    const int row = (t - seq.cu0) * p.group + hq % p.group, r = row % RT, tile = first_tile<RT>(p, seq.b, seq.cu0) + row / RT;
     TileSpan ts;
-    if (tile >= job.n_tiles || !span_of<RT, TK>(p, b, tile, ts)) return;
+    if (tile >= job.n_tiles || !span_of<RT, TK>(p, seq, tile, ts)) return;
     const int n_parts = Parts(job, ts.n_vt).n;
     if (n_parts == 1) return;
     const int64_t base = (static_cast<int64_t>(kvh) * job.n_tiles + tile) * job.n_split * RT + r;

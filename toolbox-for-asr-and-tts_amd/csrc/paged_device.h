@@ -8,23 +8,48 @@ namespace asrfe {
 
 typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 
-// Largest b with cu_q[b] <= t, for a wave-uniform t: every step a wave compares 64 entries and keeps the interval behind
-// the last one that is not above t, so 65535 sequences take three dependent loads.  -1 if the row belongs to nobody.
-__device__ __forceinline__ int find_sequence(const int32_t* __restrict__ cu_q, int batch, int t) {
+// A sequence, its packed rows [cu0, cu1) and its length (the same in every lane).
+struct Sequence {
+    int b, cu0, cu1, len;
+};
+
+// Largest b whose first row cu_q[b] has upto(b, cu_q[b]), for rising ones: every step a wave compares 64 entries and keeps the
+// interval behind the last one that has it, so 4096 sequences take two dependent loads.  The last step brings the rest
+// along: loading it afterwards would be one more.  False if none has it.
+template <class Upto>
+__device__ __forceinline__ bool find_sequence(const PagedView& c, Sequence& s, Upto&& upto) {
     const int lane = threadIdx.x & 63;
-    int lo = 0, span = batch + 1, step = 1;
+    int lo = 0, span = c.batch, step = 1;
     while (step * 64 < span) step *= 64;
     for (;; step >>= 6) {
         const int i = lo + lane * step;
-        const bool below = i < lo + span && cu_q[i] <= t;
-        const int c = __builtin_popcountll(__ballot(below));
-        if (c == 0) return -1;
-        lo += (c - 1) * step;
-        const int left = span - (c - 1) * step;
+        const bool in = i < lo + span;
+        int cu0 = 0, cu1 = 0, len = 0;
+        if (in) {
+            cu0 = c.cu_q[i];
+            if (step == 1) {
+                cu1 = c.cu_q[i + 1];
+                len = c.kv_lens[i];
+            }
+        }
+        const int n = __builtin_popcountll(__ballot(in && upto(i, cu0)));
+        if (n == 0) return false;
+        lo += (n - 1) * step;
+        if (step == 1) {
+            s.b = __builtin_amdgcn_readfirstlane(lo);
+            s.cu0 = __builtin_amdgcn_readlane(cu0, n - 1);
+            s.cu1 = __builtin_amdgcn_readlane(cu1, n - 1);
+            s.len = __builtin_amdgcn_readlane(len, n - 1);
+            return true;
+        }
+        const int left = span - (n - 1) * step;
         span = left < step ? left : step;
-        if (step == 1) break;
     }
-    return lo < batch ? lo : -1;
+}
+
+// The sequence of packed row t (the same in every lane); false if the row belongs to nobody.
+__device__ __forceinline__ bool sequence_of(const PagedView& c, int t, Sequence& s) {
+    return find_sequence(c, s, [&](int, int cu) { return cu <= t; }) && t < s.cu1;
 }
 
 // Page of position pos of sequence b, -1 where there is none.

@@ -25,13 +25,12 @@ __global__ __launch_bounds__(kPagedThreads) void kv_append_kernel(const KvAppend
     const int t = blockIdx.x * (kPagedThreads / 64) + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     if (t >= p.n_tokens) return;
     const int lane = threadIdx.x & 63, sub = lane / kLanes, col = lane % kLanes;
-    const int b = find_sequence(p.c.cu_q, p.c.batch, t);
-    if (b < 0) return;
-    const int len = p.c.kv_lens[b];
-    const int64_t pos64 = static_cast<int64_t>(len) - p.c.cu_q[b + 1] + t;
-    if (pos64 < 0 || pos64 >= len) return;  // (more new rows than positions)
+    Sequence seq;
+    if (!sequence_of(p.c, t, seq)) return;
+    const int64_t pos64 = static_cast<int64_t>(seq.len) - seq.cu1 + t;
+    if (pos64 < 0 || pos64 >= seq.len) return;  // (more new rows than positions)
     const int pos = static_cast<int>(pos64);
-    const int page = page_of(p.c, b, pos);
+    const int page = page_of(p.c, seq.b, pos);
     if (page < 0) return;
     for (int h0 = 0; h0 < p.c.n_heads; h0 += kRows) {
         const int h = h0 + sub;
