@@ -141,6 +141,15 @@ def test_numbers_at_the_ends(pkg, ctx):
             assert torch.equal(got, want) if want is not None else bool((got >= last).all())
 
 
+def test_temperatures_that_are_no_numbers_or_have_no_end(pkg, ctx):
+    x, _ = make(4, 3000, torch.float32, seed=17)
+    u = torch.tensor([0.9, 0.9, 0.9, 0.25], device="cuda")
+    t = torch.tensor([float("nan"), -1.0, 0.0, float("inf")], device="cuda")
+    ids, lp = pkg.sample_tokens(ctx, x, u, temperature=t)
+    assert ids[:3].tolist() == x[:3].argmax(1).tolist() and lp[:3].tolist() == [0.0, 0.0, 0.0]
+    assert int(ids[3]) == 750 and abs(float(lp[3]) + np.log(3000.0)) < 1e-6  # all weights are one: the 751st sum is the first above 750
+
+
 def test_rows_behind_an_utterances_tokens(pkg, ctx):
     x, u = make(15, 300, torch.float16, seed=4)
     num = torch.tensor([5, 0, 3], dtype=torch.int32, device="cuda")

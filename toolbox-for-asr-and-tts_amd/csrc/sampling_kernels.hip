@@ -607,8 +607,8 @@ struct Sampler {
 
     __device__ __forceinline__ void run(int r) {
         SampleLds<NT>& s = sample_lds<NT>();
-        const float temp = fminf(p.temperature ? p.temperature[r] : 1.0f, 1e30f);  // (beyond it all weights are one as well)
-        const bool greedy = !(temp > 0.0f);
+        const float given = p.temperature ? p.temperature[r] : 1.0f, temp = fminf(given, 1e30f);  // (beyond it all weights are one as well)
+        const bool greedy = !(given > 0.0f);  // (NaN, too)
         if (!greedy)
             for (int i = tid; i < 1024; i += NT) s.table[i] = exp2(i / 1024.0) * 0x1p44;
         const int top_k = p.top_k ? p.top_k[r] : 0;
