@@ -326,7 +326,7 @@ int32_t asrfe_kv_append(asrfe_ctx* ctx, const asrfe_kv_cache* cache, const void*
                         int32_t table_stride, int32_t batch, void* stream);
 
 /* Reads positions 0 .. t_max - 1 of every sequence back: k, v [batch][t_max][n_heads][head_dim] dense, of `dtype` (as in
- * asrfe_kv_append; 16-byte aligned).  Positions at and past kv_lens[b], and those of pages that do not exist, are zero.
+ * asrfe_kv_append; 16-byte aligned; batch * t_max below 2^26).  Positions at and past kv_lens[b], and those of pages that do not exist, are zero.
  * Every e4m3 code under its scale is exact in bf16 and, inside its range, in fp16 (beyond it: +-65504). */
 int32_t asrfe_kv_read(asrfe_ctx* ctx, const asrfe_kv_cache* cache, const int32_t* kv_lens, const int32_t* block_table,
                       int32_t table_stride, int32_t batch, int32_t t_max, void* k, void* v, int32_t dtype, void* stream);
@@ -337,7 +337,7 @@ int32_t asrfe_kv_read(asrfe_ctx* ctx, const asrfe_kv_cache* cache, const int32_t
  * zero.  What a row does not see has no influence on it, infinities and NaN in hidden keys or values included (a visible
  * value that is infinite counts as long as its weight does not vanish in 16 bits).  The caller's new positions have to be in the cache
  * already (asrfe_kv_append on the same stream).  q, out: elements (t, h, d) at t * token_stride + h * head_stride + d,
- * strides multiples of 8, bases 16-byte aligned, of `dtype` (F16 or BF16; the cache's own for a 16-bit cache).
+ * strides multiples of 8 (out's rows must not overlap), bases 16-byte aligned, of `dtype` (F16 or BF16; the cache's own for a 16-bit cache).
  * n_q_heads: a multiple of n_heads.  max_kv: an upper bound of kv_lens (it shapes the launch; positions past it are not
  * seen).  Scores, softmax statistics and sums are fp32; the weights p enter their product in `dtype`.
  * workspace: >= asrfe_paged_attention_workspace_bytes(...) of the same numbers, 256-byte aligned, of this call alone
@@ -360,7 +360,7 @@ int32_t asrfe_paged_attention(asrfe_ctx* ctx, const asrfe_kv_cache* cache, const
  * min_p, u: one per row; each of the first four may be NULL (1, all, all, all).  A temperature that is not above zero
  * takes the first of the order (the arg-max).  NaN logits count as -inf, and a -inf logit is never chosen; where a row
  * holds +inf logits, they share all the weight.  A row with nothing above -inf gives 0 and logprob -inf.  token_num
- * [rows / rows_per] (optional): rows r with r % rows_per >= token_num[r / rows_per] get -1 and logprob 0 (rows behind an
+ * [rows / rows_per] (optional; rows up to 2^23): rows r with r % rows_per >= token_num[r / rows_per] get -1 and logprob 0 (rows behind an
  * utterance's tokens, as asrfe_decoder_forward marks them).  Weights are formed and summed with errors below 1e-9 and
  * the sums do not depend on the order of execution: the same call gives the same bits. */
 int32_t asrfe_sample_tokens(asrfe_ctx* ctx, const void* logits, int32_t dtype, int64_t ld, int32_t rows, int32_t vocab,

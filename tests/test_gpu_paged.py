@@ -412,3 +412,14 @@ def test_python_refusals(pkg, ctx):
         with pytest.raises((ValueError, pkg.AsrfeError)):
             c.attend(q, cu, lens, table, **kw)
     assert c.attend(q[:0], cu, lens, table).shape == (0, 4, 64)
+
+
+def test_more_threads_than_a_launch_holds_are_refused(pkg, ctx):
+    """65535 sequences on 256 heads of keys are more row tiles than one launch takes (the queries repeat one row: no memory)."""
+    n, heads = 65535, 256
+    cache = pkg.PagedKvCache.allocate(ctx, 1, 16, heads, 64)
+    q = torch.zeros(1, 1, 64, dtype=F16, device="cuda").expand(n, heads, 64)
+    cu = torch.arange(n + 1, dtype=torch.int32, device="cuda")
+    lens, table = torch.ones(n, dtype=torch.int32, device="cuda"), torch.zeros(n, 1, dtype=torch.int32, device="cuda")
+    with pytest.raises(pkg.AsrfeError, match="too many"):
+        cache.attend(q, cu, lens, table)

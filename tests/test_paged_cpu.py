@@ -125,6 +125,11 @@ def test_sample_refuses(abi, kw, code):
     assert abi.sample(**kw) == code
 
 
+@pytest.mark.parametrize("rc", [lambda a: a.read(batch=1 << 10, t_max=1 << 16), lambda a: a.read(batch=1, t_max=1 << 26), lambda a: a.sample(rows=(1 << 23) + 1)])
+def test_more_threads_than_a_launch_holds_are_refused(abi, rc):
+    assert rc(abi) == SHAPE
+
+
 # ---- the Python layer ---------------------------------------------------------------------------------------------------------
 def test_cache_refuses_bad_buffers(pkg):
     def make(shape=(2, 4, 16, 64), dtype=torch.float16, **kw):

@@ -83,9 +83,9 @@ extern "C" int32_t asrfe_kv_read(asrfe_ctx* ctx, const asrfe_kv_cache* cache, co
     constexpr const char* kWho = "asrfe_kv_read";
     if (!ctx) return ASRFE_ERR_BAD_ARG;
     KvReadParams p{};
+    if (t_max < 0 || static_cast<int64_t>(batch) * t_max >= (int64_t{1} << 26))  // (a wave each: a launch holds fewer than 2^32 threads)
+        return bad(ctx, ASRFE_ERR_SHAPE, kWho, "t_max >= 0, batch * t_max below 2^26");
     if (int32_t rc = view_of(ctx, kWho, cache, dtype, kv_lens, kv_lens, block_table, table_stride, batch, &p.c)) return rc;
-    if (t_max < 0 || static_cast<int64_t>(batch) * t_max > (int64_t{1} << 30))
-        return bad(ctx, ASRFE_ERR_SHAPE, kWho, "t_max >= 0, batch * t_max up to 2^30");
     if (batch == 0 || t_max == 0) return ASRFE_OK;
     if (!k || !v || !aligned16(k) || !aligned16(v)) return bad(ctx, ASRFE_ERR_BAD_ARG, kWho, "k and v must be 16-byte aligned");
     p.t_max = t_max;
@@ -145,8 +145,8 @@ extern "C" int32_t asrfe_sample_tokens(asrfe_ctx* ctx, const void* logits, int32
     constexpr const char* kWho = "asrfe_sample_tokens";
     if (!ctx) return ASRFE_ERR_BAD_ARG;
     if (dtype != ASRFE_DT_F32 && dtype != ASRFE_DT_F16 && dtype != ASRFE_DT_BF16) return bad(ctx, ASRFE_ERR_BAD_ARG, kWho, "dtype must be F32, F16 or BF16");
-    if (rows < 0 || rows > (1 << 24) || vocab < 1 || vocab > (1 << 18) || ld < vocab)
-        return bad(ctx, ASRFE_ERR_SHAPE, kWho, "rows in 0..2^24, vocab in 1..2^18, ld >= vocab");
+    if (rows < 0 || rows > (1 << 23) || vocab < 1 || vocab > (1 << 18) || ld < vocab)
+        return bad(ctx, ASRFE_ERR_SHAPE, kWho, "rows in 0..2^23, vocab in 1..2^18, ld >= vocab");
     if (token_num && rows_per < 1) return bad(ctx, ASRFE_ERR_SHAPE, kWho, "rows_per must be positive where token_num is given");
     int dev = -1;
     if (hipGetDevice(&dev) != hipSuccess || dev != ctx->device)

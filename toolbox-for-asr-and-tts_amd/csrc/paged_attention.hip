@@ -1067,7 +1067,7 @@ int64_t paged_attention_workspace(const asrfe_ctx* ctx, int head_dim, int n_head
 template <int D, bool F16, bool E4M3>
 static int32_t launch_attn(asrfe_ctx* ctx, const AttnJob& job, const AttnPlan& a, hipStream_t s) {
     const int64_t items = static_cast<int64_t>(a.n_tiles) * job.p.c.n_heads, wgs = items * a.n_split;
-    if (wgs > INT32_MAX) return set_err(ctx, ASRFE_ERR_SHAPE, "paged_attention: too many rows and heads for one launch");
+    if (wgs * 256 > UINT32_MAX) return set_err(ctx, ASRFE_ERR_SHAPE, "paged_attention: too many rows and heads for one launch");
     const dim3 grid(static_cast<uint32_t>(wgs));
     if (a.row_tile == 16 && a.one_wave) hipLaunchKernelGGL((paged_attn_few_kernel<D, F16, E4M3, 1, 1>), grid, dim3(64), 0, s, job);
     else if (a.row_tile == 16) hipLaunchKernelGGL((paged_attn_few_kernel<D, F16, E4M3, 1, 4>), grid, dim3(256), 0, s, job);
