@@ -414,6 +414,19 @@ def test_python_refusals(pkg, ctx):
     assert c.attend(q[:0], cu, lens, table).shape == (0, 4, 64)
 
 
+def test_numbers_past_32_bits_and_overlapping_results(pkg, ctx):
+    s = Setup(pkg, ctx, [(40, 3), (25, 1)], F16, None, 64, 2, 16)
+    c, (cu, lens, table), q = s.cache, s.plan(), s.rows(4, 4)
+    want = c.attend(q, cu, lens, table)
+    assert torch.equal(c.attend(q, cu, lens, table, max_kv=(1 << 32) + 8), want)
+    assert torch.equal(c.attend(q, cu, lens, table, window=1 << 32), want)
+    assert torch.equal(c.attend(q, cu, lens, table, window=5, sinks=(1 << 32) + 1), want)  # every position is a sink
+    buf = torch.zeros(4, 4, 64, dtype=F16, device="cuda")
+    for out in (buf[:1].expand(4, 4, 64), buf[:, :1].expand(4, 4, 64), buf.view(-1).as_strided((4, 4, 64), (256, 32, 1))):
+        with pytest.raises(ValueError, match="overlap"):
+            c.attend(q, cu, lens, table, out=out)
+
+
 def test_more_threads_than_a_launch_holds_are_refused(pkg, ctx):
     """65535 sequences on 256 heads of keys are more row tiles than one launch takes (the queries repeat one row: no memory)."""
     n, heads = 65535, 256

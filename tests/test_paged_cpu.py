@@ -114,7 +114,7 @@ def test_null_contexts_and_caches_are_refused(pkg):
     assert lib.asrfe_kv_append(abi.ctx, None, 16, 16, 2, 8, 8, 8, 8, 1, 16, 16, 16, 1, 1, None) == BAD
     assert lib.asrfe_paged_attention_workspace_bytes(abi.ctx, None, 1, 1, 1, 1) == -1
     assert lib.asrfe_paged_attention_workspace_bytes(None, good, 1, 4, 1, 1) == -1
-    for args in ((-1, 4, 1, 1), (1, 5, 1, 1), (1, 0, 1, 1), (1, 4, -1, 1), (1, 4, 1, -1)):
+    for args in ((-1, 4, 1, 1), (1, 5, 1, 1), (1, 0, 1, 1), (1, 4, -1, 1), (1, 4, 1, -1), (1, 4, 65536, 1), ((1 << 24) + 1, 4, 1, 1), (1, 4 * 257, 1, 1)):
         assert lib.asrfe_paged_attention_workspace_bytes(abi.ctx, good, *args) == -1
 
 

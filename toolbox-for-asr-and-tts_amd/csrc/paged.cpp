@@ -96,7 +96,8 @@ extern "C" int32_t asrfe_kv_read(asrfe_ctx* ctx, const asrfe_kv_cache* cache, co
 
 extern "C" int64_t asrfe_paged_attention_workspace_bytes(const asrfe_ctx* ctx, const asrfe_kv_cache* cache, int32_t n_tokens,
                                                          int32_t n_q_heads, int32_t batch, int32_t max_kv) {
-    if (!ctx || !cache || n_tokens < 0 || n_q_heads < 1 || batch < 0 || max_kv < 0 || cache->n_heads < 1 || n_q_heads % cache->n_heads != 0) return -1;
+    if (!ctx || !cache || n_tokens < 0 || n_tokens > (1 << 24) || batch < 0 || batch > 65535 || max_kv < 0) return -1;
+    if (cache->n_heads < 1 || cache->n_heads > 256 || n_q_heads < 1 || n_q_heads % cache->n_heads != 0 || n_q_heads / cache->n_heads > 256) return -1;
     return paged_attention_workspace(ctx, cache->head_dim, cache->n_heads, n_tokens, n_q_heads, batch, max_kv);
 }
 
@@ -120,6 +121,8 @@ extern "C" int32_t asrfe_paged_attention(asrfe_ctx* ctx, const asrfe_kv_cache* c
     if (!q || !out || !aligned16(q) || !aligned16(out)) return bad(ctx, ASRFE_ERR_BAD_ARG, kWho, "q and out must be 16-byte aligned");
     if (!stride_ok(q_token_stride) || !stride_ok(q_head_stride) || !stride_ok(out_token_stride) || !stride_ok(out_head_stride))
         return bad(ctx, ASRFE_ERR_BAD_ARG, kWho, "strides must be non-negative multiples of 8 elements");
+    if ((n_tokens > 1 && out_token_stride < cache->head_dim) || (n_q_heads > 1 && out_head_stride < cache->head_dim))
+        return bad(ctx, ASRFE_ERR_BAD_ARG, kWho, "the rows of out must not overlap");
     const int64_t need = paged_attention_workspace(ctx, cache->head_dim, cache->n_heads, n_tokens, n_q_heads, batch, max_kv);
     if (need > 0 && (!workspace || reinterpret_cast<uintptr_t>(workspace) % 256 != 0))
         return bad(ctx, ASRFE_ERR_WORKSPACE, kWho, "workspace must be 256-byte aligned");

@@ -149,10 +149,14 @@ class PagedKvCache:
             ots, ohs = self._rows("attend", "out", out, heads)
             if out.shape[0] != n or out.dtype is not q.dtype:
                 raise ValueError("PagedKvCache.attend: out must have q's shape and type")
+            if (n > 1 and ots < dim) or (heads > 1 and ohs < dim):
+                raise ValueError("PagedKvCache.attend: the rows of out must not overlap")
         if not n:
             return out
         batch, width = block_table.shape
-        max_kv = width * self.page_size if max_kv is None else int(max_kv)
+        most = width * self.page_size
+        max_kv = most if max_kv is None else min(int(max_kv), most)
+        window, sinks = min(window, 1 << 30), min(sinks, 1 << 30)  # (a position is less: what does not fit 32 bits must not wrap)
         nbytes = self.ctx.lib.asrfe_paged_attention_workspace_bytes(self.ctx.handle, self._ref, n, heads, batch, max_kv)
         if nbytes < 0:
             raise ValueError("PagedKvCache.attend: bad sizes")
