@@ -129,6 +129,28 @@ def test_rows_with_infinities_and_nan(pkg, ctx):
     assert ids.tolist() == [0, 0] and lp.tolist() == [-inf, -inf]
 
 
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("left", [1, 3, 300, 2500])
+def test_rows_that_a_mask_leaves_little_of(pkg, ctx, dtype, left):
+    x, u = make(12, 40000, dtype, seed=left)
+    g = torch.Generator(device="cuda").manual_seed(left)
+    keep = torch.rand(x.shape, generator=g, device="cuda").argsort(1) < left
+    low = torch.tensor([-float("inf"), torch.finfo(dtype).min, -60000.0], device="cuda").to(dtype).repeat(4)
+    x = torch.where(keep, x, low[:, None])
+    for settings in (dict(top_k=50), dict(top_k=200, top_p=0.9), dict(top_k=1000), dict(top_p=0.8), dict(min_p=0.05), dict(top_k=7, temperature=1e5), {}):
+        check(pkg, ctx, x, u, **settings)
+
+
+@pytest.mark.parametrize("rows, vocab", [(300, 9001), (770, 33001)])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float16, torch.bfloat16])
+def test_many_rows(pkg, ctx, rows, vocab, dtype):
+    x, u = make(rows, vocab, dtype, seed=vocab, pad=5)
+    g = torch.Generator(device="cuda").manual_seed(7)
+    pick = lambda *v: torch.tensor(v, device="cuda")[torch.randint(len(v), (rows,), generator=g, device="cuda")]  # noqa: E731
+    check(pkg, ctx, x, u, temperature=pick(0.0, 0.7, 1.0, 1.6), top_k=pick(0, 0, 20, 200, 700).int(), top_p=pick(0.3, 0.9, 0.97, 1.0),
+          min_p=pick(0.0, 0.0, 0.02, 0.2))
+
+
 def test_numbers_at_the_ends(pkg, ctx):
     """u = 0 takes the first kept token; a number outside [0, 1), which no generator gives, takes an end instead of running on."""
     x, _ = make(5, 900, torch.float32, seed=8)

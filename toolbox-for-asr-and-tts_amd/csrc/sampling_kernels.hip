@@ -716,7 +716,7 @@ struct Sampler {
         if (top_k > 0 && top_k <= kTopKList) {
             // The top_k-th largest partial maximum, or a little below it: by number, over the distance from the top, in
             // bins of a hundredth of it or so (its upper bits, from 2^-16 on).  d < e is l > top - e, exactly: e has few bits,
-            // and roundings keep the order.  (Where it lies 2^16 and more down there is no bound: the general way.)
+            // and roundings keep the order.  (Bins reach down to 2^16.)
             constexpr int kFine = 23 - (kNear == 4096 ? 7 : 6);
             constexpr uint32_t kLeast = 111u << 23;  // 2^-16
             for (int i = tid; i < kNear; i += NT) s.near[i] = 0;
@@ -732,6 +732,9 @@ struct Sampler {
             find_bin<1, kNear>(s.near, static_cast<u64>(top_k), sum);
             const uint32_t b = static_cast<uint32_t>(s.res[1]);
             if (b < static_cast<uint32_t>(kNear)) bound = fmaxf(top - __uint_as_float(kLeast + ((b + 1) << kFine)), -3.402823466e38f);
+            // fewer than top_k are so near (a mask of -inf or of the type's least value hides the others): they may be all
+            // that has a weight
+            else if (a * 65536.0 >= 2.0 * kOctaves) bound = fmaxf(top - 65536.0f, -3.402823466e38f);
         }
         // (top_p measures against all that top_k leaves: the list has to hold that, whatever min_p drops afterwards)
         if (min_p > 0.0f && !(some_k && top_p < 1.0f)) {
