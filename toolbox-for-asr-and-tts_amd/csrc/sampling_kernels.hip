@@ -78,6 +78,20 @@ __device__ __forceinline__ u64 last_lane(u64 v) {
 }
 __device__ __forceinline__ u64 wave_sum(u64 v) { return last_lane(wave_scan(v)); }
 
+// 2^(44 + j / 1024), for weight()
+struct Powers {
+    double v[1024];
+    constexpr Powers() : v() {
+        for (int j = 0; j < 1024; ++j) {
+            const double x = j * (0.6931471805599453 / 1024.0);  // e^x: 20 terms, the last below 1e-20
+            double sum = 0.0;
+            for (int i = 20; i >= 1; --i) sum = (1.0 + sum) * x / i;
+            v[j] = (1.0 + sum) * 17592186044416.0;
+        }
+    }
+};
+__device__ constexpr Powers kPowers;
+
 template <int NT>
 struct SampleLds {
     static constexpr int kWaves = NT / 64;
@@ -625,8 +639,9 @@ struct Sampler {
         SampleLds<NT>& s = sample_lds<NT>();
         const float given = p.temperature ? p.temperature[r] : 1.0f, temp = fminf(given, 1e30f);  // (beyond it all weights are one as well)
         const bool greedy = !(given > 0.0f);  // (NaN, too)
-        if (!greedy)
-            for (int i = tid; i < 1024; i += NT) s.table[i] = exp2(i / 1024.0) * 0x1p44;
+        double power[1024 / NT];  // on their way while the maximum is found
+#pragma unroll
+        for (int i = 0; i < 1024 / NT; ++i) power[i] = kPowers.v[i * NT + tid];
         const int top_k = p.top_k ? p.top_k[r] : 0;
         const float top_p = p.top_p ? p.top_p[r] : 1.0f, min_p = p.min_p ? p.min_p[r] : 0.0f;
         // ---- the maximum, and partial maxima of kSub places per thread; for the arg-max its first index, too
@@ -657,6 +672,8 @@ struct Sampler {
                 }
             });
         }
+#pragma unroll
+        for (int i = 0; i < 1024 / NT; ++i) s.table[i * NT + tid] = power[i];
         top = part[0];
 #pragma unroll
         for (int i = 1; i < kSub; ++i) top = fmaxf(top, part[i]);
