@@ -18,6 +18,17 @@ namespace asrfe {
 
 constexpr int kPagedThreads = 256;
 
+// maximum over the 8 or 16 neighbours that hold a row: pairs, fours, eights (a mirrored half row), sixteens
+template <int N>
+__device__ __forceinline__ float max_of_row(float v) {
+    auto with = [&](auto ctrl) { v = fmaxf(v, __int_as_float(__builtin_amdgcn_mov_dpp(__float_as_int(v), decltype(ctrl)::value, 0xf, 0xf, true))); };
+    with(std::integral_constant<int, 0xb1>{});
+    with(std::integral_constant<int, 0x4e>{});
+    with(std::integral_constant<int, 0x141>{});
+    if constexpr (N == 16) with(std::integral_constant<int, 0x140>{});
+    return v;
+}
+
 template <int D, bool F16, bool E4M3>
 __global__ __launch_bounds__(kPagedThreads) void kv_append_kernel(const KvAppendParams p) {
     constexpr int kLanes = D / 8;           // lanes of a row
@@ -56,8 +67,7 @@ __global__ __launch_bounds__(kPagedThreads) void kv_append_kernel(const KvAppend
                     const float a = __builtin_fabsf(f[i]);
                     top = fmaxf(top, a < INFINITY ? a : 0.0f);  // (infinities and NaN take no part)
                 }
-#pragma unroll
-                for (int o = 1; o < kLanes; o <<= 1) top = fmaxf(top, __shfl_xor(top, o));
+                top = max_of_row<kLanes>(top);
                 const uint32_t bits = __float_as_uint(top);
                 int e = static_cast<int>(bits >> 23) - 127 - ((bits & 0x7fffffu) > 0x600000u ? 7 : 8);
                 e = top > 0.0f ? (e > -126 ? e : -126) : 0;
