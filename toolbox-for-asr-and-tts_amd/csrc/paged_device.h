@@ -89,20 +89,20 @@ inline int32_t launched(asrfe_ctx* ctx, const char* who) {
     return ASRFE_OK;
 }
 
-// one instance per head width, 16-bit type and storage
-#define PAGED_DISPATCH(KERNEL, grid, block, s, p)                                                     \
+// one instance per head width, 16-bit type and storage (ONE: the kernel's last argument)
+#define PAGED_DISPATCH(KERNEL, ONE, grid, block, s, p)                                                \
     do {                                                                                              \
         const bool f16 = dtype == ASRFE_DT_F16;                                                       \
         if (head_dim == 64) {                                                                         \
-            if (f16 && e4m3) hipLaunchKernelGGL((KERNEL<64, true, true>), grid, block, 0, s, p);      \
-            else if (f16) hipLaunchKernelGGL((KERNEL<64, true, false>), grid, block, 0, s, p);        \
-            else if (e4m3) hipLaunchKernelGGL((KERNEL<64, false, true>), grid, block, 0, s, p);       \
-            else hipLaunchKernelGGL((KERNEL<64, false, false>), grid, block, 0, s, p);                \
+            if (f16 && e4m3) hipLaunchKernelGGL((KERNEL<64, true, true, ONE>), grid, block, 0, s, p); \
+            else if (f16) hipLaunchKernelGGL((KERNEL<64, true, false, ONE>), grid, block, 0, s, p);   \
+            else if (e4m3) hipLaunchKernelGGL((KERNEL<64, false, true, ONE>), grid, block, 0, s, p);  \
+            else hipLaunchKernelGGL((KERNEL<64, false, false, ONE>), grid, block, 0, s, p);           \
         } else {                                                                                      \
-            if (f16 && e4m3) hipLaunchKernelGGL((KERNEL<128, true, true>), grid, block, 0, s, p);     \
-            else if (f16) hipLaunchKernelGGL((KERNEL<128, true, false>), grid, block, 0, s, p);       \
-            else if (e4m3) hipLaunchKernelGGL((KERNEL<128, false, true>), grid, block, 0, s, p);      \
-            else hipLaunchKernelGGL((KERNEL<128, false, false>), grid, block, 0, s, p);               \
+            if (f16 && e4m3) hipLaunchKernelGGL((KERNEL<128, true, true, ONE>), grid, block, 0, s, p);\
+            else if (f16) hipLaunchKernelGGL((KERNEL<128, true, false, ONE>), grid, block, 0, s, p);  \
+            else if (e4m3) hipLaunchKernelGGL((KERNEL<128, false, true, ONE>), grid, block, 0, s, p); \
+            else hipLaunchKernelGGL((KERNEL<128, false, false, ONE>), grid, block, 0, s, p);          \
         }                                                                                             \
     } while (0)
 
