@@ -964,9 +964,88 @@ __global__ __launch_bounds__(64 * KW, (NQ == 1 ? 2 : 1)) void paged_attn_few_ker
     }
 }
 
-// Joins the parts of one row (at most kMostParts): a thread adds four channels over every eighth part or so, the sums meet in
-// the LDS.  A chain of dependent loads: 8.3 us for 2048 rows of 4 parts, 6.3 us for 128 rows of up to 128 (first loads of the
-// parts ahead of their weights change neither).
+// ---- joining parts -----------------------------------------------------------------------------------------------------
+// Row (t, hq): where its parts begin (place `at` of n, RT places apart); false if there is nothing to join.
+template <int RT, int TK>
+__device__ __forceinline__ bool parts_of(const AttnJob& job, int t, int hq, int& n, int64_t& at) {
+    const PagedAttnParams& p = job.p;
+    Sequence seq;
+    if (!sequence_of(p.c, t, seq)) return false;
+    const int row = (t - seq.cu0) * p.group + hq % p.group, tile = first_tile<RT>(p, seq.b, seq.cu0) + row / RT;
+    TileSpan ts;
+    if (tile >= job.n_tiles || !span_of<RT, TK>(p, seq, tile, ts)) return false;
+    n = Parts(job, ts.n_vt).n;
+    at = (static_cast<int64_t>(hq / p.group) * job.n_tiles + tile) * job.n_split * RT + row % RT;
+    return n > 1;
+}
+
+__device__ __forceinline__ void add(float4& a, const float4 o, float w) {
+    a.x = fmaf(o.x, w, a.x);
+    a.y = fmaf(o.y, w, a.y);
+    a.z = fmaf(o.z, w, a.z);
+    a.w = fmaf(o.w, w, a.w);
+}
+
+template <bool F16>
+__device__ __forceinline__ void put_row(const PagedAttnParams& p, int t, int hq, int ch, const float4 a, float inv) {
+    uint16_t* out = p.out + t * p.o_ts + hq * p.o_hs + ch;
+    *reinterpret_cast<uint2*>(out) = make_uint2(pack_result<F16>(a.x * inv, a.y * inv), pack_result<F16>(a.z * inv, a.w * inv));
+}
+
+// A wave joins a row of few parts: lane i weighs part i, then D / 4 lanes add four channels of a part, two or four parts at a
+// time.  (10700 rows of 64 channels in 4 parts: the whole call 35 us, 47 us with a workgroup a row.)
+constexpr int kFewParts = 16;
+
+template <int D, bool F16, int RT, int TK>
+__global__ __launch_bounds__(256) void paged_join_few_kernel(const AttnJob job) {
+    constexpr int kT = D / 4, kSlices = 64 / kT;
+    const PagedAttnParams& p = job.p;
+    const int i = blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), t = i / p.n_q_heads, hq = i % p.n_q_heads;
+    if (t >= p.n_tokens) return;
+    int n;
+    int64_t at;
+    if (!parts_of<RT, TK>(job, t, hq, n, at)) return;
+    const int lane = threadIdx.x & 63, slice = lane / kT, ch = 4 * (lane % kT);
+    float2 ml = make_float2(-INFINITY, 0.0f);
+    if (lane < n) ml = *reinterpret_cast<const float2*>(job.part_ml + (at + static_cast<int64_t>(lane) * RT) * 2);
+    const float* part = job.part_o + at * D + ch;
+    constexpr int kEarly = 4;  // on their way while the weights are found
+    float4 early[kEarly];
+#pragma unroll
+    for (int k = 0; k < kEarly; ++k) {
+        const int j = slice + k * kSlices;
+        early[k] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        if (j < n) early[k] = *reinterpret_cast<const float4*>(part + static_cast<int64_t>(j) * RT * D);
+    }
+    float top = ml.x;
+#pragma unroll
+    for (int o = kFewParts / 2; o >= 1; o >>= 1) top = fmaxf(top, __shfl_xor(top, o));
+    const float f = __builtin_amdgcn_exp2f(ml.x - (top == -INFINITY ? 0.0f : top));
+    float sum = ml.y * f;
+#pragma unroll
+    for (int o = kFewParts / 2; o >= 1; o >>= 1) sum += __shfl_xor(sum, o);
+    sum = __shfl(sum, 0);
+    float4 a = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll
+    for (int k = 0; k < kFewParts / kSlices; ++k) {
+        if (k * kSlices >= n) break;
+        const int j = slice + k * kSlices;
+        const float w = __shfl(f, j);
+        if (j < n) add(a, k < kEarly ? early[k < kEarly ? k : 0] : *reinterpret_cast<const float4*>(part + static_cast<int64_t>(j) * RT * D), w);
+    }
+#pragma unroll
+    for (int o = kT; o < 64; o <<= 1) {
+        a.x += __shfl_xor(a.x, o);
+        a.y += __shfl_xor(a.y, o);
+        a.z += __shfl_xor(a.z, o);
+        a.w += __shfl_xor(a.w, o);
+    }
+    if (slice == 0) put_row<F16>(p, t, hq, ch, a, inverse(sum));
+}
+
+// A workgroup joins a row of many (at most kMostParts): a thread adds four channels over every eighth part or so, the sums meet
+// in the LDS.  A chain of dependent loads: 6.3 us for 128 rows of up to 128 parts (first loads of the parts ahead of their
+// weights do not change it).
 constexpr int kMostParts = 256;
 
 template <int D, bool F16, int RT, int TK>
@@ -976,17 +1055,12 @@ __global__ __launch_bounds__(256) void paged_join_kernel(const AttnJob job) {
     __shared__ float4 sums[kSlices][kT];
     __shared__ float red[8];
     const PagedAttnParams& p = job.p;
-    const int t = blockIdx.x / p.n_q_heads, hq = blockIdx.x % p.n_q_heads, kvh = hq / p.group, tid = threadIdx.x;
-    Sequence seq;
-    if (!sequence_of(p.c, t, seq)) return;
-    const int row = (t - seq.cu0) * p.group + hq % p.group, r = row % RT, tile = first_tile<RT>(p, seq.b, seq.cu0) + row / RT;
-    TileSpan ts;
-    if (tile >= job.n_tiles || !span_of<RT, TK>(p, seq, tile, ts)) return;
-    const int n_parts = Parts(job, ts.n_vt).n;
-    if (n_parts == 1) return;
-    const int64_t base = (static_cast<int64_t>(kvh) * job.n_tiles + tile) * job.n_split * RT + r;
+    const int t = blockIdx.x / p.n_q_heads, hq = blockIdx.x % p.n_q_heads, tid = threadIdx.x;
+    int n;
+    int64_t at;
+    if (!parts_of<RT, TK>(job, t, hq, n, at)) return;
     float2 ml = make_float2(-INFINITY, 0.0f);
-    if (tid < n_parts) ml = *reinterpret_cast<const float2*>(job.part_ml + (base + static_cast<int64_t>(tid) * RT) * 2);
+    if (tid < n) ml = *reinterpret_cast<const float2*>(job.part_ml + (at + static_cast<int64_t>(tid) * RT) * 2);
     float top = ml.x;
 #pragma unroll
     for (int o = 32; o >= 1; o >>= 1) top = fmaxf(top, __shfl_xor(top, o));
@@ -1000,28 +1074,16 @@ __global__ __launch_bounds__(256) void paged_join_kernel(const AttnJob job) {
     for (int o = 32; o >= 1; o >>= 1) sum += __shfl_xor(sum, o);
     if ((tid & 63) == 0) red[4 + (tid >> 6)] = sum;
     __syncthreads();
-    const int d = tid % kT, slice = tid / kT;
+    const int ch = 4 * (tid % kT), slice = tid / kT;
     float4 a = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
 #pragma unroll 4
-    for (int i = slice; i < n_parts; i += kSlices) {
-        const float4 o = *reinterpret_cast<const float4*>(job.part_o + (base + static_cast<int64_t>(i) * RT) * D + 4 * d);
-        const float w = weight[i];
-        a.x = fmaf(o.x, w, a.x);
-        a.y = fmaf(o.y, w, a.y);
-        a.z = fmaf(o.z, w, a.z);
-        a.w = fmaf(o.w, w, a.w);
-    }
-    sums[slice][d] = a;
+    for (int i = slice; i < n; i += kSlices) add(a, *reinterpret_cast<const float4*>(job.part_o + (at + static_cast<int64_t>(i) * RT) * D + ch), weight[i]);
+    sums[slice][tid % kT] = a;
     __syncthreads();
     if (slice != 0) return;
 #pragma unroll
-    for (int i = 1; i < kSlices; ++i) {
-        const float4 o = sums[i][d];
-        a.x += o.x; a.y += o.y; a.z += o.z; a.w += o.w;
-    }
-    const float inv = inverse((red[4] + red[5]) + (red[6] + red[7]));
-    uint16_t* out = p.out + t * p.o_ts + hq * p.o_hs + 4 * d;
-    *reinterpret_cast<uint2*>(out) = make_uint2(pack_result<F16>(a.x * inv, a.y * inv), pack_result<F16>(a.z * inv, a.w * inv));
+    for (int i = 1; i < kSlices; ++i) add(a, sums[i][tid % kT], 1.0f);
+    put_row<F16>(p, t, hq, ch, a, inverse((red[4] + red[5]) + (red[6] + red[7])));
 }
 
 namespace {
@@ -1076,10 +1138,18 @@ static int32_t launch_attn(asrfe_ctx* ctx, const AttnJob& job, const AttnPlan& a
     else hipLaunchKernelGGL((paged_attn_many_kernel<D, F16, E4M3>), grid, dim3(256), 0, s, job);
     if (int32_t rc = launched(ctx, "paged_attention")) return rc;
     if (a.n_split == 1) return ASRFE_OK;
-    const dim3 jg(static_cast<uint32_t>(job.p.n_tokens) * job.p.n_q_heads);  // (at most 2^30: checked at the entry)
-    if (a.row_tile == 16) hipLaunchKernelGGL((paged_join_kernel<D, F16, 16, 32>), jg, dim3(256), 0, s, job);
-    else if (a.row_tile == 32) hipLaunchKernelGGL((paged_join_kernel<D, F16, 32, 32>), jg, dim3(256), 0, s, job);
-    else hipLaunchKernelGGL((paged_join_kernel<D, F16, 128, 64>), jg, dim3(256), 0, s, job);
+    const int64_t rows = static_cast<int64_t>(job.p.n_tokens) * job.p.n_q_heads;  // (at most 2^30: checked at the entry)
+    const bool few = a.n_split <= kFewParts;
+    const dim3 jg(static_cast<uint32_t>(few ? (rows + 3) / 4 : rows));
+#define JOIN(RT, TK)                                                                                              \
+    do {                                                                                                          \
+        if (few) hipLaunchKernelGGL((paged_join_few_kernel<D, F16, RT, TK>), jg, dim3(256), 0, s, job);           \
+        else hipLaunchKernelGGL((paged_join_kernel<D, F16, RT, TK>), jg, dim3(256), 0, s, job);                   \
+    } while (0)
+    if (a.row_tile == 16) JOIN(16, 32);
+    else if (a.row_tile == 32) JOIN(32, 32);
+    else JOIN(128, 64);
+#undef JOIN
     return launched(ctx, "paged_attention join");
 }
 
