@@ -1090,6 +1090,10 @@ namespace {
 // Key tiles a part has at least: below this a part costs more than the time its neighbours save (one stream of 500 positions:
 // 9.3 us whole, 10.3 us as two parts and their join).
 constexpr int kMinChunk = 16;
+// The same for 128 rows of many tiles, which a workgroup alone on its compute unit takes slowly (4 chunks of 61 tokens over 1609
+// positions 28 us with parts of 16, 21 us with parts of 8 or 4; of fewer than 24 tiles the join takes what the parts give: 8
+// chunks of 50 over 331 13 us whole, 20 us in parts of 4).
+constexpr int kManyTiles = 24, kMinChunkMany = 6;
 // Key tiles up to which one wave takes a row tile by itself (256 chunks of 10 frames under a window of 50: 13.5 us, with
 // four waves 19.9 us).
 constexpr int kOneWave = 4;
@@ -1108,7 +1112,10 @@ AttnPlan plan_of(const asrfe_ctx* ctx, int n_heads, int n_tokens, int n_q_heads,
     const int64_t tiles = window > 0 ? std::min(all, seen / a.key_tile + 3) : all;
     // enough parts for every compute unit to have several, so that sequences of different lengths even out
     const int64_t want = (a.row_tile == 128 ? 2 : 8) * ctx->num_cus;
-    auto most_of = [&](int64_t n) { return std::max<int64_t>(1, std::min<int64_t>({want / std::max<int64_t>(1, items), (n + kMinChunk - 1) / kMinChunk, kMostParts})); };
+    auto most_of = [&](int64_t n) {  // (not falling as n rises: the workspace is that of all tiles)
+        const int least = a.row_tile == 128 && n >= kManyTiles ? kMinChunkMany : kMinChunk;
+        return std::max<int64_t>(1, std::min<int64_t>({want / std::max<int64_t>(1, items), (n + least - 1) / least, kMostParts}));
+    };
     a.most_split = static_cast<int>(most_of(all));
     a.chunk = static_cast<int>((tiles + most_of(tiles) - 1) / most_of(tiles));
     a.n_split = static_cast<int>((tiles + a.chunk - 1) / a.chunk);
