@@ -144,6 +144,40 @@ def test_attend(pkg, ctx, name, dtype, store, dim):
     check_attend(s, q, out, untouched=7.0, **kw)
 
 
+def repeats(lens, heads, group, e4m3, cus, window=0, sinks=0):
+    """How often a batch has to hold `lens` for its rows to be taken in tiles of 128: rows * heads * key tiles from 64 * 3
+    (8-bit caches: 6) per compute unit on, a window's key tiles being those of its keys, the tokens of a sequence and 3."""
+    tokens = sum(q for _, q in lens)
+    tiles = -(-max(n for n, _ in lens) // 64)
+    if window:
+        tiles = min(tiles, (window + sinks + tokens // len(lens)) // 64 + 3)
+    return -(-64 * (6 if e4m3 else 3) * cus // (tokens * group * heads * tiles))
+
+
+@pytest.mark.parametrize("dtype, store, dim", [(F16, None, 128), (BF16, None, 64), (F16, E4M3, 128), (BF16, E4M3, 64)],
+                         ids=["f16-128", "bf16-64", "f16-e4m3-128", "bf16-e4m3-64"])
+@pytest.mark.parametrize("name", ["long rows", "whole chunk", "prompt", "prompt over cache", "window", "window and sinks", "many sinks", "sinks meet the window",
+                                  "empty sequences"])
+def test_attend_in_tiles_of_128_rows(pkg, ctx, name, dtype, store, dim):
+    lens, heads, group, page, kw = ATTEND[name]
+    heads = 8
+    kv = [n for n, _ in lens]
+    n = repeats(lens, heads, group, store == E4M3, torch.cuda.get_device_properties(0).multi_processor_count, kw.get("window", 0), kw.get("sinks", 0))
+    s = Setup(pkg, ctx, lens * n, dtype, store, dim, heads, page, seed=len(name))
+    q = s.rows(s.n, heads * group, 1.5)
+    assert max(kv) <= s.table.shape[1] * page < max(kv) + page
+    out = s.cache.attend(q, *s.plan(), **kw)
+    few = sorted({0, len(lens) - 1, len(lens) * (n - 1), len(lens) * n - 1})  # some of the sequences, each with its rows
+    for b in few:
+        part = Setup.__new__(Setup)
+        part.__dict__.update(s.__dict__)
+        part.kv, part.table, part.cu = s.kv[b:b + 1], s.table[b:b + 1], np.array([0, s.nq[b]])
+        part.n = int(s.nq[b])
+        at = int(s.cu[b])
+        if part.n:
+            check_attend(part, q[at:at + part.n], out[at:at + part.n], **kw)
+
+
 def test_attend_strided_output_and_one_large_score(pkg, ctx):
     """An output inside a wider array, and scores far above the rest of their row (the running maximum moves late)."""
     s = Setup(pkg, ctx, [(700, 3), (390, 40)], F16, heads=2, page=32, seed=5)
@@ -157,12 +191,13 @@ def test_attend_strided_output_and_one_large_score(pkg, ctx):
 
 
 @pytest.mark.parametrize("store", [None, E4M3], ids=["16", "e4m3"])
-@pytest.mark.parametrize("rows", [1, 3, 70, 150])
-def test_attend_hidden_infinities_and_nan(pkg, ctx, store, rows):
+@pytest.mark.parametrize("rows, others", [(1, 0), (3, 0), (70, 0), (150, 0), (70, 60), (150, 60)])  # (60 others: tiles of 128 rows)
+def test_attend_hidden_infinities_and_nan(pkg, ctx, store, rows, others):
     """What no row sees (behind the end, on pages of others) is NaN and infinite; what later rows see alone must not reach
     the earlier ones."""
-    s = Setup(pkg, ctx, [(203, rows), (180, 1)], F16, store, 128, 2, 16, seed=9)
+    s = Setup(pkg, ctx, [(203, rows), (180, 1)] + [(130, 130)] * others, F16, store, 128, 2, 16, seed=9)
     c = s.cache
+    assert not others or repeats([(203, rows), (180, 1)] + [(130, 130)] * others, 2, 2, bool(store), 256, 20, 3) == 1
     bad_page = int(s.free[0])
     for t in (c.k, c.v):
         raw = t.view(torch.uint8) if store else t

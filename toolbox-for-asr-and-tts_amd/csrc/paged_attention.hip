@@ -592,7 +592,7 @@ __global__ __launch_bounds__(256, (D == 64 && !E4M3 ? 3 : 2)) void paged_attn_ma
     if (!has_rows || rbase + l31 >= ts.n_rows) return;
     const float l_tot = l_run + __shfl_xor(l_run, 32);
     const float inv = inverse(l_tot);
-    const int64_t part_row = (static_cast<int64_t>(item) * job.n_split + part) * S::kRowTile + wave * 32 + l31;
+    const int64_t part_row = ((static_cast<int64_t>(kvh) * job.n_tiles + tile) * job.n_split + part) * S::kRowTile + wave * 32 + l31;
     uint16_t* out = p.out + (ts.tok0 + tok) * p.o_ts + hq * p.o_hs + 4 * h;
     float* po = job.part_o + part_row * D + 4 * h;
 #pragma unroll
