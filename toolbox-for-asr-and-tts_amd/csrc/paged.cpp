@@ -98,7 +98,7 @@ extern "C" int64_t asrfe_paged_attention_workspace_bytes(const asrfe_ctx* ctx, c
                                                          int32_t n_q_heads, int32_t batch, int32_t max_kv) {
     if (!ctx || !cache || n_tokens < 0 || n_tokens > (1 << 24) || batch < 0 || batch > 65535 || max_kv < 0) return -1;
     if (cache->n_heads < 1 || cache->n_heads > 256 || n_q_heads < 1 || n_q_heads % cache->n_heads != 0 || n_q_heads / cache->n_heads > 256) return -1;
-    return paged_attention_workspace(ctx, cache->head_dim, cache->n_heads, n_tokens, n_q_heads, batch, max_kv);
+    return paged_attention_workspace(ctx, cache->head_dim, cache->dtype == ASRFE_DT_E4M3, cache->n_heads, n_tokens, n_q_heads, batch, max_kv);
 }
 
 extern "C" int32_t asrfe_paged_attention(asrfe_ctx* ctx, const asrfe_kv_cache* cache, const void* q, int32_t dtype, int64_t q_token_stride,
@@ -123,7 +123,7 @@ extern "C" int32_t asrfe_paged_attention(asrfe_ctx* ctx, const asrfe_kv_cache* c
         return bad(ctx, ASRFE_ERR_BAD_ARG, kWho, "strides must be non-negative multiples of 8 elements");
     if ((n_tokens > 1 && out_token_stride < cache->head_dim) || (n_q_heads > 1 && out_head_stride < cache->head_dim))
         return bad(ctx, ASRFE_ERR_BAD_ARG, kWho, "the rows of out must not overlap");
-    const int64_t need = paged_attention_workspace(ctx, cache->head_dim, cache->n_heads, n_tokens, n_q_heads, batch, max_kv);
+    const int64_t need = paged_attention_workspace(ctx, cache->head_dim, cache->dtype == ASRFE_DT_E4M3, cache->n_heads, n_tokens, n_q_heads, batch, max_kv);
     if (need > 0 && (!workspace || reinterpret_cast<uintptr_t>(workspace) % 256 != 0))
         return bad(ctx, ASRFE_ERR_WORKSPACE, kWho, "workspace must be 256-byte aligned");
     if (workspace_bytes < need) return bad(ctx, ASRFE_ERR_WORKSPACE, kWho, "workspace too small");

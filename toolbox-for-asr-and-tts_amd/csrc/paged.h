@@ -60,7 +60,7 @@ struct SampleParams {
 
 int32_t launch_kv_append(asrfe_ctx* ctx, const KvAppendParams& p, int head_dim, int dtype, bool e4m3, hipStream_t s);
 int32_t launch_kv_read(asrfe_ctx* ctx, const KvReadParams& p, int head_dim, int dtype, bool e4m3, hipStream_t s);
-int64_t paged_attention_workspace(const asrfe_ctx* ctx, int head_dim, int n_heads, int n_tokens, int n_q_heads, int batch, int max_kv);
+int64_t paged_attention_workspace(const asrfe_ctx* ctx, int head_dim, bool e4m3, int n_heads, int n_tokens, int n_q_heads, int batch, int max_kv);
 // max_kv: the caller's number, which shapes the launch and the workspace (p.max_kv is cut to the table's width)
 int32_t launch_paged_attention(asrfe_ctx* ctx, const PagedAttnParams& p, int head_dim, int dtype, bool e4m3, void* ws, int max_kv,
                                hipStream_t s);
