@@ -4,8 +4,9 @@
 //
 //   Rows.  The query heads that share a cache head read the same keys, so the rows of a product are (token, head of the
 //   group) pairs: row r of a sequence is token r / group, head r % group.  A workgroup takes a tile of 128 rows (prompts:
-//   four waves with 32 rows each share every key tile) or of 32 rows (single tokens and short chunks: every wave has the
-//   same rows and key tiles of its own, so that four tiles are in flight and no barrier stands between them).
+//   four waves with 32 rows each share every key tile) or of 16 or 32 (single tokens, short chunks, and all calls of little
+//   work: every wave has the same rows and key tiles of its own, so that four tiles are in flight and no barrier stands
+//   between them).
 //
 //   Keys.  One pass with a running maximum and sum.  Scores are formed transposed, S^T = K Q^T (v_mfma_f32_32x32x16), so a
 //   lane holds the scores of one row; the weights are then already laid out as the operand of O^T = V^T P^T, V being read
@@ -109,8 +110,8 @@ struct AttnPlan {
 struct AttnJob {
     PagedAttnParams p;
     int n_tiles, n_split, chunk;
-    float* part_o;   // [item][part][row][D]
-    float* part_ml;  // [item][part][row][2]: running maximum (scaled, base 2) and sum
+    float* part_o;   // [head, row tile][part][row][D]
+    float* part_ml;  // [head, row tile][part][row][2]: running maximum (scaled, base 2) and sum
 };
 
 // How a row tile's n_vt key tiles are cut: never into more parts than the launch has places for, whatever the host took for

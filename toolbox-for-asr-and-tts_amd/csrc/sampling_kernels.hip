@@ -13,10 +13,10 @@
 //     * else a cut is found by histograms in the LDS, one a wave, first over the logarithm of the weight, then over the keys of
 //       the values left in the bin where the cut lies, until one value is left (or few: they go into a list, too);
 //     * the number is then looked up in the running sum over the vocabulary: per wave, per step of that wave, per lane.
-//   A row's time is its compute unit's arithmetic (20 instructions a weight, 3 a maximum): 256 rows of 131072 16-bit logits
-//   take 14 us for the arg-max (4.7 TB/s), 36 us under top_k, 50 us without a filter, 80 us under a top_p that keeps
-//   thousands, 70 us each with filters of its own; one row of 8404 in 32 bits takes 12 us with all filters, 4.4 us for the
-//   arg-max; 4000 rows of 8404 in 32 bits 80 us.
+//   A row's time is its compute unit's arithmetic (some 25 instructions a weight, 3 a maximum): 256 rows of 131072 16-bit logits
+//   take 14 us for the arg-max (4.9 TB/s), 34 us under top_k, 47 us without a filter, 75 us under a top_p that keeps
+//   thousands, 68 us each with filters of its own; one row of 8404 in 32 bits takes 10.5 us with all filters, 4.1 us for the
+//   arg-max; 4000 rows of 8404 in 32 bits 68 us.
 #include "elem.h"
 #include "paged_device.h"
 
@@ -430,9 +430,9 @@ struct Sampler {
         return t < total ? t : total - 1;
     }
 
-    // ---- few candidates: those at or above `bound`; false if there are too many.  top_p is measured against `all`: known
-    // (not zero), or summed over the row (need_all), or what top_k leaves.
-    __device__ __forceinline__ bool from_list(int r, float bound, int top_k, float top_p, float min_p, u64 all, bool need_all) {
+    // ---- few candidates: those at or above `bound`; false if there are too many.  top_p is measured against `all`, or, where
+    // that is zero, against what top_k leaves.
+    __device__ __forceinline__ bool from_list(int r, float bound, int top_k, float top_p, float min_p, u64 all) {
         SampleLds<NT>& s = sample_lds<NT>();
         __syncthreads();
         int n = 0, early = 0;  // of this wave; those found before its run began anew at its first step
@@ -444,13 +444,6 @@ struct Sampler {
             for (int e = 0; e < kVec; ++e) {
                 who[e] = __ballot(x[e] >= bound);
                 any |= who[e];
-            }
-            if (need_all) {
-#pragma unroll
-                for (int e = 0; e < kVec; ++e) {
-                    all += weight(x[e]);
-                    if (e % 4 == 3) __builtin_amdgcn_sched_barrier(0);
-                }
             }
             if (any != 0) {
                 int at = n;
@@ -470,7 +463,6 @@ struct Sampler {
                     }
             }
         });
-        if (need_all) all = block_sum(all);
         if (lane == 0) s.n[wave] = n;
         __syncthreads();
         int start = 0, total_n = 0;
@@ -774,10 +766,16 @@ struct Sampler {
             const double edge = static_cast<double>(top) + log2(fmin(static_cast<double>(min_p), 1.0)) / a;
             bound = fmaxf(bound, static_cast<float>(edge - 1e-6 * (fabs(edge) + fabs(static_cast<double>(top))) - 1e-30));
         }
-        if (bound > -INFINITY) {
-            bound = fminf(bound, top);
-            if (from_list(r, bound, top_k, top_p, min_p, 0, top_p < 1.0f && !some_k)) return false;
+        // (top_p alone measures against all of the row, whose sum comes with a histogram: then the list has its turn behind that)
+        bool few = bound > -INFINITY && (some_k || !(top_p < 1.0f));
+        if (few && !(top_k > 0 && top_k <= kTopKList)) {  // (where the partial maxima alone are too many, so are the values)
+            int many = 0;
+#pragma unroll
+            for (int i = 0; i < kSub; ++i) many += part[i] >= bound;
+            few = block_sum(static_cast<u64>(many)) <= kList;
         }
+        bound = fminf(bound, top);
+        if (few && from_list(r, bound, top_k, top_p, min_p, 0)) return false;
         float most[kSub / 4];
 #pragma unroll
         for (int i = 0; i < kSub / 4; ++i) most[i] = fmaxf(fmaxf(part[4 * i], part[4 * i + 1]), fmaxf(part[4 * i + 2], part[4 * i + 3]));
@@ -819,13 +817,14 @@ struct Sampler {
                 left = n;
             }
             bool settled = false;
-            cut = reach<true>(want, top_p, before, mine, settled, [&](float from, u64 all) {
+            cut = reach<true>(want, top_p, before, mine, settled, [&](float least, u64 all) {
+                const float from = fmaxf(least, bound);
                 // Few values go into a list.  How many there are is not known, but most of few are maxima of a thread: 256 are
                 // 226 of 1024 maxima, or 201 of 512, where they lie anywhere.
                 int many = 0;
 #pragma unroll
                 for (int i = 0; i < kSub / 4; ++i) many += most[i] >= from;
-                return block_sum(static_cast<u64>(many)) <= kList / 8 * 7 && from_list(r, from, top_k, top_p, min_p, some_k ? left : all, false);
+                return block_sum(static_cast<u64>(many)) <= kList / 8 * 7 && from_list(r, from, top_k, top_p, min_p, some_k ? left : all);
             });
             if (settled) return false;
             each = weight(cut);
