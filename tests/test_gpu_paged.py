@@ -332,6 +332,39 @@ def test_read_lengths_pages_and_types(pkg, ctx):
     assert k.shape == (0, 5, 3, 64)
 
 
+@pytest.mark.parametrize("store", [None, E4M3], ids=["16", "e4m3"])
+@pytest.mark.parametrize("heads, dim", [(1, 64), (2, 64), (3, 64), (5, 64), (1, 128), (2, 128), (3, 128)])
+def test_few_heads_share_a_wave(pkg, ctx, heads, dim, store):
+    """Neighbouring positions of a wave may belong to several sequences, have other pages, or none."""
+    lens = [(5, 1), (1, 1), (0, 0), (40, 2), (17, 1), (2, 2), (3, 1), (33, 1), (16, 1), (9, 1), (1, 1), (20, 3), (64, 1)]
+    s = Setup(pkg, ctx, lens, F16, store, dim, heads, 16, seed=heads)
+    s.table[6, 0] = -1
+    for t_max in (1, 2, 3, 21):
+        got = s.cache.read(i32(s.kv), i32(s.table), t_max)
+        for name, t in zip("kv", got):
+            want = np.zeros((len(lens), t_max, heads, dim))
+            x = values_of(s.cache, name)
+            for b in range(len(lens)):
+                for j in range(min(t_max, int(s.kv[b]))):
+                    if s.table[b, j // 16] >= 0:
+                        want[b, j] = x[s.table[b, j // 16], :, j % 16]
+            np.testing.assert_array_equal(t.double().cpu().numpy(), want)
+    k, v = s.rows(s.n + 9, heads), s.rows(s.n + 9, heads)
+    before = values_of(s.cache, "k"), values_of(s.cache, "v")
+    s.cache.append(k, v, *s.plan())
+    for x, new, name in ((before[0], k, "k"), (before[1], v, "v")):
+        new = new.double().cpu().numpy()
+        for b in range(len(lens)):
+            for i in range(int(s.nq[b])):
+                j = int(s.kv[b] - s.nq[b]) + i
+                if s.table[b, j // 16] >= 0:
+                    row = new[s.cu[b] + i]
+                    if store:
+                        row = po.dequantise(*po.quantise(row))
+                    x[s.table[b, j // 16], :, j % 16] = row
+        np.testing.assert_array_equal(values_of(s.cache, name), x)
+
+
 def test_append_of_bad_pages_writes_nothing(pkg, ctx):
     s = Setup(pkg, ctx, [(40, 40), (20, 20)], F16, None, 64, 2, 16, seed=4)
     s.table[0, 1], s.table[1, 0] = -1, 1 << 29
