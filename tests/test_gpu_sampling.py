@@ -172,6 +172,28 @@ def test_temperatures_that_are_no_numbers_or_have_no_end(pkg, ctx):
     assert int(ids[3]) == 750 and abs(float(lp[3]) + np.log(3000.0)) < 1e-6  # all weights are one: the 751st sum is the first above 750
 
 
+@pytest.mark.parametrize("dtype, rows", [(torch.float32, 9), (torch.float16, 9), (torch.bfloat16, 9), (torch.float16, 300), (torch.bfloat16, 300)])
+def test_a_cut_just_below_zero(pkg, ctx, dtype, rows):
+    """Zeros of both signs above the cut, the least negative values at and below it: bins of keys that end right below zero
+    hold no zeros.  (The maxima differ by row, so that bins end at every distance from zero; the first one's keys end
+    there in 32 bits, too.)"""
+    vocab, g = 3000, torch.Generator(device="cuda").manual_seed(3)
+    tiny = torch.finfo(dtype).smallest_normal * torch.finfo(dtype).eps  # the least subnormal
+    x = torch.full((rows, vocab), -1.0, device="cuda", dtype=torch.float64)
+    x[:, 100:300] = 0.0
+    x[:, 200:300] *= -1
+    x[:, 300:1000] = -tiny * torch.randint(1, 64 if dtype is not torch.float32 else 1 << 22, (rows, 700), generator=g, device="cuda")
+    x = x.to(dtype)
+    bits = torch.int32 if dtype is torch.float32 else torch.int16
+    top = {torch.float32: 0x3fffffff, torch.float16: 0x3fff, torch.bfloat16: 0x3fff}[dtype]
+    x[:, 0] = (top - torch.arange(rows, device="cuda")).to(bits).view(dtype)
+    x = x[:, torch.randperm(vocab, generator=g, device="cuda")].contiguous()
+    u = torch.rand(rows, generator=g, device="cuda")
+    for settings in (dict(top_k=650), dict(top_p=0.2), dict(top_k=2000, top_p=0.3)):
+        for temperature in (1.0, 100.0):
+            check(pkg, ctx, x, u, temperature=temperature, **settings)
+
+
 def test_rows_behind_an_utterances_tokens(pkg, ctx):
     x, u = make(15, 300, torch.float16, seed=4)
     num = torch.tensor([5, 0, 3], dtype=torch.int32, device="cuda")

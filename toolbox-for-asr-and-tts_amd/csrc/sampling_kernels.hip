@@ -29,7 +29,7 @@ constexpr int kList = 256;        // candidates the list path takes
 constexpr int kTopKList = 200;    // largest top_k that tries it: the list holds ties and near misses too
 constexpr double kOctaves = 46.0; // weights below 2^-45 are zero in multiples of 2^-44
 
-// an order-preserving whole number per value (16 bits for 16-bit logits); -0 and +0 have the same
+// an order-preserving whole number per value (16 bits for 16-bit logits); -0 and +0 have the same, kMinusZero + 1
 template <int DT>
 __device__ __forceinline__ uint32_t key_of(float v) {
     v += 0.0f;
@@ -137,6 +137,7 @@ struct Sampler {
     static constexpr int kBins = SampleLds<NT>::kBins, kNear = SampleLds<NT>::kNear;
     static constexpr int kVec = DT == ASRFE_DT_F32 ? 4 : 8;
     static constexpr int kSub = NT == 1024 ? 4 : 8;  // partial maxima of a thread
+    static constexpr uint32_t kMinusZero = DT == ASRFE_DT_F32 ? 0x7fffffffu : 0x7fffu;
 
     const SampleParams& p;
     const int tid, lane, wave;
@@ -402,6 +403,9 @@ struct Sampler {
             }
             lo = __builtin_amdgcn_readfirstlane(lo);
             hi = __builtin_amdgcn_readfirstlane(hi);
+            // No element has the key of -0.  As the upper end it would let zeros in, whose key lies above it: their place in the
+            // next histogram would be far outside of it.  (The bin holds an element, so a key below remains.)
+            if (hi == kMinusZero) --hi;
             from = value_of<DT>(lo);
             if (shift < 0 && settle(from, all)) {
                 settled = true;
