@@ -144,6 +144,16 @@ def test_cache_refuses_bad_buffers(pkg):
         make(dtype=torch.float8_e4m3fn, k_exp=torch.zeros(2, 4, 16), v_exp=torch.zeros(2, 4, 16))
 
 
+def test_lengths_given_as_offsets_are_refused(pkg):
+    """One tensor as kv_lens and cu_q has an entry too few: the kernels would read past its end."""
+    c = pkg.PagedKvCache.__new__(pkg.PagedKvCache)
+    c._index, c.device = -1, torch.device("cpu")  # (a host tensor's device index)
+    lens, table, x = torch.ones(3, dtype=torch.int32), torch.zeros(3, 2, dtype=torch.int32), torch.zeros(3, 4, 64)
+    for call in (lambda: c.append(x, x, lens, lens, table), lambda: c.attend(x, lens, lens, table)):
+        with pytest.raises(ValueError, match="one entry more"):
+            call()
+
+
 def test_sample_tokens_refuses_host_tensors(pkg):
     with pytest.raises(ValueError, match="CUDA"):
         pkg.sample_tokens(None, torch.zeros(2, 8), torch.zeros(2))

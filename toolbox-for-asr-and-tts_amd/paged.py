@@ -67,13 +67,13 @@ class PagedKvCache:
         return cls(ctx, k.view(dtype), v.view(dtype), *(torch.full(shape[:3], 127, dtype=torch.uint8, device=device) for _ in range(2)))
 
     # ---- checks (in the order of what is cheap to ask: small calls are bound by the host) -------------------
-    def _plan(self, who, lens, table, cu):
+    def _plan(self, who, lens, table, cu=None):
         i32, index = torch.int32, self._index
-        for t, dim in ((lens, 1), (table, 2), (cu, 1)):
+        for t, dim in ((lens, 1), (table, 2)) if cu is None else ((lens, 1), (table, 2), (cu, 1)):
             if t.dtype is not i32 or t.dim() != dim or t.get_device() != index or not t.is_contiguous():
                 raise ValueError(f"PagedKvCache.{who}: cu_q, kv_lens and block_table must be contiguous int32 tensors [B + 1], [B] and "
                                  f"[B, n] on {self.device}")
-        if table.shape[0] != lens.shape[0] or (cu is not lens and cu.shape[0] != lens.shape[0] + 1):
+        if table.shape[0] != lens.shape[0] or (cu is not None and cu.shape[0] != lens.shape[0] + 1):
             raise ValueError(f"PagedKvCache.{who}: one length and one row of the table per sequence, cu_q one entry more")
 
     def _rows(self, who, name, t, heads):
@@ -115,7 +115,7 @@ class PagedKvCache:
     def read(self, kv_lens: torch.Tensor, block_table: torch.Tensor, t_max: int, dtype: torch.dtype | None = None):
         """-> k, v [B, t_max, n_heads, head_dim]: positions 0 .. t_max - 1 of every sequence, zero at and past kv_lens[b] and
         where there is no page.  ``dtype``: of the copies (the cache's own for 16-bit caches; float16 unless given for e4m3)."""
-        self._plan("read", kv_lens, block_table, kv_lens)
+        self._plan("read", kv_lens, block_table)
         dtype = dtype or (self.dtype if self.dtype in _DT else torch.float16)
         if dtype not in _DT or (self.dtype in _DT and dtype != self.dtype):
             raise ValueError("PagedKvCache.read: dtype must be the cache's own, float16 or bfloat16 for an e4m3 cache")
