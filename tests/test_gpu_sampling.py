@@ -109,6 +109,20 @@ def test_ties_go_to_the_lowest_index(pkg, ctx, dtype):
     assert ids.tolist() == [0, 256, 512, 1023]
 
 
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("ties", [3, 300, 3000])
+def test_min_p_above_one_keeps_the_first_alone(pkg, ctx, dtype, ties):
+    g = torch.Generator(device="cuda").manual_seed(ties)
+    x = torch.randn(6, 3000, generator=g, device="cuda").clamp(max=2.0).to(dtype)
+    at = torch.rand(x.shape, generator=g, device="cuda").argsort(1)[:, :ties]
+    x.scatter_(1, at, torch.full(at.shape, 3.0, device="cuda", dtype=dtype))
+    u = torch.rand(6, generator=g, device="cuda") * 0.5 + 0.5
+    for settings in ({}, dict(top_k=2), dict(top_k=300), dict(top_k=2500), dict(top_p=0.05), dict(top_p=0.9), dict(top_k=1000, top_p=0.5)):
+        check(pkg, ctx, x, u, min_p=2.0, **settings)
+        ids, lp = pkg.sample_tokens(ctx, x, u, min_p=2.0, **settings)
+        assert torch.equal(ids.long(), at.min(1).values) and not bool(lp.any())
+
+
 def test_rows_with_infinities_and_nan(pkg, ctx):
     inf, nan = float("inf"), float("nan")
     x, u = make(12, 700, torch.float32, seed=5)

@@ -846,7 +846,7 @@ struct Sampler {
                 else l = mid + 1;
             }
             const float c = value_of<DT>(l);
-            if (c > cut) {
+            if (c > cut || min_p > 1.0f) {  // (above one: only the first of the order stays, also of ties that are the cut already)
                 known = false;
                 cut = c;
                 ties = min_p > 1.0f ? 1 : ~0ull >> 1;
