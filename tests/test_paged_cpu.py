@@ -118,6 +118,34 @@ def test_null_contexts_and_caches_are_refused(pkg):
         assert lib.asrfe_paged_attention_workspace_bytes(abi.ctx, good, *args) == -1
 
 
+@pytest.mark.parametrize("n, heads, ts, hs", [
+    (3, 4, 128, 128), (3, 4, 256, 128), (3, 4, 512, 0), (3, 4, 512, 64), (3, 4, 384, 128), (2, 4, 504, 128), (3, 4, 128, 256), (4, 3, 320, 640),
+    (9, 2, 136, 1024), (2, 8, 128 * 9 + 64, 384), (2, 2, 1 << 62, 1 << 62), (1, 4, 0, 120), (2, 1, 120, 0)])
+def test_results_that_overlap_are_refused(abi, n, heads, ts, hs):
+    assert abi.attend(n=n, heads=heads, ots=ts, ohs=hs, cache=abi.cache(n_heads=1)) == BAD and "overlap" in abi.error()
+
+
+ROWS_APART = [(3, 4, 512, 128), (3, 4, 128, 384), (1, 4, 0, 128), (4, 1, 128, 0), (2, 8, 128 * 9, 256), (4, 3, 256, 384 + 512), (2, 3, 3 * 128 + 8, 1024)]
+
+
+@pytest.mark.skipif(torch.cuda.is_available(), reason="would run on made-up pointers")
+@pytest.mark.parametrize("n, heads, ts, hs", ROWS_APART)
+def test_results_that_do_not_overlap_are_taken(abi, n, heads, ts, hs):
+    _reaches_the_device_check(abi, abi.attend(n=n, heads=heads, ots=ts, ohs=hs, cache=abi.cache(n_heads=1)))
+
+
+def test_overlap_by_its_definition(pkg):
+    """Both layers' rule against a count of the elements, over all small layouts."""
+    from toolbox_for_asr_and_tts_amd.paged import _rows_apart
+
+    for n in range(1, 5):
+        for heads in range(1, 5):
+            for ts in range(0, 34):
+                for hs in range(0, 34):
+                    at = [t * ts + h * hs + d for t in range(n) for h in range(heads) for d in range(3)]
+                    assert _rows_apart(n, heads, 3, ts, hs) == (len(set(at)) == len(at)), (n, heads, ts, hs)
+
+
 @pytest.mark.parametrize("kw, code", [
     (dict(dtype=3), BAD), (dict(dtype=9), BAD), (dict(rows=-1), SHAPE), (dict(vocab=0), SHAPE), (dict(vocab=(1 << 18) + 1, ld=1 << 20), SHAPE),
     (dict(ld=99), SHAPE), (dict(num=64, per=0), SHAPE), (dict(rows=(1 << 24) + 1), SHAPE)])

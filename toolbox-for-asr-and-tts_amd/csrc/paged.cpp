@@ -3,6 +3,7 @@
 // skip what does not exist.
 #include <algorithm>
 #include <cmath>
+#include <cstdlib>
 
 #include "paged.h"
 
@@ -11,6 +12,14 @@ using namespace asrfe;
 namespace {
 int32_t bad(asrfe_ctx* ctx, int32_t code, const char* who, const char* what) {
     return set_err(ctx, code, std::string(who) + ": " + what);
+}
+
+// (asked last: what is wrong with the arguments alone is then told without a device, too)
+int32_t on_device(asrfe_ctx* ctx, const char* who) {
+    int dev = -1;
+    if (hipGetDevice(&dev) != hipSuccess || dev != ctx->device)
+        return bad(ctx, ASRFE_ERR_BAD_ARG, who, "the context belongs to another device than the current one");
+    return ASRFE_OK;
 }
 
 bool aligned16(const void* p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; }
@@ -36,9 +45,6 @@ int32_t view_of(asrfe_ctx* ctx, const char* who, const asrfe_kv_cache* c, int32_
     if ((c->dtype == ASRFE_DT_E4M3) != (c->k_exp != nullptr) || (c->dtype == ASRFE_DT_E4M3) != (c->v_exp != nullptr))
         return bad(ctx, ASRFE_ERR_BAD_ARG, who, "k_exp and v_exp belong to an E4M3 cache and to no other");
     if (!aligned16(c->k_exp) || !aligned16(c->v_exp)) return bad(ctx, ASRFE_ERR_BAD_ARG, who, "k_exp and v_exp must be 16-byte aligned");
-    int dev = -1;
-    if (hipGetDevice(&dev) != hipSuccess || dev != ctx->device)
-        return bad(ctx, ASRFE_ERR_BAD_ARG, who, "the context belongs to another device than the current one");
     if (batch > 0 && (!kv_lens || !cu_q || (table_stride > 0 && !block_table))) return bad(ctx, ASRFE_ERR_BAD_ARG, who, "null argument");
     out->k = static_cast<char*>(c->k);
     out->v = static_cast<char*>(c->v);
@@ -56,6 +62,20 @@ int32_t view_of(asrfe_ctx* ctx, const char* who, const asrfe_kv_cache* c, int32_
 }
 
 bool stride_ok(int64_t s) { return s >= 0 && s % 8 == 0; }
+
+// Whether no two of the n x heads rows of `dim` elements at t * ts + h * hs share an element.  Mostly one stride spans all rows
+// of the other; else every distance of heads is held against the distances of tokens next to it.
+bool rows_apart(int64_t n, int64_t heads, int64_t dim, int64_t ts, int64_t hs) {
+    if ((n > 1 && ts < dim) || (heads > 1 && hs < dim)) return false;
+    if (n <= 1 || heads <= 1) return true;
+    if (ts >> 38 || hs >> 38) return false;  // (no memory is that large, and the products below stay inside 64 bits)
+    if (ts >= (heads - 1) * hs + dim || hs >= (n - 1) * ts + dim) return true;
+    for (int64_t h = 1; h < heads; ++h) {
+        const int64_t t = std::min(h * hs / ts, n - 1);
+        if (std::abs(h * hs - t * ts) < dim || (t + 1 < n && std::abs((t + 1) * ts - h * hs) < dim)) return false;
+    }
+    return true;
+}
 }  // namespace
 
 extern "C" int32_t asrfe_kv_append(asrfe_ctx* ctx, const asrfe_kv_cache* cache, const void* k, const void* v, int32_t dtype,
@@ -71,6 +91,7 @@ extern "C" int32_t asrfe_kv_append(asrfe_ctx* ctx, const asrfe_kv_cache* cache, 
     if (!k || !v || !aligned16(k) || !aligned16(v)) return bad(ctx, ASRFE_ERR_BAD_ARG, kWho, "k and v must be 16-byte aligned");
     if (!stride_ok(k_token_stride) || !stride_ok(k_head_stride) || !stride_ok(v_token_stride) || !stride_ok(v_head_stride))
         return bad(ctx, ASRFE_ERR_BAD_ARG, kWho, "strides must be non-negative multiples of 8 elements");
+    if (int32_t rc = on_device(ctx, kWho)) return rc;
     p.k = static_cast<const uint16_t*>(k);
     p.v = static_cast<const uint16_t*>(v);
     p.k_ts = k_token_stride; p.k_hs = k_head_stride; p.v_ts = v_token_stride; p.v_hs = v_head_stride;
@@ -88,6 +109,7 @@ extern "C" int32_t asrfe_kv_read(asrfe_ctx* ctx, const asrfe_kv_cache* cache, co
     if (int32_t rc = view_of(ctx, kWho, cache, dtype, kv_lens, kv_lens, block_table, table_stride, batch, &p.c)) return rc;
     if (batch == 0 || t_max == 0) return ASRFE_OK;
     if (!k || !v || !aligned16(k) || !aligned16(v)) return bad(ctx, ASRFE_ERR_BAD_ARG, kWho, "k and v must be 16-byte aligned");
+    if (int32_t rc = on_device(ctx, kWho)) return rc;
     p.t_max = t_max;
     p.k = static_cast<uint16_t*>(k);
     p.v = static_cast<uint16_t*>(v);
@@ -121,12 +143,13 @@ extern "C" int32_t asrfe_paged_attention(asrfe_ctx* ctx, const asrfe_kv_cache* c
     if (!q || !out || !aligned16(q) || !aligned16(out)) return bad(ctx, ASRFE_ERR_BAD_ARG, kWho, "q and out must be 16-byte aligned");
     if (!stride_ok(q_token_stride) || !stride_ok(q_head_stride) || !stride_ok(out_token_stride) || !stride_ok(out_head_stride))
         return bad(ctx, ASRFE_ERR_BAD_ARG, kWho, "strides must be non-negative multiples of 8 elements");
-    if ((n_tokens > 1 && out_token_stride < cache->head_dim) || (n_q_heads > 1 && out_head_stride < cache->head_dim))
+    if (!rows_apart(n_tokens, n_q_heads, cache->head_dim, out_token_stride, out_head_stride))
         return bad(ctx, ASRFE_ERR_BAD_ARG, kWho, "the rows of out must not overlap");
     const int64_t need = paged_attention_workspace(ctx, cache->head_dim, cache->dtype == ASRFE_DT_E4M3, cache->n_heads, n_tokens, n_q_heads, batch, max_kv);
     if (need > 0 && (!workspace || reinterpret_cast<uintptr_t>(workspace) % 256 != 0))
         return bad(ctx, ASRFE_ERR_WORKSPACE, kWho, "workspace must be 256-byte aligned");
     if (workspace_bytes < need) return bad(ctx, ASRFE_ERR_WORKSPACE, kWho, "workspace too small");
+    if (int32_t rc = on_device(ctx, kWho)) return rc;
     p.q = static_cast<const uint16_t*>(q);
     p.out = static_cast<uint16_t*>(out);
     p.q_ts = q_token_stride; p.q_hs = q_head_stride; p.o_ts = out_token_stride; p.o_hs = out_head_stride;
@@ -151,12 +174,10 @@ extern "C" int32_t asrfe_sample_tokens(asrfe_ctx* ctx, const void* logits, int32
     if (rows < 0 || rows > (1 << 23) || vocab < 1 || vocab > (1 << 18) || ld < vocab)
         return bad(ctx, ASRFE_ERR_SHAPE, kWho, "rows in 0..2^23, vocab in 1..2^18, ld >= vocab");
     if (token_num && rows_per < 1) return bad(ctx, ASRFE_ERR_SHAPE, kWho, "rows_per must be positive where token_num is given");
-    int dev = -1;
-    if (hipGetDevice(&dev) != hipSuccess || dev != ctx->device)
-        return bad(ctx, ASRFE_ERR_BAD_ARG, kWho, "the context belongs to another device than the current one");
     if (rows == 0) return ASRFE_OK;
     if (!logits || !u || !ids) return bad(ctx, ASRFE_ERR_BAD_ARG, kWho, "null argument");
     if (reinterpret_cast<uintptr_t>(logits) % (dtype == ASRFE_DT_F32 ? 4 : 2) != 0) return bad(ctx, ASRFE_ERR_BAD_ARG, kWho, "logits must be aligned to their type");
+    if (int32_t rc = on_device(ctx, kWho)) return rc;
     SampleParams p{};
     p.logits = logits; p.ld = ld; p.rows = rows; p.vocab = vocab; p.u = u; p.temperature = temperature; p.top_k = top_k;
     p.top_p = top_p; p.min_p = min_p; p.token_num = token_num; p.rows_per = rows_per; p.ids = ids; p.logprobs = logprobs;

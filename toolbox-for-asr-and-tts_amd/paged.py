@@ -26,6 +26,15 @@ PAGE_SIZES = (16, 32, 64, 128, 256)
 HEAD_DIMS = (64, 128)
 
 
+def _rows_apart(n, heads, dim, ts, hs):
+    """Whether no two of the n x heads rows of ``dim`` elements at t * ts + h * hs share an element."""
+    if (n > 1 and ts < dim) or (heads > 1 and hs < dim):
+        return False
+    if n == 1 or heads == 1 or ts >= (heads - 1) * hs + dim or hs >= (n - 1) * ts + dim:  # (one stride spans the other's rows)
+        return True
+    return all(abs(h * hs - t * ts) >= dim for h in range(1, heads) for t in (min(h * hs // ts, n - 1), min(h * hs // ts + 1, n - 1)))
+
+
 class PagedKvCache:
     def __init__(self, ctx: _lib.Context, k: torch.Tensor, v: torch.Tensor, k_exp: torch.Tensor | None = None,
                  v_exp: torch.Tensor | None = None):
@@ -149,7 +158,7 @@ class PagedKvCache:
             ots, ohs = self._rows("attend", "out", out, heads)
             if out.shape[0] != n or out.dtype is not q.dtype:
                 raise ValueError("PagedKvCache.attend: out must have q's shape and type")
-            if (n > 1 and ots < dim) or (heads > 1 and ohs < dim):
+            if n and not _rows_apart(n, heads, dim, ots, ohs):
                 raise ValueError("PagedKvCache.attend: the rows of out must not overlap")
         if not n:
             return out
