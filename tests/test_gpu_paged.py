@@ -216,6 +216,44 @@ def test_attend_hidden_infinities_and_nan(pkg, ctx, store, rows, others):
     check_attend(s, q, c.attend(q, *s.plan(), window=20, sinks=3), window=20, sinks=3)
 
 
+@pytest.mark.parametrize("store", [None, E4M3], ids=["16", "e4m3"])
+@pytest.mark.parametrize("lens", [[(4003, 1)], [(4003, 25), (900, 3)], [(2100, 100)] * 60], ids=["token", "chunk", "tiles of 128"])
+@pytest.mark.parametrize("nats", [9, 13, 16, 18, 21])
+def test_small_weights_beside_a_sink(pkg, ctx, nats, lens, store):
+    """The first position takes nearly all weight and has a value of zero: the result is what thousands of weights of e^-nats
+    leave.  Bound: as elsewhere, but a weight is held to 2^-34 of the largest one absolutely."""
+    s = Setup(pkg, ctx, lens, F16, store, 128, 2, 16, seed=nats)
+    assert len(lens) < 60 or repeats(lens, 2, 2, bool(store), 256) == 1
+    c, q = s.cache, s.rows(s.n, 4, 0.02)
+    q[..., 0] = 16.0  # with channel 0 of the keys, zero but for the first position's: its score is `nats`, about
+    if store:
+        c.k_exp.fill_(123)
+        c.v_exp.fill_(127)
+    first = i32(s.table[:, 0]).long()
+
+    def put(t, at, value):
+        if store:
+            t.view(torch.uint8)[at] = torch.tensor(value).to(E4M3).view(torch.uint8).item()
+        else:
+            t[at] = value
+
+    put(c.k, (..., 0), 0.0)
+    put(c.k, (first, slice(None), 0, 0), nats * 128 ** 0.5 / 16 * (16 if store else 1))
+    put(c.v, ..., 1.0)
+    put(c.v, (..., slice(1, None, 2)), 24.0)
+    put(c.v, (first, slice(None), 0), 0.0)
+    out = s.cache.attend(q, *s.plan())
+    k, v = values_of(c, "k"), values_of(c, "v")
+    rows = np.unique(np.linspace(0, s.n - 1, 12).astype(int))  # some of the rows, each as a batch of its own sequence
+    for t in rows:
+        b = int(np.searchsorted(s.cu, t, side="right") - 1)
+        n = int(s.kv[b] - s.cu[b + 1] + t + 1)
+        want, absv, reach, _ = po.attend(q[t:t + 1].double().cpu().numpy(), k, v, [0, 1], [n], s.table[b:b + 1], 16)
+        tol = bound(F16, 128, n, want, absv, reach, 0.0) + n * 24.0 * 2.0 ** -34
+        err = np.abs(out[t:t + 1].double().cpu().numpy() - want)
+        assert (err <= tol).all(), (t, n, float((err / tol).max()), float(want.max()))
+
+
 def test_attend_pages_that_do_not_exist(pkg, ctx):
     """-1 and numbers past the pool are pages that were given back; a length past the table's width has no pages there."""
     s = Setup(pkg, ctx, [(300, 1), (200, 40), (170, 3), (64, 2)], BF16, None, 64, 2, 16, seed=3)

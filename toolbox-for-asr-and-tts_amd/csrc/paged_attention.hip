@@ -20,8 +20,9 @@
 //
 //   Long caches with few rows are cut along the keys into parts, whose sums a second kernel joins.
 //
-//   Scores, maxima, sums and outputs are fp32; the weights p <= 1 are rounded to the 16 bits of the product's other operand (the
-//   sum they are divided by takes them before that), which costs an output about as much as its own rounding does.
+//   Scores, maxima, sums and outputs are fp32.  The weights are rounded to the 16 bits of the product's other operand (the sum they
+//   are divided by takes them before that): half a step of each weight, at random, so an output is off by at most as much
+//   as its own rounding adds (of sum p |v|), and less the more weights there are.  See Raised for small ones.
 #include <algorithm>
 
 #include "lds_dma.h"
@@ -53,6 +54,16 @@ template <class T>
 __device__ __forceinline__ __attribute__((address_space(3))) T* lds(uint32_t addr) {
     return (__attribute__((address_space(3))) T*)addr;
 }
+
+// Weights are 2^(score - reference), scores in base 2.  The reference is the largest score seen less kRaise, brought up to
+// that when a tile exceeds it by more than kLag: a weight is at most 2^(kLag + kRaise), the largest one seen at least 2^kRaise.
+// fp16 has little range below one: raised by 2^9, weights down to 2^-23 of the largest keep all bits of their rounding and
+// those below 2^-34 become zero in the product (without it 2^-14 and 2^-25, and such weights of 131072 positions can hold
+// 0.4 % of the sum).  Six and nine cost nothing; with four and eleven prompts under a window take 2 % longer.
+template <bool F16>
+struct Raised {
+    static constexpr float kLag = F16 ? 6.0f : 8.0f, kRaise = F16 ? 9.0f : 0.0f;
+};
 
 // 1 / a sum of weights; 0 where there were none, NaN where a score was
 __device__ __forceinline__ float inverse(float sum) { return sum > 0.0f ? 1.0f / sum : (sum == 0.0f ? 0.0f : sum); }
@@ -111,7 +122,7 @@ struct AttnJob {
     PagedAttnParams p;
     int n_tiles, n_split, chunk;
     float* part_o;   // [head, row tile][part][row][D]
-    float* part_ml;  // [head, row tile][part][row][2]: running maximum (scaled, base 2) and sum
+    float* part_ml;  // [head, row tile][part][row][2]: reference (see Raised) and sum
 };
 
 // How a row tile's n_vt key tiles are cut: never into more parts than the launch has places for, whatever the host took for
@@ -409,7 +420,7 @@ __global__ __launch_bounds__(256, (D == 64 && !E4M3 ? 3 : 2)) void paged_attn_ma
     for (int mt = 0; mt < kMt; ++mt)
 #pragma unroll
         for (int e = 0; e < 16; ++e) oacc[mt][e] = 0.0f;
-    float mc = -INFINITY, l_run = 0.0f;  // running maximum (scaled, base 2) and sum of this lane's half of the keys
+    float mc = -INFINITY, l_run = 0.0f;  // reference (see Raised) and sum of this lane's half of the keys
 
     auto compute = [&](uint32_t tile_base, int key0, uint32_t exist, bool special, auto edge_c) __attribute__((always_inline)) {
         constexpr bool edge = decltype(edge_c)::value;
@@ -470,9 +481,10 @@ __global__ __launch_bounds__(256, (D == 64 && !E4M3 ? 3 : 2)) void paged_attn_ma
             const auto sw = __builtin_amdgcn_permlane32_swap(__float_as_uint(rmax), __float_as_uint(rmax), false, false);
             rmax = fmaxf(__uint_as_float(sw[0]), __uint_as_float(sw[1]));
         }
-        // the maximum only has to keep exp2 in range: it is raised when a tile exceeds it by more than 2^8
-        const bool grew = rmax * c > mc + 8.0f;
-        const float m_new = grew ? rmax * c : mc;
+        // the maximum only has to keep the weights in range
+        const float seen = fmaf(rmax, c, -Raised<F16>::kRaise);
+        const bool grew = seen > mc + Raised<F16>::kLag;
+        const float m_new = grew ? seen : mc;
         const float alpha = grew ? __builtin_amdgcn_exp2f(mc - m_new) : 1.0f;
         mc = m_new;
         const float sub = mc == -INFINITY ? 0.0f : mc;  // (nothing seen yet: every weight below is exp2(-inf))
@@ -793,9 +805,10 @@ __global__ __launch_bounds__(64 * KW, (NQ == 1 ? 2 : 1)) void paged_attn_few_ker
 #pragma unroll
                 for (int i = 0; i < 4; ++i) rmax = fmaxf(rmax, sacc[n][u][i]);
             rmax = max_of_row(rmax);
-            // the maximum only has to keep exp2 in range: it is raised when a tile exceeds it by more than 2^8
-            const bool grew = rmax * c > mc[n] + 8.0f;
-            const float m_new = grew ? rmax * c : mc[n];
+            // the maximum only has to keep the weights in range
+            const float seen = fmaf(rmax, c, -Raised<F16>::kRaise);
+            const bool grew = seen > mc[n] + Raised<F16>::kLag;
+            const float m_new = grew ? seen : mc[n];
             const float alpha = grew ? __builtin_amdgcn_exp2f(mc[n] - m_new) : 1.0f;
             mc[n] = m_new;
             const float sub = m_new == -INFINITY ? 0.0f : m_new;  // (nothing seen yet: every weight below is exp2(-inf))
