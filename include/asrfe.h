@@ -334,8 +334,8 @@ int32_t asrfe_kv_read(asrfe_ctx* ctx, const asrfe_kv_cache* cache, const int32_t
 /* Attention of the new rows over the cache: out[t][h] = sum_j p_j v_j, p = softmax_j(scale * q[t][h] . k_j) over the
  * positions j the row sees, h's keys being those of cache head h / (n_q_heads / n_heads).  A row at position i sees j <
  * kv_lens[b] with j <= i (causal != 0), and, where window > 0, j > i - window or j < sinks.  A row that sees nothing is
- * zero.  What a row does not see has no influence on it, infinities and NaN in hidden keys or values included (a visible
- * value that is infinite counts as long as its weight does not vanish in 16 bits).  The caller's new positions have to be in the cache
+ * zero.  What a row does not see has no influence on it, infinities and NaN in hidden keys or values included; a value
+ * that it sees counts, infinite or NaN, however small its weight (unless its score is -inf).  The caller's new positions have to be in the cache
  * already (asrfe_kv_append on the same stream).  q, out: elements (t, h, d) at t * token_stride + h * head_stride + d,
  * strides multiples of 8 (out's rows must not overlap), bases 16-byte aligned, of `dtype` (F16 or BF16; the cache's own for a 16-bit cache).
  * n_q_heads: a multiple of n_heads.  max_kv: an upper bound of kv_lens (it shapes the launch; positions past it are not

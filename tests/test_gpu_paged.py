@@ -216,6 +216,63 @@ def test_attend_hidden_infinities_and_nan(pkg, ctx, store, rows, others):
     check_attend(s, q, c.attend(q, *s.plan(), window=20, sinks=3), window=20, sinks=3)
 
 
+SEEN = {
+    # name: (positions, new rows) per sequence, kw: tiles of 16 rows (one wave; four; in parts), of 32, of 128 (whole; in parts)
+    "one wave": ([(100, 1)], {}),
+    "token": ([(420, 1), (300, 1)], {}),
+    "parts": ([(9000, 1)], {}),
+    "chunk": ([(420, 20)], {}),
+    "chunk in parts": ([(5000, 25)], {}),
+    "window": ([(900, 3)], dict(window=400, sinks=40)),
+    "prompts": ([(500, 200)] * 60, {}),
+    "prompts under a window": ([(700, 300)] * 40, dict(window=300, sinks=70)),
+    "prompts in parts": ([(8000, 200)], dict(causal=False)),
+}
+
+
+@pytest.mark.parametrize("dtype, dim", [(F16, 128), (BF16, 128), (F16, 64)], ids=["f16", "bf16", "f16-64"])
+@pytest.mark.parametrize("later", [False, True], ids=["below", "left behind"])
+@pytest.mark.parametrize("name", SEEN)
+def test_values_that_are_infinite_count_however_small_their_weight(pkg, ctx, name, later, dtype, dim):
+    """Infinite values at positions inside every mask, with a weight that every format holds (20 nats below the largest: also one
+    that 16 bits lose) and with one of e^-110, of which 32 bits hold nothing: by a score of its own (`below`), or because a
+    later position's is so much larger (`left behind`).  Rows that do not see them are as if they were not there."""
+    lens, kw = SEEN[name]
+    s = Setup(pkg, ctx, lens, dtype, None, dim, 2, 32, seed=len(name))
+    c, q = s.cache, s.rows(s.n, 4, 0.1)
+    q[..., 0] = 16.0  # with channel 0 of the keys: a position's score in nats
+    c.k[..., 0] = 0.0
+    unit = dim ** 0.5 / 16
+
+    def put(b, p, nats, values):
+        page, at = int(s.table[b, p // 32]), p % 32
+        c.k[page, :, at, 0] = nats * unit
+        for (head, channel), v in values.items():
+            c.v[page, head, at, channel] = v
+
+    inf, nan = float("inf"), float("nan")
+    some = sorted({0, len(lens) - 1})
+    for b in some:
+        n, m = lens[b]
+        first = max(0, n - m - kw.get("window", n) + 2)  # positions that all rows see lie from here to n - m
+        at = [first + (n - m - first) * i // 5 for i in (0, 1, 2, 3)]
+        put(b, at[0], 0.0 if later else -110.0, {(0, 3): inf, (1, 40): -inf, (0, 9): inf})
+        put(b, at[1], -20.0, {(0, 5): -inf, (0, 9): inf})
+        put(b, at[2], 0.0 if later else -110.0, {(1, 7): nan, (0, 9): -inf, (0, 11): inf})
+        put(b, at[3], 110.0 if later else 1.0, {})
+        if m > 1:
+            put(b, n - m // 2, -110.0, {(0, 21): inf, (1, 21): -inf})  # half of the rows see this one (all, without the causal mask)
+    if "in parts" in name or name == "parts":
+        assert ctx.lib.asrfe_paged_attention_workspace_bytes(ctx.handle, c._ref, s.n, 4, len(lens), s.table.shape[1] * 32) > 0
+    out = c.attend(q, *s.plan(), **kw)
+    for b in some:
+        part = Setup.__new__(Setup)
+        part.__dict__.update(s.__dict__)
+        part.kv, part.table, part.cu = s.kv[b:b + 1], s.table[b:b + 1], np.array([0, s.nq[b]])
+        a = int(s.cu[b])
+        check_attend(part, q[a:a + int(s.nq[b])], out[a:a + int(s.nq[b])], **kw)
+
+
 @pytest.mark.parametrize("store", [None, E4M3], ids=["16", "e4m3"])
 @pytest.mark.parametrize("lens", [[(4003, 1)], [(4003, 25), (900, 3)], [(2100, 100)] * 60], ids=["token", "chunk", "tiles of 128"])
 @pytest.mark.parametrize("nats", [9, 13, 16, 18, 21])

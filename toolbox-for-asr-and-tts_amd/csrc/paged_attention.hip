@@ -15,8 +15,10 @@
 //   two).  A tile is made of 16-position pieces, each inside one page, so pages may end anywhere in a tile.
 //
 //   Masks.  Only the tiles a mask's edge crosses (the causal diagonal, either end of the window, the end of the sequence,
-//   a page that does not exist) look at positions; there, too, hidden values that are infinite or NaN are kept out of the
-//   product (0 * inf).  Tiles no row of the workgroup sees are not loaded: a window's walk skips from the sinks to it.
+//   a page that does not exist) look at positions; there, too, values that are infinite or NaN are kept out of the product
+//   (0 * inf) and added to the rows that see them.  Other tiles multiply them as they are; where a weight that became zero made
+//   NaN of one, the tiles are gone through again, all of them as edge tiles.  Tiles no row of the workgroup sees are not
+//   loaded: a window's walk skips from the sinks to it.
 //
 //   Long caches with few rows are cut along the keys into parts, whose sums a second kernel joins.
 //
@@ -65,6 +67,10 @@ struct Raised {
     static constexpr float kLag = F16 ? 6.0f : 8.0f, kRaise = F16 ? 9.0f : 0.0f;
 };
 
+// What brings sums from one reference to another.  Never zero: an infinite sum stays infinite (and 2^-126 of a finite one is
+// less than any rounding leaves).
+__device__ __forceinline__ float factor(float from, float to) { return fmaxf(__builtin_amdgcn_exp2f(from - to), 0x1p-126f); }
+
 // 1 / a sum of weights; 0 where there were none, NaN where a score was
 __device__ __forceinline__ float inverse(float sum) { return sum > 0.0f ? 1.0f / sum : (sum == 0.0f ? 0.0f : sum); }
 
@@ -86,9 +92,9 @@ __device__ __forceinline__ uint32_t large_scales(uint32_t x) { return x & 0x8080
 // Infinities and NaN among pairs of 16-bit elements.  An element whose exponent field is all ones carries into its sign bit
 // when one is added below the field.
 //
-// A product meets them where a weight of zero (a hidden key) would make NaN of them: there the finite part is multiplied as
-// usual, and for each kind of the others a product of indicators tells which (channel, row) pairs meet one under a weight
-// that is not zero.
+// A product meets them where a weight of zero (a hidden key, or one far below the row's largest) would make NaN of them: there
+// the finite part is multiplied as usual, and for each kind of the others a product of indicators tells which (channel, row)
+// pairs meet one under a score that is not -inf.
 template <bool F16>
 struct OddValues {
     static constexpr uint32_t kExp = (F16 ? 0x7c00u : 0x7f80u) * 0x10001u, kUnit = (F16 ? 0x0400u : 0x0080u) * 0x10001u;
@@ -103,7 +109,12 @@ struct OddValues {
         const u32x4 o = odd(w), nan = ((w & kMant) + kRest) & o;
         return ((t == 0 ? (o & ~nan & ~w) : t == 1 ? (o & ~nan & w) : nan) >> 15) * kOne;
     }
-    __device__ static u32x4 nonzero(const u32x4 w) { return ((((w & kRest) + kRest) & kSign) >> 15) * kOne; }
+    __device__ static u32x4 ones(uint32_t bits) {  // in the places of the set ones of eight bits
+        u32x4 r;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) r[i] = ((bits >> (2 * i) & 1) | (bits >> (2 * i + 1) & 1) << 16) * kOne;
+        return r;
+    }
     __device__ static float value(int t) { return t == 0 ? INFINITY : t == 1 ? -INFINITY : __builtin_nanf(""); }
 };
 
@@ -281,7 +292,8 @@ __global__ __launch_bounds__(256, (D == 64 && !E4M3 ? 3 : 2)) void paged_attn_ma
     constexpr uint32_t kAll = (1u << S::kPieces) - 1;
     using O = OddValues<F16>;
     __shared__ __attribute__((aligned(1024))) char smem[4 * kTile];
-    __shared__ int odd_tile;  // the last edge tile in whose V an infinity or NaN was found
+    __shared__ int odd_tile;   // the last edge tile in whose V an infinity or NaN was found
+    __shared__ int once_more;  // whether the tiles are to be gone through again
     // (no saturate_fp16_conversions here: in that mode the matrix instructions lose infinities and NaN in their accumulators)
     const PagedAttnParams& p = job.p;
     const int tid = threadIdx.x, lane = tid & 63, l31 = lane & 31, h = lane >> 5;
@@ -391,12 +403,14 @@ __global__ __launch_bounds__(256, (D == 64 && !E4M3 ? 3 : 2)) void paged_attn_ma
 
     // ---- first tile, queries
     uint32_t valid = 0;  // of the tile that is about to be used: which of its pieces exist
-    if (vt0 < vt1) {
+    auto first_tile_of_walk = [&]() __attribute__((always_inline)) {
+        if (vt0 >= vt1) return;
         const Pieces<S::kPieces> pc = pages.tile<S::kPieces>(key0_of(vt0));
         valid = pc.valid;
         if constexpr (E4M3) issue8(pc);
         else issue16(pc, 0);
-    }
+    };
+    first_tile_of_walk();
     const float c = fmaxf(__builtin_fabsf(p.scale_log2), 1e-37f);  // (a scale of zero weighs all positions the same)
     u16x8 qf[D / 16];
     {
@@ -416,11 +430,21 @@ __global__ __launch_bounds__(256, (D == 64 && !E4M3 ? 3 : 2)) void paged_attn_ma
     }
 
     f32x16 oacc[kMt];
+    float mc, l_run;  // reference (see Raised) and sum of this lane's half of the keys
+    int buf, vt;
+    auto begin = [&]() __attribute__((always_inline)) {
 #pragma unroll
-    for (int mt = 0; mt < kMt; ++mt)
+        for (int mt = 0; mt < kMt; ++mt)
 #pragma unroll
-        for (int e = 0; e < 16; ++e) oacc[mt][e] = 0.0f;
-    float mc = -INFINITY, l_run = 0.0f;  // reference (see Raised) and sum of this lane's half of the keys
+            for (int e = 0; e < 16; ++e) oacc[mt][e] = 0.0f;
+        mc = -INFINITY;
+        l_run = 0.0f;
+        buf = 0;
+        vt = vt0;
+        if (tid == 0) odd_tile = -1;  // (every use of it lies behind a barrier)
+    };
+    begin();
+    if (tid == 0) once_more = 0;
 
     auto compute = [&](uint32_t tile_base, int key0, uint32_t exist, bool special, auto edge_c) __attribute__((always_inline)) {
         constexpr bool edge = decltype(edge_c)::value;
@@ -465,12 +489,17 @@ __global__ __launch_bounds__(256, (D == 64 && !E4M3 ? 3 : 2)) void paged_attn_ma
             vf[T % kRing] = v_frag(T / (2 * kMt), (T / kMt) & 1, T % kMt);
         };
         if constexpr (!edge) static_for<kRing>([&](auto tc) { v_step(tc); });
+        uint32_t seen = 0;  // of this lane's 32 scores, where that is asked for
         if constexpr (edge) {
             const RowMask mask{lo, hi, p.sinks};
 #pragma unroll
             for (int kk = 0; kk < 2; ++kk)
                 mask.hide<16>(key0, exist, kAll, [&](int r) { return kk * 32 + 8 * r + 4 * h; }, [&](int r) { return 2 * kk + (r >> 1); },
                               [&](int e) -> float& { return reinterpret_cast<float*>(&sacc[kk])[e]; });
+            if (special) {
+#pragma unroll
+                for (int e = 0; e < 32; ++e) seen |= sacc[e / 16][e % 16] == -INFINITY ? 0u : 1u << e;
+            }
         }
         float rmax = sacc[0][0];
 #pragma unroll
@@ -482,10 +511,10 @@ __global__ __launch_bounds__(256, (D == 64 && !E4M3 ? 3 : 2)) void paged_attn_ma
             rmax = fmaxf(__uint_as_float(sw[0]), __uint_as_float(sw[1]));
         }
         // the maximum only has to keep the weights in range
-        const float seen = fmaf(rmax, c, -Raised<F16>::kRaise);
-        const bool grew = seen > mc + Raised<F16>::kLag;
-        const float m_new = grew ? seen : mc;
-        const float alpha = grew ? __builtin_amdgcn_exp2f(mc - m_new) : 1.0f;
+        const float most = fmaf(rmax, c, -Raised<F16>::kRaise);
+        const bool grew = most > mc + Raised<F16>::kLag;
+        const float m_new = grew ? most : mc;
+        const float alpha = grew ? factor(mc, m_new) : 1.0f;
         mc = m_new;
         const float sub = mc == -INFINITY ? 0.0f : mc;  // (nothing seen yet: every weight below is exp2(-inf))
         if (__any(grew)) {
@@ -547,7 +576,7 @@ __global__ __launch_bounds__(256, (D == 64 && !E4M3 ? 3 : 2)) void paged_attn_ma
                             f32x16 hit;
 #pragma unroll
                             for (int e = 0; e < 16; ++e) hit[e] = 0.0f;
-                            hit = times(O::kind(v, t), O::nonzero(pf[kk][s2]), hit);
+                            hit = times(O::kind(v, t), O::ones(seen >> (16 * kk + 8 * s2)), hit);
 #pragma unroll
                             for (int e = 0; e < 16; ++e) oacc[mt][e] += hit[e] > 0.0f ? O::value(t) : 0.0f;
                             __builtin_amdgcn_sched_barrier(0);
@@ -557,13 +586,12 @@ __global__ __launch_bounds__(256, (D == 64 && !E4M3 ? 3 : 2)) void paged_attn_ma
     };
 
     // Tiles [inner0, inner1) lie inside every row's mask.  They run in a loop of their own: with both kinds in one loop the
-    // accumulators would be copied between them, 64 registers a tile.
+    // accumulators would be copied between them, 64 registers a tile.  (The way back, for infinities, costs heads of 64 some 1 %
+    // even if none takes it; a second copy of the edge loop instead of it costs 8-bit caches 11 %.)
     const int first_row = ts.row0 / p.group, last_row = (ts.row0 + S::kRowTile - 1 < ts.n_rows ? ts.row0 + S::kRowTile - 1 : ts.n_rows - 1) / p.group;
     const int all_lo = lo_of(ts.pos0 + last_row), from = (all_lo + kKeys - 1) / kKeys - ts.first;
     const int inner0 = ts.sink_tiles + (from > 0 ? from : 0), to = ts.sink_tiles + hi_of(ts.pos0 + first_row) / kKeys - ts.first;
-    const int inner1 = to < vt1 ? to : vt1;
-    int buf = 0, vt = vt0;
-    if (tid == 0) odd_tile = -1;  // (every use of it lies behind a barrier)
+    int inner1 = to < vt1 ? to : vt1;
     auto turn = [&](auto edge_c) __attribute__((always_inline)) {
         constexpr bool edge = decltype(edge_c)::value;
         if constexpr (E4M3) put8(lds0 + buf * 2 * kTile);
@@ -592,13 +620,30 @@ __global__ __launch_bounds__(256, (D == 64 && !E4M3 ? 3 : 2)) void paged_attn_ma
         buf ^= 1;
         ++vt;
     };
-    while (vt < vt1) {
-        if (vt >= inner0 && vt < inner1 && valid == kAll) {
-            do turn(std::false_type{});
-            while (vt < inner1 && valid == kAll);
-        } else {
-            turn(std::true_type{});
+    for (;;) {
+        bool plain = false;  // an inner tile was met
+        while (vt < vt1) {
+            if (vt >= inner0 && vt < inner1 && valid == kAll) {
+                plain = true;
+                do turn(std::false_type{});
+                while (vt < inner1 && valid == kAll);
+            } else {
+                turn(std::true_type{});
+            }
         }
+        if (!plain) break;
+        // a sum that is NaN though no score was: an infinity may have met a weight of zero in an inner tile
+        bool nan = false;
+#pragma unroll
+        for (int mt = 0; mt < kMt; ++mt)
+#pragma unroll
+            for (int e = 0; e < 16; e += 2) nan |= __builtin_isunordered(oacc[mt][e], oacc[mt][e + 1]);
+        if (__any(nan && l_run == l_run)) once_more = 1;
+        __syncthreads();
+        if (__builtin_amdgcn_readfirstlane(once_more) == 0) break;
+        inner1 = vt0;  // none is
+        begin();
+        first_tile_of_walk();
     }
 
     // ---- results: lane (l31, h) holds of its row the channels 32 mt + 8 (e >> 2) + 4 h + (e & 3)
@@ -606,7 +651,9 @@ __global__ __launch_bounds__(256, (D == 64 && !E4M3 ? 3 : 2)) void paged_attn_ma
     const float l_tot = l_run + __shfl_xor(l_run, 32);
     const float inv = inverse(l_tot);
     const int64_t part_row = ((static_cast<int64_t>(kvh) * job.n_tiles + tile) * job.n_split + part) * S::kRowTile + wave * 32 + l31;
-    uint16_t* out = p.out + (ts.tok0 + tok) * p.o_ts + hq * p.o_hs + 4 * h;
+    int t = ts.tok0 + tok, head = hq;
+    asm volatile("" : "+v"(t), "+v"(head));  // (addresses are formed here: not kept through the loop)
+    uint16_t* out = p.out + t * p.o_ts + head * p.o_hs + 4 * h;
     float* po = job.part_o + part_row * D + 4 * h;
 #pragma unroll
     for (int mt = 0; mt < kMt; ++mt)
@@ -683,7 +730,8 @@ __global__ __launch_bounds__(64 * KW, (NQ == 1 ? 2 : 1)) void paged_attn_few_ker
     const int pmin = __builtin_amdgcn_readfirstlane(ts.pos0 + ts.row0 / p.group), pmax = __builtin_amdgcn_readfirstlane(ts.pos0 + last / p.group);
     auto hi_of = [&](int i) { return i < 0 ? 0 : (p.causal && i + 1 < ts.len ? i + 1 : ts.len); };
     auto lo_of = [&](int i) { return p.window > 0 && i - p.window + 1 > 0 ? i - p.window + 1 : 0; };
-    const int w_hi_min = hi_of(pmin), w_lo_max = lo_of(pmax);
+    int w_hi_min = hi_of(pmin);
+    const int w_lo_max = lo_of(pmax);
     int hi[NQ], lo[NQ];
     int64_t out_at[NQ];
     u32x4 qf[NQ][D / 32];
@@ -761,13 +809,6 @@ __global__ __launch_bounds__(64 * KW, (NQ == 1 ? 2 : 1)) void paged_attn_few_ker
 
     f32x4 oacc[NQ][kMb];
     float mc[NQ], l_run[NQ];
-#pragma unroll
-    for (int n = 0; n < NQ; ++n) {
-        mc[n] = -INFINITY;
-        l_run[n] = 0.0f;
-#pragma unroll
-        for (int m = 0; m < kMb; ++m) oacc[n][m] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-    }
 
     auto compute = [&](const Keys& k, uint32_t tile_base, int key0, uint32_t valid, auto edge_c) __attribute__((always_inline)) {
         constexpr bool edge = decltype(edge_c)::value;
@@ -806,10 +847,10 @@ __global__ __launch_bounds__(64 * KW, (NQ == 1 ? 2 : 1)) void paged_attn_few_ker
                 for (int i = 0; i < 4; ++i) rmax = fmaxf(rmax, sacc[n][u][i]);
             rmax = max_of_row(rmax);
             // the maximum only has to keep the weights in range
-            const float seen = fmaf(rmax, c, -Raised<F16>::kRaise);
-            const bool grew = seen > mc[n] + Raised<F16>::kLag;
-            const float m_new = grew ? seen : mc[n];
-            const float alpha = grew ? __builtin_amdgcn_exp2f(mc[n] - m_new) : 1.0f;
+            const float most = fmaf(rmax, c, -Raised<F16>::kRaise);
+            const bool grew = most > mc[n] + Raised<F16>::kLag;
+            const float m_new = grew ? most : mc[n];
+            const float alpha = grew ? factor(mc[n], m_new) : 1.0f;
             mc[n] = m_new;
             const float sub = m_new == -INFINITY ? 0.0f : m_new;  // (nothing seen yet: every weight below is exp2(-inf))
             if (__any(grew)) {
@@ -852,6 +893,13 @@ __global__ __launch_bounds__(64 * KW, (NQ == 1 ? 2 : 1)) void paged_attn_few_ker
                 for (int n = 0; n < NQ; ++n) oacc[n][m] = mfma16<F16>(v, pf[n], oacc[n][m]);
             }
         } else {
+            uint32_t seen[NQ];  // of this lane's eight scores of a row
+#pragma unroll
+            for (int n = 0; n < NQ; ++n) {
+                seen[n] = 0;
+#pragma unroll
+                for (int e = 0; e < 8; ++e) seen[n] |= sacc[n][e >> 2][e & 3] == -INFINITY ? 0u : 1u << e;
+            }
 #pragma unroll
             for (int m = 0; m < kMb; ++m) {
                 const u32x4 v = v_frag(m);
@@ -860,7 +908,7 @@ __global__ __launch_bounds__(64 * KW, (NQ == 1 ? 2 : 1)) void paged_attn_few_ker
                     oacc[n][m] = mfma16<F16>(O::finite(v), pf[n], oacc[n][m]);
 #pragma unroll
                     for (int t = 0; t < 3; ++t) {
-                        const f32x4 hit = mfma16<F16>(O::kind(v, t), O::nonzero(pf[n]), f32x4{0.0f, 0.0f, 0.0f, 0.0f});
+                        const f32x4 hit = mfma16<F16>(O::kind(v, t), O::ones(seen[n]), f32x4{0.0f, 0.0f, 0.0f, 0.0f});
 #pragma unroll
                         for (int i = 0; i < 4; ++i) oacc[n][m][i] += hit[i] > 0.0f ? O::value(t) : 0.0f;
                         __builtin_amdgcn_sched_barrier(0);
@@ -870,14 +918,25 @@ __global__ __launch_bounds__(64 * KW, (NQ == 1 ? 2 : 1)) void paged_attn_few_ker
         }
     };
 
-    int vt = vt0 + wave;
+    int vt;
     uint32_t valid = 0;  // of the tile that is about to be used: which of its pieces exist
+    bool plain = false;  // an inner tile was met
     Keys ka, kb;
-    if (vt < vt1) {
-        const Pieces<2> pc = pages.tile<2>(key0_of(vt));
-        valid = pc.valid;
-        issue(pc, ka, 0);
-    }
+    auto begin = [&]() __attribute__((always_inline)) {
+#pragma unroll
+        for (int n = 0; n < NQ; ++n) {
+            mc[n] = -INFINITY;
+            l_run[n] = 0.0f;
+#pragma unroll
+            for (int m = 0; m < kMb; ++m) oacc[n][m] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+        }
+        vt = vt0 + wave;
+        if (vt < vt1) {
+            const Pieces<2> pc = pages.tile<2>(key0_of(vt));
+            valid = pc.valid;
+            issue(pc, ka, 0);
+        }
+    };
     auto turn = [&](Keys& now_k, Keys& next_k, int buf) __attribute__((always_inline)) {
         // everything of this tile is in, and the reads of the tile before are done with the other buffer
         __builtin_amdgcn_s_waitcnt(0x0070);  // vmcnt(0) lgkmcnt(0)
@@ -905,14 +964,33 @@ __global__ __launch_bounds__(64 * KW, (NQ == 1 ? 2 : 1)) void paged_attn_few_ker
             issue(pc, next_k, E4M3 ? 0 : buf ^ 1);
         }
         const uint32_t base = own_base + (E4M3 ? 0 : buf * kTile);
-        if (key0 + kKeys <= w_hi_min && (key0 >= w_lo_max || key0 + kKeys <= p.sinks) && now == 3) compute(now_k, base, key0, now, std::false_type{});
-        else compute(now_k, base, key0, now, std::true_type{});
+        if (key0 + kKeys <= w_hi_min && (key0 >= w_lo_max || key0 + kKeys <= p.sinks) && now == 3) {
+            plain = true;
+            compute(now_k, base, key0, now, std::false_type{});
+        } else {
+            compute(now_k, base, key0, now, std::true_type{});
+        }
         vt = next;
     };
-    while (vt < vt1) {
-        turn(ka, kb, 0);
-        if (vt >= vt1) break;
-        turn(kb, ka, 1);
+    begin();
+    for (;;) {
+        while (vt < vt1) {
+            turn(ka, kb, 0);
+            if (vt >= vt1) break;
+            turn(kb, ka, 1);
+        }
+        if (!plain) break;
+        // a sum that is NaN though no score was: an infinity may have met a weight of zero in an inner tile
+        bool nan = false;
+#pragma unroll
+        for (int n = 0; n < NQ; ++n)
+#pragma unroll
+            for (int m = 0; m < kMb; ++m)
+                nan |= (__builtin_isunordered(oacc[n][m][0], oacc[n][m][1]) | __builtin_isunordered(oacc[n][m][2], oacc[n][m][3])) & (l_run[n] == l_run[n]);
+        if (!__any(nan)) break;
+        w_hi_min = -1;  // none is
+        plain = false;
+        begin();
     }
 
     // ---- results: lane (col, g) holds of row col the channels 16 m + 4 g .. + 3
@@ -956,7 +1034,7 @@ __global__ __launch_bounds__(64 * KW, (NQ == 1 ? 2 : 1)) void paged_attn_few_ker
             const float sub = top == -INFINITY ? 0.0f : top;
 #pragma unroll
             for (int i = 0; i < KW; ++i) sum += ml[(i * NQ + n) * 32 + 16 + col] * __builtin_amdgcn_exp2f(ml[(i * NQ + n) * 32 + col] - sub);
-            const float f = __builtin_amdgcn_exp2f(mc[n] - sub);
+            const float f = factor(mc[n], sub);
 #pragma unroll
             for (int m = 0; m < kMb; ++m)
                 *reinterpret_cast<float4*>(os + (((wave * NQ + n) * kMb + m) * 64 + lane) * 4) = make_float4(oacc[n][m][0] * f, oacc[n][m][1] * f, oacc[n][m][2] * f, oacc[n][m][3] * f);
@@ -1035,7 +1113,7 @@ __global__ __launch_bounds__(256) void paged_join_few_kernel(const AttnJob job) 
     float top = ml.x;
 #pragma unroll
     for (int o = kFewParts / 2; o >= 1; o >>= 1) top = fmaxf(top, __shfl_xor(top, o));
-    const float f = __builtin_amdgcn_exp2f(ml.x - (top == -INFINITY ? 0.0f : top));
+    const float f = factor(ml.x, top == -INFINITY ? 0.0f : top);
     float sum = ml.y * f;
 #pragma unroll
     for (int o = kFewParts / 2; o >= 1; o >>= 1) sum += __shfl_xor(sum, o);
@@ -1082,7 +1160,7 @@ __global__ __launch_bounds__(256) void paged_join_kernel(const AttnJob job) {
     if ((tid & 63) == 0) red[tid >> 6] = top;
     __syncthreads();
     top = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
-    const float f = __builtin_amdgcn_exp2f(ml.x - (top == -INFINITY ? 0.0f : top));
+    const float f = factor(ml.x, top == -INFINITY ? 0.0f : top);
     weight[tid] = f;
     float sum = ml.y * f;
 #pragma unroll
