@@ -304,7 +304,7 @@ int32_t asrfe_frame_decibel(asrfe_ctx* ctx, const void* pcm, int32_t pcm_dtype, 
 typedef struct asrfe_kv_cache {
     void* k;                 /* [n_pages][n_heads][page_size][head_dim], 16-byte aligned; dtype F16, BF16 or E4M3 */
     void* v;                 /* the same for the values */
-    uint8_t* k_exp;          /* E4M3: [n_pages][n_heads][page_size], 16-byte aligned, a stored value is code * 2^(exp - 127); else NULL */
+    uint8_t* k_exp;          /* E4M3: [n_pages][n_heads][page_size], 16-byte aligned, a stored value is code * 2^(exp - 127), exp 0 .. 254; else NULL */
     uint8_t* v_exp;
     int32_t n_pages;
     int32_t page_size;       /* 16, 32, 64, 128 or 256 positions */
@@ -327,14 +327,15 @@ int32_t asrfe_kv_append(asrfe_ctx* ctx, const asrfe_kv_cache* cache, const void*
 
 /* Reads positions 0 .. t_max - 1 of every sequence back: k, v [batch][t_max][n_heads][head_dim] dense, of `dtype` (as in
  * asrfe_kv_append; 16-byte aligned; batch * t_max below 2^26).  Positions at and past kv_lens[b], and those of pages that do not exist, are zero.
- * Every e4m3 code under its scale is exact in bf16 and, inside its range, in fp16 (beyond it: +-65504). */
+ * A stored e4m3 value is what BF16 and F16 have of it: exact in BF16 (subnormal values may be flushed to zero), in F16
+ * rounded to nearest below 2^-14 and +-65504 beyond that. */
 int32_t asrfe_kv_read(asrfe_ctx* ctx, const asrfe_kv_cache* cache, const int32_t* kv_lens, const int32_t* block_table,
                       int32_t table_stride, int32_t batch, int32_t t_max, void* k, void* v, int32_t dtype, void* stream);
 
 /* Attention of the new rows over the cache: out[t][h] = sum_j p_j v_j, p = softmax_j(scale * q[t][h] . k_j) over the
  * positions j the row sees, h's keys being those of cache head h / (n_q_heads / n_heads).  A row at position i sees j <
  * kv_lens[b] with j <= i (causal != 0), and, where window > 0, j > i - window or j < sinks.  A row that sees nothing is
- * zero.  What a row does not see has no influence on it, infinities and NaN in hidden keys or values included; a value
+ * zero.  Keys and values of an E4M3 cache enter in `dtype`, as asrfe_kv_read gives them.  What a row does not see has no influence on it, infinities and NaN in hidden keys or values included; a value
  * that it sees counts, infinite or NaN, however small its weight (unless its score is -inf).  The caller's new positions have to be in the cache
  * already (asrfe_kv_append on the same stream).  q, out: elements (t, h, d) at t * token_stride + h * head_stride + d,
  * strides multiples of 8 (out's rows must not overlap), bases 16-byte aligned, of `dtype` (F16 or BF16; the cache's own for a 16-bit cache).

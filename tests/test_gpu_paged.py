@@ -311,6 +311,74 @@ def test_small_weights_beside_a_sink(pkg, ctx, nats, lens, store):
         assert (err <= tol).all(), (t, n, float((err / tol).max()), float(want.max()))
 
 
+IN_TILES = {"16": ([(37, 1)] * 150, 2, 1), "32": ([(60, 30), (45, 28)] * 6, 2, 1), "128": ([(330, 200)] * 80, 2, 2)}
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("rows", IN_TILES)
+def test_every_scale_of_values_in_attention(pkg, ctx, rows, dim, dtype):
+    """A window of one position gives the position's value with a weight of one, that is, the stored number in the product's
+    type: every scale 0 .. 254 and every code, rounded to nearest and, in fp16, kept inside its range."""
+    lens, heads, group = IN_TILES[rows]
+    assert rows != "128" or repeats(lens, heads, group, True, 256, 1) == 1
+    s = Setup(pkg, ctx, lens, dtype, E4M3, dim, heads, 16, seed=dim)
+    c = s.cache
+    codes = torch.randint(0, 254, c.v.shape, generator=s.g, device="cuda")
+    c.v.view(torch.uint8).copy_(codes + (codes >= 127))  # (all but the NaN)
+    c.v_exp.copy_(torch.randint(0, 255, c.v_exp.shape, generator=s.g, device="cuda"))
+    out = c.attend(s.rows(s.n, heads * group), *s.plan(), window=1).cpu()
+    v = values_of(c, "v")
+    for b in {0, 1, len(lens) // 2, len(lens) - 1}:
+        n, m = lens[b]
+        got = out[int(s.cu[b]):int(s.cu[b + 1])]
+        want = torch.from_numpy(np.repeat(po.dense(v, s.table, 16, b, n)[0][n - m:], group, axis=1))
+        fine = (want.abs() >= 2.0 ** -126) | (want == 0)  # (what is subnormal in fp32 and bf16 may be flushed)
+        fine &= want.abs() < 3e38
+        want = (want.clamp(-65504, 65504) if dtype == F16 else want).to(dtype)
+        assert torch.equal(got[fine], want[fine])
+
+
+SCALES = {
+    # name: exponents of keys, of values, size of the queries
+    "at the border": ((134, 135), (134, 135), 1e-4),
+    "large": ((133, 134, 135, 136, 140, 143), (133, 135, 137, 143), 1e-4),
+    "large keys": ((134, 135, 138), (119, 120), 1e-4),
+    "a few large keys": ((119,) * 40 + (135, 139), (119, 120), 1e-3),
+    "large values": ((118, 119), (134, 135, 139), 1.0),
+    "a few large values": ((118, 119), (119,) * 40 + (135, 141), 1.0),
+    "small": ((100, 104, 108, 111), (100, 103, 106, 110), 60.0),
+    "all sizes": ((100, 110, 120, 128, 134, 135, 137), (100, 110, 120, 128, 134, 135, 137), 1e-4),
+}
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("rows", IN_TILES)
+@pytest.mark.parametrize("name", SCALES)
+def test_attend_scales_of_all_sizes(pkg, ctx, name, rows, dim, dtype):
+    """Keys and values take part as what they are in the product's type: exact in bf16, in fp16 rounded to nearest where they are
+    below 2^-14 and kept inside +-65504."""
+    lens, heads, group = IN_TILES[rows]
+    s = Setup(pkg, ctx, lens, dtype, E4M3, dim, heads, 16, seed=len(name))
+    c = s.cache
+    for t, exps in ((c.k_exp, SCALES[name][0]), (c.v_exp, SCALES[name][1])):
+        t.copy_(torch.tensor(exps, device="cuda")[torch.randint(len(exps), t.shape, generator=s.g, device="cuda")])
+    q = s.rows(s.n, heads * group, SCALES[name][2])
+    for kw in ({}, dict(window=20, sinks=3)):
+        out = c.attend(q, *s.plan(), **kw)
+        k, v = (torch.from_numpy(values_of(c, x)) for x in "kv")
+        if dtype == F16:
+            k, v = (t.clamp(-65504, 65504).to(F16).double() for t in (k, v))
+        k, v, vmax = k.numpy(), v.numpy(), float(v.abs().max())
+        for b in {0, len(lens) - 1}:
+            a0, a1, n = int(s.cu[b]), int(s.cu[b + 1]), int(s.kv[b])
+            want, absv, reach, _ = po.attend(q[a0:a1].double().cpu().numpy(), k, v, [0, a1 - a0], [n], s.table[b:b + 1], 16, **kw)
+            tol = bound(dtype, dim, n, want, absv, reach, 0.0) + (n * vmax * 2.0 ** -34 if dtype == F16 else 0.0)
+            err = np.abs(out[a0:a1].double().cpu().numpy() - want)
+            assert (err <= tol).all(), (b, float((err / tol).max()), float(err.max()), float(np.abs(want).max()))
+
+
 def test_attend_pages_that_do_not_exist(pkg, ctx):
     """-1 and numbers past the pool are pages that were given back; a length past the table's width has no pages there."""
     s = Setup(pkg, ctx, [(300, 1), (200, 40), (170, 3), (64, 2)], BF16, None, 64, 2, 16, seed=3)

@@ -11,8 +11,8 @@
 //   Keys.  One pass with a running maximum and sum.  Scores are formed transposed, S^T = K Q^T (v_mfma_f32_32x32x16), so a
 //   lane holds the scores of one row; the weights are then already laid out as the operand of O^T = V^T P^T, V being read
 //   transposed from the LDS.  Tiles arrive by 16-byte global -> LDS loads (16-bit caches) with the bank swizzle applied to
-//   the source address, or through registers, where e4m3 codes become 16-bit values (exactly: the scales are powers of
-//   two).  A tile is made of 16-position pieces, each inside one page, so pages may end anywhere in a tile.
+//   the source address, or through registers, where e4m3 codes become 16-bit values (their scales are powers of two: exact
+//   but for fp16 below 2^-14 and past 65504, see dequantise8).  A tile is made of 16-position pieces, each inside one page, so pages may end anywhere in a tile.
 //
 //   Masks.  Only the tiles a mask's edge crosses (the causal diagonal, either end of the window, the end of the sequence,
 //   a page that does not exist) look at positions; there, too, values that are infinite or NaN are kept out of the product

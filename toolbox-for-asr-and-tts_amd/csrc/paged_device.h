@@ -65,7 +65,8 @@ __device__ __forceinline__ int64_t cache_row(const PagedView& c, int page, int h
     return ((static_cast<int64_t>(page) * c.n_heads + head) << c.page_shift) + (pos & ((1 << c.page_shift) - 1));
 }
 
-// Eight e4m3 codes (two dwords) times 2^(exp - 127), rounded to the 16-bit type: exact wherever the type has the value.
+// Eight e4m3 codes (two dwords) times 2^(exp - 127), rounded to the 16-bit type: exact wherever the type has the value, which
+// bf16 has and fp16 from 2^-24 times the code's last place on, up to 65504.
 // LARGE: the scale may lead out of fp16's range; what does becomes its largest value.
 template <bool F16, bool LARGE>
 __device__ __forceinline__ u32x4 dequantise8(uint32_t c0, uint32_t c1, uint32_t exp) {

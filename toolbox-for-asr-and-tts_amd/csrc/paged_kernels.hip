@@ -9,7 +9,7 @@
 //   e4m3: the largest finite magnitude of a row is found across its lanes, e = the least integer >= -126 with
 //   max <= 448 * 2^e comes from its exponent and mantissa fields (448 = 1.75 * 2^8: a mantissa above 1.75 needs one more),
 //   and the codes are the conversion instruction's round-to-nearest-even of x * 2^-e.  With a power of two as the scale
-//   the multiplication rounds nothing, and reading back is exact in both 16-bit types.
+//   the multiplication rounds nothing, and reading a row back in the type it came in rounds nothing more (in fp16, what became 65536 is 65504).
 //
 //   Eight heads of 128: 8 prompts of up to 4096 tokens into an e4m3 cache 30 us (5.0 TB/s), 16 sequences of up to 8192
 //   positions out of one 145 us (5.1 TB/s, what a copy reaches).  Eight single tokens 4.0 us: a launch and the chain from

@@ -7,6 +7,8 @@ cache of its own.  ``PagedKvCache`` is what a streaming or autoregressive model 
 e4m3 bytes with a power-of-two scale per position and head.  One step is ``append`` (the new positions' keys and values go
 into their pages) and ``attend`` (the new queries attend to everything their sequence holds); ``read`` gives dense copies
 back.  Everything runs on the device through libasrfe; there is no CPU path.
+An e4m3 value takes part as what the queries' type has of it: exactly in bfloat16, in float16 rounded below 2 ** -14 and kept
+inside +-65504.
 
 A batch is described by three int32 device tensors: ``cu_q`` [B + 1] (rows of the packed new tokens), ``kv_lens`` [B] (positions
 of every sequence, the new ones included: they are its last) and ``block_table`` [B, n] (page numbers; -1 where there is no
@@ -39,7 +41,7 @@ class PagedKvCache:
     def __init__(self, ctx: _lib.Context, k: torch.Tensor, v: torch.Tensor, k_exp: torch.Tensor | None = None,
                  v_exp: torch.Tensor | None = None):
         """k, v [n_pages, n_heads, page_size, head_dim] of float16, bfloat16 or float8_e4m3fn; for float8_e4m3fn also k_exp,
-        v_exp [n_pages, n_heads, page_size] uint8 (a stored value is code * 2 ** (exp - 127)).  The buffers stay the
+        v_exp [n_pages, n_heads, page_size] uint8 (a stored value is code * 2 ** (exp - 127), exp 0 .. 254).  The buffers stay the
         caller's; see ``allocate`` for new ones."""
         e4m3 = k.dtype == torch.float8_e4m3fn
         if k.dim() != 4 or k.shape != v.shape or k.dtype != v.dtype or not (e4m3 or k.dtype in _DT):
