@@ -1,6 +1,7 @@
 """CPU tests of the paged cache, its attention and the choice of a token: refusals of both layers before anything touches a
 device, and the oracle against independent statements (torch's own e4m3 conversion, its softmax, known answers)."""
 import ctypes as C
+import glob
 import os
 import re
 import subprocess
@@ -156,6 +157,18 @@ def test_sample_refuses(abi, kw, code):
 @pytest.mark.parametrize("rc", [lambda a: a.read(batch=1 << 10, t_max=1 << 16), lambda a: a.read(batch=1, t_max=1 << 26), lambda a: a.sample(rows=(1 << 23) + 1)])
 def test_more_threads_than_a_launch_holds_are_refused(abi, rc):
     assert rc(abi) == SHAPE
+
+
+def test_documents_fill_the_cache_structure_in_its_order(pkg):
+    """The examples that build it from its fields one after the other, evaluated."""
+    names = [n for n, _ in pkg._lib.KvCache._fields_]
+    given = dict(zip(names, (64, 128, 192, 256, 7, 16, 3, 128, pkg._lib.DT_E4M3)))
+    scope = dict(given, **{n: getattr(pkg._lib, "DT_E4M3") for n in ("DT_E4M3", "ASRFE_DT_E4M3")}, KvCache=pkg._lib.KvCache)
+    calls = [m for path in glob.glob(os.path.join(ROOT, "*.md")) for m in re.findall(r"(?<![A-Za-z])KvCache\([^()]*\)", open(path).read())]
+    assert calls
+    for call in calls:
+        built = eval(call, {}, scope)
+        assert {n: getattr(built, n) for n in names} == given, call
 
 
 # ---- the Python layer ---------------------------------------------------------------------------------------------------------
