@@ -159,6 +159,11 @@ def test_more_threads_than_a_launch_holds_are_refused(abi, rc):
     assert rc(abi) == SHAPE
 
 
+@pytest.mark.parametrize("scale", [float("inf"), float("-inf"), float("nan"), 2.4e38, -3e38])
+def test_scales_that_are_not_finite_in_base_two_are_refused(abi, scale):
+    assert abi.attend(scale=scale) == BAD and "scale" in abi.error()
+
+
 def test_documents_fill_the_cache_structure_in_its_order(pkg):
     """The examples that build it from its fields one after the other, evaluated."""
     names = [n for n, _ in pkg._lib.KvCache._fields_]

@@ -138,7 +138,8 @@ extern "C" int32_t asrfe_paged_attention(asrfe_ctx* ctx, const asrfe_kv_cache* c
     if (n_tokens < 0 || n_tokens > (1 << 24) || static_cast<int64_t>(n_tokens) * n_q_heads > (int64_t{1} << 30))
         return bad(ctx, ASRFE_ERR_SHAPE, kWho, "n_tokens in 0..2^24, n_tokens * n_q_heads up to 2^30");
     if (max_kv < 0 || window < 0 || sinks < 0) return bad(ctx, ASRFE_ERR_SHAPE, kWho, "max_kv, window and sinks must not be negative");
-    if (!std::isfinite(scale)) return bad(ctx, ASRFE_ERR_BAD_ARG, kWho, "scale must be finite");
+    const float scale_log2 = scale * 1.4426950408889634f;
+    if (!std::isfinite(scale_log2)) return bad(ctx, ASRFE_ERR_BAD_ARG, kWho, "scale must be finite, and below 2.3e38");
     if (n_tokens == 0 || batch == 0) return ASRFE_OK;
     if (!q || !out || !aligned16(q) || !aligned16(out)) return bad(ctx, ASRFE_ERR_BAD_ARG, kWho, "q and out must be 16-byte aligned");
     if (!stride_ok(q_token_stride) || !stride_ok(q_head_stride) || !stride_ok(out_token_stride) || !stride_ok(out_head_stride))
@@ -160,7 +161,7 @@ extern "C" int32_t asrfe_paged_attention(asrfe_ctx* ctx, const asrfe_kv_cache* c
     p.window = std::min(window, 1 << 30);
     p.sinks = std::min(sinks, 1 << 30);
     p.causal = causal != 0;
-    p.scale_log2 = scale * 1.4426950408889634f;
+    p.scale_log2 = scale_log2;
     return launch_paged_attention(ctx, p, cache->head_dim, dtype, cache->dtype == ASRFE_DT_E4M3, workspace, max_kv, static_cast<hipStream_t>(stream));
 }
 
