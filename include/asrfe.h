@@ -360,11 +360,12 @@ int32_t asrfe_paged_attention(asrfe_ctx* ctx, const asrfe_kv_cache* cache, const
  * the lowest index at which the running sum of the kept weights, in the order of the vocabulary, exceeds u[r] times
  * their sum (u in [0, 1)), logprobs[r] (optional) the logarithm of its share of that sum.  temperature, top_k, top_p,
  * min_p, u: one per row; each of the first four may be NULL (1, all, all, all).  A temperature that is not above zero
- * takes the first of the order (the arg-max).  NaN logits count as -inf, and a -inf logit is never chosen; where a row
+ * takes the first of the order (the arg-max), one above 1e30 counts as 1e30 (logits of up to 1e20 all weigh the same there).  NaN logits count as -inf, and a -inf logit is never chosen; where a row
  * holds +inf logits, they share all the weight.  A row with nothing above -inf gives 0 and logprob -inf.  token_num
  * [rows / rows_per] (optional; rows up to 2^23): rows r with r % rows_per >= token_num[r / rows_per] get -1 and logprob 0 (rows behind an
- * utterance's tokens, as asrfe_decoder_forward marks them).  Weights are formed and summed with errors below 1e-9 and
- * the sums do not depend on the order of execution: the same call gives the same bits. */
+ * utterance's tokens, as asrfe_decoder_forward marks them).  A weight is formed to 1e-11 of itself and rounded to a multiple
+ * of 2^-44 of the largest, so a sum of n is off by at most n 2^-45 (7.5e-9 for the largest vocabulary) and 1e-11 of itself; sums do not
+ * depend on the order of execution: the same call gives the same bits. */
 int32_t asrfe_sample_tokens(asrfe_ctx* ctx, const void* logits, int32_t dtype, int64_t ld, int32_t rows, int32_t vocab,
                             const float* u, const float* temperature, const int32_t* top_k, const float* top_p,
                             const float* min_p, const int32_t* token_num, int32_t rows_per, int32_t* ids,

@@ -186,6 +186,29 @@ def test_temperatures_that_are_no_numbers_or_have_no_end(pkg, ctx):
     assert int(ids[3]) == 750 and abs(float(lp[3]) + np.log(3000.0)) < 1e-6  # all weights are one: the 751st sum is the first above 750
 
 
+@pytest.mark.parametrize("vocab", [1000, 1 << 18])
+def test_many_weights_below_the_last_place_of_the_sum(pkg, ctx, vocab):
+    """Weights of 2^-45.2 round to zero, of 2^-44.4 to 2^-44: the sums are off by n 2^-45 at most, and so is the share."""
+    for nats in (31.32, 30.78):
+        x = torch.full((2, vocab), -nats, device="cuda")
+        x[:, vocab // 2] = 0.0
+        ids, lp = pkg.sample_tokens(ctx, x, torch.full((2,), 0.5, device="cuda"))
+        want = -np.log1p((vocab - 1) * np.exp(float(x[0, 0])))
+        assert ids.tolist() == [vocab // 2] * 2
+        assert (np.abs(lp.double().cpu().numpy() - want) <= vocab * 2.0 ** -45 + 1e-11).all()
+
+
+def test_temperatures_past_the_largest(pkg, ctx):
+    """They count as 1e30: what a mask of the type's lowest value hides stays hidden in 32 bits."""
+    x, u = make(6, 2000, torch.float32, seed=3)
+    x[:, ::3] = torch.finfo(torch.float32).min
+    t = torch.tensor([1e30, 2e30, 1e36, 3e38, float("inf"), 1e29], device="cuda")
+    ids, lp = pkg.sample_tokens(ctx, x, u, temperature=t)
+    kept = torch.arange(2000, device="cuda")[torch.arange(2000, device="cuda") % 3 != 0]
+    assert torch.equal(ids.long(), kept[(u.double() * len(kept)).long()])
+    assert torch.allclose(lp, torch.full_like(lp, -np.log(len(kept))), rtol=1e-6)
+
+
 @pytest.mark.parametrize("dtype, rows", [(torch.float32, 9), (torch.float16, 9), (torch.bfloat16, 9), (torch.float16, 300), (torch.bfloat16, 300)])
 def test_a_cut_just_below_zero(pkg, ctx, dtype, rows):
     """Zeros of both signs above the cut, the least negative values at and below it: bins of keys that end right below zero

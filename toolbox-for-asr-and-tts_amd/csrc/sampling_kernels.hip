@@ -633,7 +633,7 @@ struct Sampler {
 
     __device__ __forceinline__ void run(int r) {
         SampleLds<NT>& s = sample_lds<NT>();
-        const float given = p.temperature ? p.temperature[r] : 1.0f, temp = fminf(given, 1e30f);  // (beyond it all weights are one as well)
+        const float given = p.temperature ? p.temperature[r] : 1.0f, temp = fminf(given, 1e30f);  // (as documented; only logits past 1e20 would see a difference)
         const bool greedy = !(given > 0.0f);  // (NaN, too)
         double power[1024 / NT];  // on their way while the maximum is found
 #pragma unroll

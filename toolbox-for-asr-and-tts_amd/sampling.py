@@ -37,8 +37,8 @@ def sample_tokens(ctx: _lib.Context, logits: torch.Tensor, u: torch.Tensor, temp
     Weights are exp((l - max l) / temperature).  In the order of falling logits (equal ones by rising index) the first ``top_k``
     are kept (<= 0: all), of those the shortest prefix with at least ``top_p`` of their weight, of those the ones with at
     least ``min_p`` of the largest weight, and always the first; the id is the lowest one at which the running sum of the
-    kept weights exceeds ``u`` times their sum.  A temperature that is not above zero takes the arg-max.  Every setting is one
-    number (u, too), a tensor [rows] or None.  NaN logits count as -inf; a row with nothing above -inf gives id 0 and logprob -inf.
+    kept weights exceeds ``u`` times their sum.  A temperature that is not above zero takes the arg-max, one
+    above 1e30 counts as 1e30.  Every setting is one number (u, too), a tensor [rows] or None.  NaN logits count as -inf; a row with nothing above -inf gives id 0 and logprob -inf.
     ``token_num`` [rows / n] int32: of every n rows the ones behind an utterance's tokens get id -1 and logprob 0."""
     if not logits.is_cuda or logits.dtype not in _DT or logits.dim() != 2 or not 1 <= logits.shape[1] <= MAX_VOCAB:
         raise ValueError(f"sample_tokens: logits must be a float32, float16 or bfloat16 CUDA tensor [rows, 1 .. {MAX_VOCAB}]")
