@@ -274,7 +274,8 @@ struct RowMask {
 // Bound by instruction issue: 64 scores cost 32 cycles of matrix instructions at 128 channels (16 at 64), an exponential of 16
 // and some 20 cycles of other vector work.  Two chunks of 2048 tokens over 16 k positions, 16 heads of 128 on 4: 441 us, 970
 // TFLOP/s (an 8192-cubed library product: 1296), 539 us from an 8-bit cache, whose tiles every workgroup converts; heads of
-// 64: 261 us and 717 TFLOP/s for 4 prompts of up to 4096 over 6000, 113 us under a window of 1024.  (Cards differ: 474, 562, 276
+// 64: 261 us and 717 TFLOP/s for 4 prompts of up to 4096 over 6000, 113 us under a window of 1024; 64 sequences of up to 8192
+// positions with 16 new tokens each, 32 heads on 8 of 128, 273 us.  (Cards differ: 474, 562, 276
 // and 117 us on the slowest one met.)
 template <int D, bool E4M3>
 struct ManyShape {
@@ -675,7 +676,7 @@ __global__ __launch_bounds__(256, (D == 64 && !E4M3 ? 3 : 2)) void paged_attn_ma
 // either half of the tile, for row lane % 16: taken in this order they are the second operand of O^T = V^T P^T as they are.
 //
 // Bound by memory: 64 sequences of up to 8192 positions, 32 heads on 8 of 128: 219 us and 5.4 TB/s in 16 bits, 132 us in 8
-// (4.5 TB/s), 273 us with 16 new tokens each; 8 sequences of up to 131072 in 8 bits 95 us, 4.5 TB/s; 256 chunks of 10 frames
+// (4.5 TB/s); 8 sequences of up to 131072 in 8 bits 95 us, 4.5 TB/s; 256 chunks of 10 frames
 // under a window of 50 13.5 us in 16 bits, 12.5 us in 8.
 template <int D, bool E4M3, int NQ, int KW>
 struct FewShape {
