@@ -341,7 +341,8 @@ int32_t asrfe_kv_read(asrfe_ctx* ctx, const asrfe_kv_cache* cache, const int32_t
  * strides multiples of 8 (out's rows must not overlap), bases 16-byte aligned, of `dtype` (F16 or BF16; the cache's own for a 16-bit cache).
  * n_q_heads: a multiple of n_heads.  max_kv: an upper bound of kv_lens (it shapes the launch; positions past it are not
  * seen).  Scores, softmax statistics and sums are fp32; the weights p enter their product in `dtype`, rounded
- * by at most half a step each and in F16 by at most 2^-34 of the row's largest (a smaller one counts in the sum alone).
+ * by at most half a step each and in F16 by at most 2^-34 of the row's largest (a smaller one counts in the sum alone); a
+ * weight is up to 2^8 in a sum until that is divided, so a sum of BF16 values past 1e30 may overflow.
  * workspace: >= asrfe_paged_attention_workspace_bytes(...) of the same numbers, 256-byte aligned, of this call alone
  * until it has run (a captured graph keeps using the one it was captured with). */
 int64_t asrfe_paged_attention_workspace_bytes(const asrfe_ctx* ctx, const asrfe_kv_cache* cache, int32_t n_tokens,

@@ -273,6 +273,31 @@ def test_values_that_are_infinite_count_however_small_their_weight(pkg, ctx, nam
         check_attend(part, q[a:a + int(s.nq[b])], out[a:a + int(s.nq[b])], **kw)
 
 
+@pytest.mark.parametrize("name", SEEN)
+def test_large_values_left_behind_leave_nothing(pkg, ctx, name):
+    """Values of 1e36 under weights that a later score makes e^-110: their sums are brought down by factors that 32 bits do not
+    hold.  What is left of them may be 2^-149 each.  (A weight may be 2^8 before that: larger values could overflow.)"""
+    lens, kw = SEEN[name]
+    s = Setup(pkg, ctx, lens, BF16, None, 128, 2, 32, seed=len(name))
+    c, q = s.cache, s.rows(s.n, 4, 0.1)
+    q[..., 0] = 16.0
+    c.k[..., 0] = 0.0
+    n, m = lens[0]
+    first = max(0, n - m - kw.get("window", n) + 2)
+    at = [first + (n - m - first) * i // 5 for i in (0, 1, 3)]
+    for i, p in enumerate(at):
+        page = int(s.table[0, p // 32])
+        c.k[page, :, p % 32, 0] = 110 * 128 ** 0.5 / 16 if i == 2 else 0.0
+        if i < 2:
+            c.v[page, :, p % 32, i::7] = (1e36, -1e36)[i]
+    out = c.attend(q, *s.plan(), **kw)
+    k, v = values_of(c, "k"), values_of(c, "v")
+    want, absv, reach, _ = po.attend(q[:m].double().cpu().numpy(), k, v, [0, m], [n], s.table[:1], 32, **kw)
+    tol = bound(BF16, 128, n, want, absv, reach, 0.0) + 1e36 * 2.0 ** -149 * 4
+    err = np.abs(out[:m].double().cpu().numpy() - want)
+    assert (err <= tol).all(), float((err / tol).max())
+
+
 @pytest.mark.parametrize("store", [None, E4M3], ids=["16", "e4m3"])
 @pytest.mark.parametrize("lens", [[(4003, 1)], [(4003, 25), (900, 3)], [(2100, 100)] * 60], ids=["token", "chunk", "tiles of 128"])
 @pytest.mark.parametrize("nats", [9, 13, 16, 18, 21])

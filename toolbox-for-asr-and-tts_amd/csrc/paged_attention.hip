@@ -12,7 +12,8 @@
 //   lane holds the scores of one row; the weights are then already laid out as the operand of O^T = V^T P^T, V being read
 //   transposed from the LDS.  Tiles arrive by 16-byte global -> LDS loads (16-bit caches) with the bank swizzle applied to
 //   the source address, or through registers, where e4m3 codes become 16-bit values (their scales are powers of two: exact
-//   but for fp16 below 2^-14 and past 65504, see dequantise8).  A tile is made of 16-position pieces, each inside one page, so pages may end anywhere in a tile.
+//   but for fp16 below 2^-14 and past 65504, see dequantise8).  A tile is made of 16-position pieces, each inside one page,
+//   so pages may end anywhere in a tile.
 //
 //   Masks.  Only the tiles a mask's edge crosses (the causal diagonal, either end of the window, the end of the sequence,
 //   a page that does not exist) look at positions; there, too, values that are infinite or NaN are kept out of the product
@@ -67,9 +68,9 @@ struct Raised {
     static constexpr float kLag = F16 ? 6.0f : 8.0f, kRaise = F16 ? 9.0f : 0.0f;
 };
 
-// What brings sums from one reference to another.  Never zero: an infinite sum stays infinite (and 2^-126 of a finite one is
-// less than any rounding leaves).
-__device__ __forceinline__ float factor(float from, float to) { return fmaxf(__builtin_amdgcn_exp2f(from - to), 0x1p-126f); }
+// What brings sums from one reference to another.  Never zero: an infinite sum stays infinite.  (2^-149, the least there is, of a
+// finite one: at most 5e-7, from values at the end of bf16's range; 2^-126 would leave 4.)
+__device__ __forceinline__ float factor(float from, float to) { return fmaxf(__builtin_amdgcn_exp2f(from - to), 0x1p-149f); }
 
 // 1 / a sum of weights; 0 where there were none, NaN where a score was
 __device__ __forceinline__ float inverse(float sum) { return sum > 0.0f ? 1.0f / sum : (sum == 0.0f ? 0.0f : sum); }
@@ -275,8 +276,7 @@ struct RowMask {
 // and some 20 cycles of other vector work.  Two chunks of 2048 tokens over 16 k positions, 16 heads of 128 on 4: 441 us, 970
 // TFLOP/s (an 8192-cubed library product: 1296), 539 us from an 8-bit cache, whose tiles every workgroup converts; heads of
 // 64: 261 us and 717 TFLOP/s for 4 prompts of up to 4096 over 6000, 113 us under a window of 1024; 64 sequences of up to 8192
-// positions with 16 new tokens each, 32 heads on 8 of 128, 273 us.  (Cards differ: 474, 562, 276
-// and 117 us on the slowest one met.)
+// positions with 16 new tokens each, 32 heads on 8 of 128, 273 us.  (Cards differ: 474, 562, 276, 117 and 289 us on the slowest.)
 template <int D, bool E4M3>
 struct ManyShape {
     static constexpr int kKeys = 64, kRowTile = 128;
@@ -676,8 +676,8 @@ __global__ __launch_bounds__(256, (D == 64 && !E4M3 ? 3 : 2)) void paged_attn_ma
 // either half of the tile, for row lane % 16: taken in this order they are the second operand of O^T = V^T P^T as they are.
 //
 // Bound by memory: 64 sequences of up to 8192 positions, 32 heads on 8 of 128: 219 us and 5.4 TB/s in 16 bits, 132 us in 8
-// (4.5 TB/s); 8 sequences of up to 131072 in 8 bits 95 us, 4.5 TB/s; 256 chunks of 10 frames
-// under a window of 50 13.5 us in 16 bits, 12.5 us in 8.
+// (4.5 TB/s); 8 sequences of up to 131072 in 8 bits 95 us, 4.5 TB/s; 256 chunks of 10 frames under a window of 50 13.5 us in 16
+// bits, 12.5 us in 8.
 template <int D, bool E4M3, int NQ, int KW>
 struct FewShape {
     static constexpr int kRowBytes = 2 * D;
