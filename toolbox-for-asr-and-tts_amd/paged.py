@@ -6,9 +6,8 @@ cache of its own.  ``PagedKvCache`` is what a streaming or autoregressive model 
 ``ParaformerHead``: pages of ``page_size`` positions in one pool, a table of page numbers per sequence, 16-bit storage or
 e4m3 bytes with a power-of-two scale per position and head.  One step is ``append`` (the new positions' keys and values go
 into their pages) and ``attend`` (the new queries attend to everything their sequence holds); ``read`` gives dense copies
-back.  Everything runs on the device through libasrfe; there is no CPU path.
-An e4m3 value takes part as what the queries' type has of it: exactly in bfloat16, in float16 rounded below 2 ** -14 and kept
-inside +-65504.
+back.  Everything runs on the device through libasrfe; there is no CPU path.  An e4m3 value takes part as what the
+queries' type has of it: exactly in bfloat16, in float16 rounded below 2 ** -14 and kept inside +-65504.
 
 A batch is described by three int32 device tensors: ``cu_q`` [B + 1] (rows of the packed new tokens), ``kv_lens`` [B] (positions
 of every sequence, the new ones included: they are its last) and ``block_table`` [B, n] (page numbers; -1 where there is no
@@ -145,7 +144,9 @@ class PagedKvCache:
         ``window`` > 0 keeps the last ``window`` up to its own, and the first ``sinks`` stay visible beside them.  A row
         that sees nothing is zero; rows behind cu_q[B] are not written (those of a new tensor hold no meaning).  ``scale``
         defaults to 1 / sqrt(head_dim); ``max_kv`` bounds kv_lens (the table's width unless given: a tighter bound shapes
-        the launch better)."""
+        the launch better).  Statistics and sums are fp32, the weights enter their product in q's type; infinities and NaN
+        reach the rows that see them and no other.  A call's work is cut by its mean: single tokens over very long caches are
+        better off in a call of their own than beside a long prompt."""
         self._plan("attend", kv_lens, block_table, cu_q)
         qts, qhs = self._rows("attend", "q", q, None)
         n, heads, dim = q.shape
