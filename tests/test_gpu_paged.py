@@ -553,6 +553,36 @@ def test_few_heads_share_a_wave(pkg, ctx, heads, dim, store):
         np.testing.assert_array_equal(values_of(s.cache, name), x)
 
 
+@pytest.mark.parametrize("store", [None, E4M3], ids=["16", "e4m3"])
+@pytest.mark.parametrize("heads", [1, 8])
+def test_thousands_of_sequences(pkg, ctx, heads, store):
+    """The search for a row's sequence takes three steps; many sequences have no new rows, the first and the last among them."""
+    rng = np.random.default_rng(heads)
+    batch = 9001 if heads == 1 else 4500
+    kv = rng.integers(0, 34, batch)
+    q = np.minimum(kv, rng.choice([0, 0, 1, 2, 7], batch))
+    q[:70] = q[-70:] = 0
+    s = Setup(pkg, ctx, list(zip(kv.tolist(), q.tolist())), F16, store, 64, heads, 16, seed=heads)
+    k, v = s.rows(s.n + 3, heads), s.rows(s.n + 3, heads)
+    want = [values_of(s.cache, x) for x in "kv"]
+    s.cache.append(k, v, *s.plan())
+    for x, new in zip(want, (k, v)):
+        new = new.double().cpu().numpy()
+        new = po.dequantise(*po.quantise(new)) if store else new
+        for t, b, p in po.new_positions(s.cu, s.kv):
+            x[s.table[b, p // 16], :, p % 16] = new[t]
+    for x, name in zip(want, "kv"):
+        np.testing.assert_array_equal(values_of(s.cache, name), x)
+    queries = s.rows(s.n + 3, 2 * heads)
+    out = torch.full_like(queries, 7.0)
+    s.cache.attend(queries, *s.plan(), out=out)
+    check_attend(s, queries, out, untouched=7.0)
+    got = s.cache.read(i32(s.kv), i32(s.table), 3)
+    for x, t in zip(want, got):
+        dense = np.stack([po.dense(x, s.table, 16, b, 3)[0] * (np.arange(3) < s.kv[b])[:, None, None] for b in range(batch)])
+        np.testing.assert_array_equal(t.double().cpu().numpy(), dense)
+
+
 def test_append_of_bad_pages_writes_nothing(pkg, ctx):
     s = Setup(pkg, ctx, [(40, 40), (20, 20)], F16, None, 64, 2, 16, seed=4)
     s.table[0, 1], s.table[1, 0] = -1, 1 << 29
