@@ -440,6 +440,41 @@ def test_attend_far_offsets(pkg, ctx):
     assert torch.equal(a[0], b[0]) and torch.equal(a[1], b[1])
 
 
+@pytest.mark.parametrize("store", [None, E4M3], ids=["16", "e4m3"])
+@pytest.mark.parametrize("rows", [(3, 1), (40, 3), (320, 4)], ids=["tokens", "chunk", "tiles of 128"])
+def test_far_rows_and_far_pages(pkg, ctx, rows, store):
+    """Rows of every operand 32 MiB apart (past 4 GiB with 320 of them), in pages past 4 GiB into each pool: as near ones."""
+    new, group = rows
+    page, heads, dim, kv = 256, 8, 128, 600
+    assert new < 300 or repeats([(kv, new)], heads, group, bool(store), 256) == 1
+    n_pages = (1 << 32) // (page * heads * dim * (1 if store else 2)) + 300
+    s = Setup(pkg, ctx, [(kv, new), (300, 1)], BF16, store, dim, heads, page, seed=new)
+    far = pkg.PagedKvCache.allocate(ctx, n_pages, page, heads, dim, store or BF16)
+    table = np.where(s.table >= 0, n_pages - 1 - 37 * s.table, -1)
+    for name in ("k", "v") + (("k_exp", "v_exp") if store else ()):
+        a, b = getattr(far, name).view(torch.uint8), getattr(s.cache, name).view(torch.uint8)
+        for x, y in zip(table.reshape(-1), s.table.reshape(-1)):
+            if y >= 0:
+                a[int(x)] = b[int(y)]
+    wide = torch.zeros(s.n << 24, dtype=BF16, device="cuda").view(s.n, 1 << 24)
+    cu, lens, near_table = s.plan()
+
+    def apart(n_heads, place):
+        return wide[:, place << 16:(place << 16) + n_heads * dim].view(s.n, n_heads, dim)
+
+    q, k, v, out = apart(heads * group, 0), apart(heads, 1), apart(heads, 2), apart(heads * group, 3)
+    for t in (q, k, v):
+        t.copy_(s.rows(s.n, t.shape[1]))
+    far.append(k, v, cu, lens, i32(table))
+    s.cache.append(k.contiguous(), v.contiguous(), cu, lens, near_table)
+    far.attend(q, cu, lens, i32(table), out=out)
+    assert torch.equal(out, s.cache.attend(q.contiguous(), cu, lens, near_table))
+    for a, b in zip(far.read(lens, i32(table), kv, dtype=BF16), s.cache.read(lens, near_table, kv, dtype=BF16)):
+        assert torch.equal(a, b)
+    assert not bool(wide[:, 1 << 18:].any())
+    check_attend(s, q, out)
+
+
 # ---- writing and reading back -----------------------------------------------------------------------------------------------
 @pytest.mark.parametrize("dtype, store, dim", [(F16, None, 64), (BF16, None, 128), (F16, E4M3, 128), (BF16, E4M3, 64)],
                          ids=["f16", "bf16", "f16-e4m3", "bf16-e4m3"])

@@ -165,6 +165,17 @@ def test_many_rows(pkg, ctx, rows, vocab, dtype):
           min_p=pick(0.0, 0.0, 0.02, 0.2))
 
 
+def test_rows_far_apart(pkg, ctx):
+    """Rows a gigabyte apart, the last ones past 8 GiB, give what they give side by side."""
+    x, u = make(10, 9001, torch.float32, seed=21)
+    far = torch.zeros(10 << 28, device="cuda").view(10, 1 << 28)[:, 3:9004]
+    far.copy_(x)
+    for settings in (dict(top_k=40, top_p=0.9), dict(top_p=0.97), dict(temperature=0.0), dict(min_p=0.01)):
+        check(pkg, ctx, far, u, **settings)
+        for a, b in zip(pkg.sample_tokens(ctx, far, u, **settings), pkg.sample_tokens(ctx, x, u, **settings)):
+            assert torch.equal(a, b)
+
+
 def test_numbers_at_the_ends(pkg, ctx):
     """u = 0 takes the first kept token; a number outside [0, 1), which no generator gives, takes an end instead of running on."""
     x, _ = make(5, 900, torch.float32, seed=8)
