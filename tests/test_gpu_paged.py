@@ -711,6 +711,57 @@ def test_attend_and_append_on_another_stream_and_in_graphs(pkg, ctx):
         assert all(torch.equal(x, want[i]) for x in got[i])
 
 
+@pytest.mark.parametrize("store", [None, E4M3], ids=["16", "e4m3"])
+@pytest.mark.parametrize("kw", [{}, dict(window=100, sinks=5), dict(causal=False)], ids=["plain", "window", "whole"])
+@pytest.mark.parametrize("n, heads, group, width", [(4, 2, 4, 200), (60, 2, 1, 60), (300, 8, 4, 90), (200, 1, 2, 500)],
+                         ids=["tokens", "chunks", "prompts", "prompts in parts"])
+def test_a_captured_step_follows_its_buffers(pkg, ctx, n, heads, group, width, kw, store):
+    """One graph of append, attend and read back, replayed while the batch in its buffers changes: other lengths, other shares of the rows, empty
+    sequences, rows that belong to nobody, pages given back.  Every replay equals an eager call on the same buffers, and the
+    definition."""
+    s = Setup(pkg, ctx, [(16 * width, n // 4)] * 4, F16, store, 64, heads, 16, seed=n)
+    c, (cu, lens, table) = s.cache, s.plan()
+    full = s.table.copy()
+    q, k, v = s.rows(n, heads * group), s.rows(n, heads), s.rows(n, heads)
+    out = torch.zeros_like(q)
+
+    def step():
+        c.append(k, v, cu, lens, table)
+        c.attend(q, cu, lens, table, out=out, **kw)
+        return c.read(lens, table, 40)
+
+    side = torch.cuda.Stream()
+    with torch.cuda.stream(side):
+        step()
+    side.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        held = step()
+    rng = np.random.default_rng(n)
+    for r in range(5):
+        last = n - (0, 3)[r % 2]
+        s.cu = np.minimum([0, *np.sort(rng.integers(0, n + 1, 3)), last], last) if r else np.array([0, 0, n // 2, n // 2, n])
+        s.nq = np.diff(s.cu)
+        s.kv = rng.integers(0, 16 * width + 1, 4)
+        s.kv[r % 4] = s.nq[r % 4]
+        s.n = int(s.cu[-1])
+        s.table = np.where(rng.random(full.shape) < (0.1 if r == 3 else 0.0), -1, full)
+        for t, x in ((cu, s.cu), (lens, s.kv), (table, s.table)):
+            t.copy_(i32(x))
+        for t in (q, k, v):
+            t.copy_(s.rows(n, t.shape[1]))
+        out.fill_(7.0)
+        torch.cuda.synchronize()
+        graph.replay()
+        torch.cuda.synchronize()
+        got, pages = out.clone(), [t.clone() for t in held]
+        out.fill_(7.0)
+        eager = step()
+        assert torch.equal(got, out) and all(torch.equal(a, b) for a, b in zip(pages, eager))
+        assert bool((got[s.n:] == 7).all())
+        check_attend(s, q[:s.n], got[:s.n], **kw)
+
+
 def test_python_refusals(pkg, ctx):
     s = Setup(pkg, ctx, [(20, 2)], F16, None, 64, 2, 16)
     c, (cu, lens, table), q = s.cache, s.plan(), s.rows(2, 4)
